@@ -300,6 +300,108 @@ size_t lfm25_splitk_decode_splits(size_t num_tokens, size_t maximum_context_toke
 int32_t lfm25_decode_one_kernel_preferred(size_t page_size, size_t context_tokens, size_t batch_size);
 
 /* ------------------------------------------------------------------------------------------
+ * 8-bit paged KV cache
+ * ------------------------------------------------------------------------------------------
+ * Keys and values as E4M3 codes with one scale for each page of 16 tokens and KV head: an element stands for
+ * code * scale.  A scale is the smallest power of two, 2^-126 at least, under which the largest finite magnitude that
+ * the page's tokens of this head brought is at most 448; a page that was never written may hold anything.  No
+ * counterpart in the reference, whose cache is bf16.  Heads of 64 or 128, any number of KV heads (up to 1024) and of
+ * query heads to each.  Code buffers, activations and norms are 16-byte aligned; token strides are counted in
+ * elements, 0 = dense, else a multiple of 8.  No entry point needs a workspace. */
+
+typedef struct lfm25_e4m3_cache {
+    size_t page_size;          /* 16 (32 is rejected with LFM25_ERR_UNSUPPORTED) */
+    size_t num_pages;
+    size_t kv_heads;
+    size_t head_dim;           /* 64 or 128 */
+    lfm25_slice key_codes;     /* u8 [num_pages, kv_heads, 16, head_dim] */
+    lfm25_slice value_codes;
+    lfm25_slice key_scales;    /* f32 [num_pages, kv_heads] */
+    lfm25_slice value_scales;
+} lfm25_e4m3_cache;
+
+/* Appends the keys and values of a step.  Consecutive tokens with consecutive slots within a page are one run; a run at
+ * the page's first token sets the page's scales, whatever was there, one further on raises them where it has to and
+ * rounds the codes in front of it to the larger scale (codes behind it are left alone).  A page takes one run a call: two
+ * that meet in a page (a skipped token in between ends a run), like two tokens with the same slot, leave it undefined, and
+ * so does a page that other sequences share (fork it first, lfm25_kv_allocator_fork_sequence).  Infinities become the
+ * largest code, NaN the NaN code; neither moves a scale. */
+typedef struct lfm25_kv_cache_write_e4m3_launch {
+    lfm25_e4m3_cache cache;    /* written */
+    lfm25_slice key;           /* bf16 [num_tokens, kv_heads, head_dim] */
+    lfm25_slice value;
+    lfm25_slice slot_mapping;  /* i64 [num_tokens]; < 0 or page >= num_pages skips the token */
+    size_t num_tokens;
+    size_t kv_token_stride;
+} lfm25_kv_cache_write_e4m3_launch;
+int32_t lfm25_kv_cache_write_e4m3(void* stream, const lfm25_kv_cache_write_e4m3_launch* launch);
+
+/* The same with RMS norm and rotation of queries and keys in front (what lfm25_qk_norm_rope_kv_write_decode does for
+ * the bf16 cache): y = x / sqrt(mean(x^2) + eps) * w, then (y[d], y[d + head_dim / 2]) turned by position * inv_freq[d].
+ * All in f32, the angle in f64; queries are rounded once, to bf16, keys once, to E4M3.  Queries of tokens without a
+ * slot are written as well. */
+typedef struct lfm25_qk_norm_rope_kv_write_e4m3_launch {
+    lfm25_e4m3_cache cache;    /* written */
+    lfm25_slice query;         /* bf16 [num_tokens, query_heads, head_dim] */
+    lfm25_slice query_out;     /* bf16 [num_tokens, query_heads, head_dim], dense; may be `query` itself where that is dense */
+    lfm25_slice key;           /* bf16 [num_tokens, kv_heads, head_dim] */
+    lfm25_slice value;
+    lfm25_slice query_norm;    /* bf16 [head_dim] */
+    lfm25_slice key_norm;
+    lfm25_slice inv_freq;      /* f32 [head_dim / 2] */
+    lfm25_slice position_ids;  /* u32 [num_tokens] */
+    lfm25_slice slot_mapping;  /* i64 [num_tokens] */
+    size_t num_tokens;
+    size_t query_heads;
+    size_t query_token_stride;
+    size_t kv_token_stride;
+    float eps;
+} lfm25_qk_norm_rope_kv_write_e4m3_launch;
+int32_t lfm25_qk_norm_rope_kv_write_e4m3(void* stream, const lfm25_qk_norm_rope_kv_write_e4m3_launch* launch);
+
+/* Attention over the cache, softmax(scale * q k) v, over the keys j <= position of the token's sequence with
+ * window == 0, j > position - window or j < sinks.  Pages between the first tokens and the window are not looked at
+ * (lfm25_kv_allocator_release_window gives them back).  A token whose request slot or position lies outside the block
+ * tables, or that sees an unassigned page, keeps the output row that was passed in. */
+typedef struct lfm25_paged_attention_e4m3_launch {
+    lfm25_e4m3_cache cache;
+    lfm25_slice query;           /* bf16 [num_tokens, query_heads, head_dim] */
+    lfm25_slice block_tables;    /* u32 [rows, block_table_stride] */
+    lfm25_slice request_slots;   /* u32 [num_tokens] */
+    lfm25_slice position_ids;    /* u32 [num_tokens] */
+    lfm25_slice output;          /* bf16 [num_tokens, query_heads, head_dim], dense, written */
+    size_t num_tokens;
+    size_t query_heads;          /* a multiple of kv_heads: head h reads KV head h / (query_heads / kv_heads) */
+    size_t query_token_stride;
+    size_t block_table_stride;
+    size_t window;               /* 0: none */
+    size_t sinks;
+    size_t maximum_context_tokens;  /* of the batch, 0: not known.  Chooses how the work is split, not what is computed */
+    float scale;                 /* finite and positive */
+    lfm25_slice token_order;     /* single tokens only, optional: as in lfm25_fast_ragged_attention_launch */
+    lfm25_slice segment_offsets; /* prompts only: u32 [num_segments + 1] */
+    size_t num_segments;         /* prompts only */
+} lfm25_paged_attention_e4m3_launch;
+/* Single tokens, each by itself: a decode step. */
+int32_t lfm25_paged_attention_e4m3(void* stream, const lfm25_paged_attention_e4m3_launch* launch);
+/* Portions of prompts, whose own keys were appended before: the tokens segment_offsets[s] .. segment_offsets[s + 1] sit at
+ * consecutive positions of one request slot; tokens outside every segment, and tokens that do not continue their
+ * segment's first, keep their output row. */
+int32_t lfm25_paged_prompt_attention_e4m3(void* stream, const lfm25_paged_attention_e4m3_launch* launch);
+
+/* Copies pages of caches: page source_pages[i] of every arena goes to page destination_pages[i] of the same arena.  An
+ * arena is one buffer of pages one behind the other (keys, values or scales of a layer, bf16 or 8-bit); one call takes all
+ * layers.  Destinations are distinct and none of them a source; a pair with a page that an arena does not have is skipped
+ * there. */
+typedef struct lfm25_page_arena {
+    void* base;                  /* 4-byte aligned; 16-byte aligned pages of a multiple of 16 bytes are copied fastest */
+    size_t page_bytes;           /* a multiple of 4 */
+    size_t num_pages;
+} lfm25_page_arena;
+int32_t lfm25_kv_pages_copy(void* stream, const lfm25_page_arena* arenas, size_t num_arenas, lfm25_slice source_pages,
+                            lfm25_slice destination_pages, size_t num_pairs); /* u32 [num_pairs] on the device */
+
+/* ------------------------------------------------------------------------------------------
  * FP8 (E4M3) producers
  * ------------------------------------------------------------------------------------------ */
 
@@ -815,6 +917,22 @@ int64_t lfm25_kv_allocator_pages_short(const lfm25_kv_allocator* allocator, cons
                                        const size_t* target_tokens, size_t sequences);
 void lfm25_kv_allocator_release_sequence(lfm25_kv_allocator* allocator, size_t tokens, uint32_t* block_table,
                                          size_t block_table_len);
+/* Copying, forking, compacting and freeing pages (no counterpart in the reference).
+ * fork_sequence: block_table becomes a second sequence over the first `tokens` tokens of source_table.  Full pages are
+ * shared, a last, partly filled one gets a page of its own: copy_pages = {source, destination} then, to be copied with
+ * lfm25_kv_pages_copy before either sequence is appended to.  Returns the number of pages to copy (0 or 1).  The entries
+ * that are filled must be unassigned before; on an error nothing has changed.
+ * release_window: gives back the pages that no later token sees, with `tokens` tokens cached, a window and first tokens that
+ * stay visible (the rule of lfm25_paged_attention_e4m3); their entries become unassigned.  Returns their number.
+ * compact: moves pages with high numbers to free ones with low numbers and rewrites `entries` block table entries (all rows of all
+ * live sequences).  Only pages whose every reference is in these entries move: those that a prefix cache holds stay.
+ * source_pages / destination_pages take up to `capacity` moves, to be copied with lfm25_kv_pages_copy.  Returns their number. */
+int64_t lfm25_kv_allocator_fork_sequence(lfm25_kv_allocator* allocator, size_t tokens, const uint32_t* source_table,
+                                         uint32_t* block_table, size_t block_table_len, uint32_t copy_pages[2]);
+int64_t lfm25_kv_allocator_release_window(lfm25_kv_allocator* allocator, size_t tokens, size_t window, size_t sinks,
+                                          uint32_t* block_table, size_t block_table_len);
+int64_t lfm25_kv_allocator_compact(lfm25_kv_allocator* allocator, uint32_t* block_tables, size_t entries,
+                                   uint32_t* source_pages, uint32_t* destination_pages, size_t capacity);
 void lfm25_kv_allocator_snapshot(const lfm25_kv_allocator* allocator, lfm25_kv_pool_snapshot* out);
 
 /* Replaces FixedBlockTables (src/cache/block_table.rs:3-31): u32 [slots, pages_per_slot], 0xffffffff = unassigned. */

@@ -60,7 +60,18 @@ FastRaggedAttentionLaunch = _launch_struct("FastRaggedAttentionLaunch", [
 SplitKRaggedAttentionLaunch = _launch_struct("SplitKRaggedAttentionLaunch", [
     "#page_size", "query", "key_cache", "value_cache", "block_tables", "request_slots", "position_ids",
     "partials", "output", "#num_tokens", "#num_pages", "#block_table_stride", "#num_splits", "token_order"])
-
+E4m3Cache = _launch_struct("E4m3Cache", [
+    "#page_size", "#num_pages", "#kv_heads", "#head_dim", "key_codes", "value_codes", "key_scales", "value_scales"])
+KvCacheWriteE4m3Launch = _launch_struct("KvCacheWriteE4m3Launch", [
+    ("cache", E4m3Cache), "key", "value", "slot_mapping", "#num_tokens", "#kv_token_stride"])
+QkNormRopeKvWriteE4m3Launch = _launch_struct("QkNormRopeKvWriteE4m3Launch", [
+    ("cache", E4m3Cache), "query", "query_out", "key", "value", "query_norm", "key_norm", "inv_freq", "position_ids",
+    "slot_mapping", "#num_tokens", "#query_heads", "#query_token_stride", "#kv_token_stride", ("eps", ctypes.c_float)])
+PagedAttentionE4m3Launch = _launch_struct("PagedAttentionE4m3Launch", [
+    ("cache", E4m3Cache), "query", "block_tables", "request_slots", "position_ids", "output", "#num_tokens", "#query_heads",
+    "#query_token_stride", "#block_table_stride", "#window", "#sinks", "#maximum_context_tokens", ("scale", ctypes.c_float),
+    "token_order", "segment_offsets", "#num_segments"])
+PageArena = _launch_struct("PageArena", [("base", ctypes.c_void_p), "#page_bytes", "#num_pages"])
 
 
 _P = ctypes.POINTER
@@ -265,6 +276,11 @@ PROTOTYPES = {
     "lfm25_decode_one_kernel_preferred": (ctypes.c_int32, [_size, _size, _size]),
     "lfm25_bf16_own_kernel_max_rows": (_size, []),
     "lfm25_blaslt_library_calls": (ctypes.c_uint64, []),
+    "lfm25_kv_cache_write_e4m3": (ctypes.c_int32, [_stream, _P(KvCacheWriteE4m3Launch)]),
+    "lfm25_qk_norm_rope_kv_write_e4m3": (ctypes.c_int32, [_stream, _P(QkNormRopeKvWriteE4m3Launch)]),
+    "lfm25_paged_attention_e4m3": (ctypes.c_int32, [_stream, _P(PagedAttentionE4m3Launch)]),
+    "lfm25_paged_prompt_attention_e4m3": (ctypes.c_int32, [_stream, _P(PagedAttentionE4m3Launch)]),
+    "lfm25_kv_pages_copy": (ctypes.c_int32, [_stream, _P(PageArena), _size, Slice, Slice, _size]),
     "lfm25_quantize_bf16_e4m3": (ctypes.c_int32, [_stream, Slice, Slice, _size, ctypes.c_float]),
     "lfm25_silu_mul_packed_bf16": (ctypes.c_int32, [_stream, Slice, Slice, _size, _size]),
     "lfm25_silu_mul_packed_bf16_to_e4m3": (ctypes.c_int32, [_stream, Slice, Slice, _size, _size, ctypes.c_float]),
@@ -329,6 +345,12 @@ PROTOTYPES = {
     "lfm25_kv_allocator_grow_sequence": (ctypes.c_int64, [ctypes.c_void_p, _size, _size, _P(ctypes.c_uint32), _size]),
     "lfm25_kv_allocator_pages_short": (ctypes.c_int64, [ctypes.c_void_p, _P(_size), _P(_size), _size]),
     "lfm25_kv_allocator_release_sequence": (None, [ctypes.c_void_p, _size, _P(ctypes.c_uint32), _size]),
+    "lfm25_kv_allocator_fork_sequence": (
+        ctypes.c_int64, [ctypes.c_void_p, _size, _P(ctypes.c_uint32), _P(ctypes.c_uint32), _size, _P(ctypes.c_uint32)]),
+    "lfm25_kv_allocator_release_window": (
+        ctypes.c_int64, [ctypes.c_void_p, _size, _size, _size, _P(ctypes.c_uint32), _size]),
+    "lfm25_kv_allocator_compact": (
+        ctypes.c_int64, [ctypes.c_void_p, _P(ctypes.c_uint32), _size, _P(ctypes.c_uint32), _P(ctypes.c_uint32), _size]),
     "lfm25_kv_allocator_snapshot": (None, [ctypes.c_void_p, _P(KvPoolSnapshot)]),
     "lfm25_block_tables_create": (ctypes.c_int32, [_size, _size, _P(ctypes.c_void_p)]),
     "lfm25_block_tables_destroy": (None, [ctypes.c_void_p]),

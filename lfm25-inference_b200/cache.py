@@ -72,6 +72,39 @@ class KvPageAllocator:
         library().lfm25_kv_allocator_release_sequence(self._handle, tokens, _table_pointer(block_table),
                                                       block_table.size)
 
+    def fork_sequence(self, tokens: int, source_table: np.ndarray, block_table: np.ndarray):
+        """`block_table` (its entries unassigned) becomes a second sequence over the first `tokens` tokens of `source_table`:
+        full pages are shared, a partly filled last one gets a page of its own.  Returns (source pages, destination pages) to be
+        copied with `ops.kv_pages_copy` before either sequence is appended to; no counterpart in the reference."""
+        pair = np.zeros(2, dtype=np.uint32)
+        if -(-tokens // 16) > source_table.size:
+            raise KvAllocationError(_abi.KV_SEQUENCE_CAPACITY_EXCEEDED)
+        copies = self._moves(library().lfm25_kv_allocator_fork_sequence(
+            self._handle, tokens, _table_pointer(source_table), _table_pointer(block_table), block_table.size, _table_pointer(pair)))
+        return pair[:copies].copy(), pair[1:1 + copies].copy()
+
+    def release_window(self, tokens: int, window: int, sinks: int, block_table: np.ndarray) -> int:
+        """Gives back the pages of a sequence of `tokens` cached tokens that no later token sees through a window with `sinks`
+        first tokens kept; returns their number.  No counterpart in the reference."""
+        return self._moves(library().lfm25_kv_allocator_release_window(self._handle, tokens, window, sinks, _table_pointer(block_table),
+                                                                       block_table.size))
+
+    def compact(self, block_tables: np.ndarray, maximum_moves: int | None = None):
+        """Moves pages with high numbers to free low ones and rewrites `block_tables` (the tables of all live sequences, any
+        shape).  Returns (source pages, destination pages) to be copied with `ops.kv_pages_copy`.  Pages that somebody else holds as
+        well (a prefix cache) stay.  No counterpart in the reference."""
+        capacity = self.snapshot()["total_pages"] if maximum_moves is None else maximum_moves
+        source, destination = (np.zeros(max(1, capacity), dtype=np.uint32) for _ in range(2))
+        moves = self._moves(library().lfm25_kv_allocator_compact(self._handle, _table_pointer(block_tables), block_tables.size,
+                                                                 _table_pointer(source), _table_pointer(destination), capacity))
+        return source[:moves].copy(), destination[:moves].copy()
+
+    @staticmethod
+    def _moves(value: int) -> int:
+        if _abi.KV_PHYSICAL_PAGES_EXHAUSTED < value < 0:      # an LFM25_ERR_* code, not an allocation error
+            check(int(value))
+        return _count(value)
+
     def snapshot(self) -> dict:
         snapshot = _abi.KvPoolSnapshot()
         library().lfm25_kv_allocator_snapshot(self._handle, ctypes.byref(snapshot))

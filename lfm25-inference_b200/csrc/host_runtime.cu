@@ -173,6 +173,129 @@ void lfm25_kv_allocator_release_sequence(lfm25_kv_allocator* self, size_t tokens
     }
 }
 
+// Gives back one reference of a table's page; an entry that is out of range or already free stays unavailable rather than
+// risking a double free.
+static void drop_reference(lfm25_kv_allocator* self, uint32_t page) {
+    if (page < self->page_refs.size() && self->page_refs[page] != 0 && --self->page_refs[page] == 0) {
+        self->free_pages.push_back(page);
+    }
+}
+
+int64_t lfm25_kv_allocator_fork_sequence(lfm25_kv_allocator* self, size_t tokens, const uint32_t* source_table,
+                                         uint32_t* block_table, size_t block_table_len, uint32_t copy_pages[2]) {
+    if (self == nullptr || source_table == nullptr || block_table == nullptr || copy_pages == nullptr) {
+        return lfm25::report_error(LFM25_ERR_NULL_POINTER, "fork of a sequence received a null pointer");
+    }
+    const size_t pages = div_ceil(tokens, self->page_size);
+    const size_t full = tokens / self->page_size;
+    if (pages > block_table_len) {
+        return LFM25_KV_SEQUENCE_CAPACITY_EXCEEDED;
+    }
+    for (size_t index = 0; index < pages; ++index) {
+        if (block_table[index] != 0xffffffffu) {
+            return lfm25::report_error(LFM25_ERR_INVALID_ARGUMENT, "fork of a sequence into a block table that holds pages");
+        }
+        const uint32_t page = source_table[index];
+        const bool released = index < full && page == 0xffffffffu;   // behind a window
+        if (!released && (page >= self->page_refs.size() || self->page_refs[page] == 0 || self->page_refs[page] == 0xffffffffu)) {
+            return LFM25_KV_PHYSICAL_PAGES_EXHAUSTED;
+        }
+    }
+    if (pages > full && self->free_pages.empty()) {
+        return LFM25_KV_PHYSICAL_PAGES_EXHAUSTED;
+    }
+    for (size_t index = 0; index < full; ++index) {
+        block_table[index] = source_table[index];
+        if (source_table[index] != 0xffffffffu) {
+            self->page_refs[source_table[index]] += 1;
+        }
+    }
+    if (pages == full) {
+        return 0;
+    }
+    const uint32_t page = self->free_pages.back();
+    self->free_pages.pop_back();
+    self->page_refs[page] = 1;
+    block_table[full] = page;
+    copy_pages[0] = source_table[full];
+    copy_pages[1] = page;
+    self->peak_allocated_pages = std::max(self->peak_allocated_pages, self->total_pages - self->free_pages.size());
+    return 1;
+}
+
+int64_t lfm25_kv_allocator_release_window(lfm25_kv_allocator* self, size_t tokens, size_t window, size_t sinks,
+                                          uint32_t* block_table, size_t block_table_len) {
+    if (self == nullptr || block_table == nullptr) {
+        return lfm25::report_error(LFM25_ERR_NULL_POINTER, "release behind a window received a null pointer");
+    }
+    if (window == 0 || tokens < window) {
+        return 0;
+    }
+    // the next token, at position `tokens`, sees the keys from tokens - window + 1 on
+    const size_t end = std::min((tokens - window + 1) / self->page_size, block_table_len);
+    int64_t released = 0;
+    for (size_t index = sinks / self->page_size + (sinks % self->page_size != 0 ? 1 : 0); index < end; ++index) {
+        if (block_table[index] != 0xffffffffu) {
+            drop_reference(self, block_table[index]);
+            block_table[index] = 0xffffffffu;
+            ++released;
+        }
+    }
+    return released;
+}
+
+int64_t lfm25_kv_allocator_compact(lfm25_kv_allocator* self, uint32_t* block_tables, size_t entries, uint32_t* source_pages,
+                                   uint32_t* destination_pages, size_t capacity) {
+    if (self == nullptr || block_tables == nullptr || source_pages == nullptr || destination_pages == nullptr) {
+        return lfm25::report_error(LFM25_ERR_NULL_POINTER, "compaction received a null pointer");
+    }
+    try {
+        std::vector<uint32_t> found(self->total_pages, 0);
+        for (size_t index = 0; index < entries; ++index) {
+            if (block_tables[index] < self->total_pages) {
+                found[block_tables[index]] += 1;
+            }
+        }
+        std::vector<uint32_t> free(self->free_pages);
+        std::sort(free.begin(), free.end());
+        std::vector<uint32_t> moved(self->total_pages, 0xffffffffu);
+        std::vector<uint32_t> left;               // pages that the moves leave free
+        left.reserve(free.size());
+        size_t moves = 0;
+        size_t page = self->total_pages;
+        while (moves < capacity && moves < free.size() && page > 0) {
+            --page;
+            if (page <= free[moves]) {
+                break;
+            }
+            if (self->page_refs[page] == 0 || found[page] != self->page_refs[page]) {
+                continue;
+            }
+            source_pages[moves] = static_cast<uint32_t>(page);
+            destination_pages[moves] = free[moves];
+            moved[page] = free[moves];
+            left.push_back(static_cast<uint32_t>(page));
+            ++moves;
+        }
+        // nothing of the allocator has changed up to here: what follows cannot fail
+        for (size_t index = 0; index < moves; ++index) {
+            self->page_refs[destination_pages[index]] = self->page_refs[source_pages[index]];
+            self->page_refs[source_pages[index]] = 0;
+        }
+        for (size_t index = 0; index < entries; ++index) {
+            if (block_tables[index] < self->total_pages && moved[block_tables[index]] != 0xffffffffu) {
+                block_tables[index] = moved[block_tables[index]];
+            }
+        }
+        left.insert(left.end(), free.begin() + static_cast<ptrdiff_t>(moves), free.end());
+        std::sort(left.begin(), left.end(), [](uint32_t a, uint32_t b) { return a > b; });   // the lowest is handed out first
+        std::copy(left.begin(), left.end(), self->free_pages.begin());
+        return static_cast<int64_t>(moves);
+    } catch (const std::bad_alloc&) {
+        return lfm25::report_error(LFM25_ERR_CUDA, "out of host memory");
+    }
+}
+
 void lfm25_kv_allocator_snapshot(const lfm25_kv_allocator* self, lfm25_kv_pool_snapshot* out) {
     out->total_pages = self->total_pages;
     out->free_pages = self->free_pages.size();
