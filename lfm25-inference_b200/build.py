@@ -27,7 +27,7 @@ SOURCES = ["api.cu", "options.cu", "attention.cu", "kv_cache.cu", "fp8_elementwi
            "stack_attention.cu", "stack_attention_umma.cu", "stack_attention_decode.cu", "delta_rule.cu", "delta_chunk.cu",
            "delta_scan.cu", "delta_split.cu", "head_linear.cu", "stack_latent.cu", "stack_latent_decode.cu", "state_space.cu",
            "state_space_chunk.cu", "stack_executor.cu", "e4m3_api.cu", "e4m3_cache_write.cu", "e4m3_attention.cu",
-           "kv_pages.cu"]
+           "e4m3_attention_umma.cu", "kv_pages.cu"]
 COMPILE_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC"]
 LINK_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-shared", "-cudart", "static", "-ldl"]
 

@@ -44,8 +44,6 @@ struct DecodeParams {
     const uint32_t* request_slots;
     const uint32_t* position_ids;
     const uint32_t* token_order;
-    const uint32_t* segment_offsets;   // prompts: [segments + 1]
-    uint32_t num_segments;             // 0: single tokens
     uint64_t block_table_stride;
     uint64_t block_table_rows;
     uint64_t query_token_stride;
@@ -117,19 +115,6 @@ e4m3_attention_kernel(const DecodeParams p) {
     const uint32_t position = p.position_ids[token];
     if (table_row >= p.block_table_rows || position >= p.block_table_stride * kPageSize) {
         return;
-    }
-    if (p.num_segments != 0) {
-        // a token of a prompt has to continue its segment's first
-        bool member = false;
-        for (uint32_t segment = lane; segment < p.num_segments; segment += 32) {
-            const uint32_t begin = p.segment_offsets[segment];
-            if (begin <= token && token < p.segment_offsets[segment + 1]) {
-                member = p.request_slots[begin] == table_row && p.position_ids[begin] + (token - begin) == position;
-            }
-        }
-        if (!__any_sync(0xffffffffu, member)) {
-            return;
-        }
     }
     const uint32_t* __restrict__ table = p.block_tables + table_row * p.block_table_stride;
     const uint32_t first_head = kv_head * p.group + chunk * 16;
@@ -457,8 +442,6 @@ cudaError_t launch_e4m3_attention(cudaStream_t stream, const E4m3AttentionLaunch
     params.request_slots = launch.request_slots;
     params.position_ids = launch.position_ids;
     params.token_order = launch.token_order;
-    params.segment_offsets = launch.segment_offsets;
-    params.num_segments = static_cast<uint32_t>(launch.num_segments);
     params.block_table_stride = launch.block_table_stride;
     params.block_table_rows = launch.block_table_rows;
     params.query_token_stride = launch.query_token_stride;
@@ -486,11 +469,6 @@ cudaError_t launch_e4m3_attention(cudaStream_t stream, const E4m3AttentionLaunch
         return params.group <= 8 ? launch_shape<64, 8, 3>(stream, params, blocks) : launch_shape<64, 16, 2>(stream, params, blocks);
     }
     return params.group <= 8 ? launch_shape<128, 8, 2>(stream, params, blocks) : launch_shape<128, 16, 1>(stream, params, blocks);
-}
-
-// Every token of a prompt by itself.
-cudaError_t launch_e4m3_prompt_attention(cudaStream_t stream, const E4m3AttentionLaunch& launch) {
-    return launch_e4m3_attention(stream, launch);
 }
 
 }  // namespace lfm25

@@ -286,6 +286,7 @@ def test_what_is_not_seen_may_hold_anything(device, kind, window, sinks):
 
 @pytest.mark.parametrize("kind", ["decode", "prompts"])
 def test_unassigned_pages_leave_the_row(device, kind):
+    """... of the tokens that see them, and of no others."""
     rng = np.random.default_rng(9)
     contexts = (70, 2131, 9, 40)
     pool = pool_of(contexts)
@@ -298,6 +299,37 @@ def test_unassigned_pages_leave_the_row(device, kind):
     out = torch.full_like(query, 3.0)
     attention_call(kind, query, arena, to_u32(tables, device), to_u32(rows, device), to_u32(positions, device), out)
     assert (out[1:] == 3.0).all() and (out[0] != 3.0).any()
+
+
+@pytest.mark.parametrize("window", [0, 12])
+def test_prompt_rows_see_their_own_nan_and_missing_pages_only(device, window):
+    rng = np.random.default_rng(16)
+    contexts = (200,)
+    pool = pool_of(contexts)
+    arena, *cache = random_cache(rng, pool, 2, 64, device)
+    tables = tables_of(rng, contexts, pool)
+    first, count = 100, 100
+    arena.value[tables[0, 150 // PAGE], 1, 150 % PAGE, 17] = 0xFF            # one NaN of KV head 1
+    arena.key[tables[0, 170 // PAGE], 0, 170 % PAGE, 3] = 0x7F
+    tables[0, 12] = plain.UNASSIGNED                                        # keys 192 ..
+    rows, positions = np.zeros(count, dtype=np.int64), np.arange(first, first + count)
+    query = bf16(rng.standard_normal((count, 4, 64)), device)
+    out = torch.full_like(query, 3.0)
+    ops.paged_prompt_attention_e4m3_into(query, arena, to_u32(tables, device), to_u32(rows, device), to_u32(positions, device),
+                                         to_u32([0, count], device), out, window=window)
+    got = host(out)
+    last = 191                                                # positions behind it see the page that is missing
+    sees = lambda key: (positions >= key) & ((positions < key + window) if window else True)    # noqa: E731
+    assert (got[positions > last] == 3.0).all()
+    rest = positions <= last
+    assert np.array_equal(np.isnan(got[rest, 2:]).all(2).all(1), sees(150)[rest])
+    assert np.array_equal(np.isnan(got[rest, :2]).all(2).all(1), sees(170)[rest])
+    for heads, key in ((slice(0, 2), 170), (slice(2, 4), 150)):
+        keep = rest & ~sees(key)
+        exact, magnitude, score = plain.attend(host(query)[keep], np.nan_to_num(cache[0].full()), np.nan_to_num(cache[1].full()), tables,
+                                               rows[keep], positions[keep], window=window)
+        bound = plain.tolerance(exact, magnitude, score, 64, BF16_WEIGHTS)
+        assert np.all(np.abs(got[keep] - exact)[:, heads] <= bound[:, heads])
 
 
 @pytest.mark.parametrize("kind,rounding", [("decode", F16_WEIGHTS), ("prompts", BF16_WEIGHTS)])
@@ -419,6 +451,29 @@ def test_two_graphs_at_once_on_streams_of_their_own(device, kind):
                 graph.replay()
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) and a.any() for a, b in zip(outs, wants))
+
+
+def test_a_wait_that_runs_out_leaves_the_rows(device, library_option):
+    """One warp that brings pages never reports its first stage: the waits end after their limit, the status words say so, no row
+    is written, and the next call is as ever."""
+    rng = np.random.default_rng(15)
+    arena, *cache = random_cache(rng, 9, 2, 64, device)
+    tables = np.arange(9)[None]
+    query = bf16(rng.standard_normal((20, 8, 64)), device)
+    given = to_u32(tables, device), to_u32(np.zeros(20), device), to_u32(np.arange(20) + 70, device), to_u32([0, 20], device)
+    out = torch.full_like(query, 3.0)
+    ops.device_status()
+    library_option("wait_limit_ns", 2_000_000)
+    library_option("wait_selftest_drop", 1)
+    ops.paged_prompt_attention_e4m3_into(query, arena, *given, out)
+    torch.cuda.synchronize()
+    waits, tag, *_ = ops.device_status()
+    assert waits > 0 and tag == 10 and (out == 3.0).all()
+    library_option("wait_selftest_drop", 0)
+    library_option("wait_limit_ns", 1_000_000_000)
+    ops.paged_prompt_attention_e4m3_into(query, arena, *given, out)
+    check_attention(out, query, cache, tables, np.zeros(20, dtype=int), np.arange(20) + 70, BF16_WEIGHTS, out)
+    assert ops.device_status()[0] == 0
 
 
 # ------------------------------------------------------------------------------------------------ pages
