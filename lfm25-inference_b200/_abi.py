@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIBRARY_PATH = os.path.join(HERE, "liblfm25_b200.so")
@@ -62,12 +63,37 @@ SplitKRaggedAttentionLaunch = _launch_struct("SplitKRaggedAttentionLaunch", [
     "partials", "output", "#num_tokens", "#num_pages", "#block_table_stride", "#num_splits", "token_order"])
 E4m3Cache = _launch_struct("E4m3Cache", [
     "#page_size", "#num_pages", "#kv_heads", "#head_dim", "key_codes", "value_codes", "key_scales", "value_scales"])
-KvCacheWriteE4m3Launch = _launch_struct("KvCacheWriteE4m3Launch", [
+
+
+def _packed_struct(name, fields):
+    """A launch struct with `packed`, which takes all its words flat (a slice is a pointer and a length): building it field by field
+    takes several times as long as the rest of a small call."""
+    made = _launch_struct(name, fields)
+
+    def words(structure):
+        out = ""
+        for _, kind in structure._fields_:
+            out += words(kind) if issubclass(kind, ctypes.Structure) else "f" if kind is ctypes.c_float else "Q"
+        return out
+
+    # native alignment and, by the 0Q, native size; all fields but floats are of 8 bytes
+    layout = struct.Struct("@" + words(made) + "0Q")
+    assert layout.size == ctypes.sizeof(made)
+    made.packed = staticmethod(lambda *values: made.from_buffer_copy(layout.pack(*values)))
+    return made
+
+
+def pack_words(values) -> bytes:
+    """size_t words one behind the other."""
+    return struct.pack(f"@{len(values)}Q", *values)
+
+
+KvCacheWriteE4m3Launch = _packed_struct("KvCacheWriteE4m3Launch", [
     ("cache", E4m3Cache), "key", "value", "slot_mapping", "#num_tokens", "#kv_token_stride"])
-QkNormRopeKvWriteE4m3Launch = _launch_struct("QkNormRopeKvWriteE4m3Launch", [
+QkNormRopeKvWriteE4m3Launch = _packed_struct("QkNormRopeKvWriteE4m3Launch", [
     ("cache", E4m3Cache), "query", "query_out", "key", "value", "query_norm", "key_norm", "inv_freq", "position_ids",
     "slot_mapping", "#num_tokens", "#query_heads", "#query_token_stride", "#kv_token_stride", ("eps", ctypes.c_float)])
-PagedAttentionE4m3Launch = _launch_struct("PagedAttentionE4m3Launch", [
+PagedAttentionE4m3Launch = _packed_struct("PagedAttentionE4m3Launch", [
     ("cache", E4m3Cache), "query", "block_tables", "request_slots", "position_ids", "output", "#num_tokens", "#query_heads",
     "#query_token_stride", "#block_table_stride", "#window", "#sinks", "#maximum_context_tokens", ("scale", ctypes.c_float),
     "token_order", "segment_offsets", "#num_segments"])

@@ -422,8 +422,7 @@ e4m3_attention_kernel(const DecodeParams p) {
 template <uint32_t DIM, uint32_t HEADS, uint32_t AHEAD>
 cudaError_t launch_shape(cudaStream_t stream, const DecodeParams& params, uint64_t blocks) {
     constexpr size_t kShared = sizeof(float) * kWarps * HEADS * (DIM + 2);
-    const cudaError_t status = cudaFuncSetAttribute(e4m3_attention_kernel<DIM, HEADS, AHEAD>,
-                                                    cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kShared));
+    const cudaError_t status = allow_shared_memory<e4m3_attention_kernel<DIM, HEADS, AHEAD>>(kShared);
     if (status != cudaSuccess) {
         return status;
     }

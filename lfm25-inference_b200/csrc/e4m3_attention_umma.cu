@@ -691,8 +691,7 @@ e4m3_prompt_attention_kernel(const PromptParams p) {
 
 template <uint32_t DIM>
 cudaError_t launch_dim(cudaStream_t stream, const PromptParams& params, uint64_t blocks) {
-    const cudaError_t status = cudaFuncSetAttribute(e4m3_prompt_attention_kernel<DIM>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                    static_cast<int>(Layout<DIM>::kAlloc));
+    const cudaError_t status = allow_shared_memory<e4m3_prompt_attention_kernel<DIM>>(Layout<DIM>::kAlloc);
     if (status != cudaSuccess) {
         return status;
     }

@@ -4,6 +4,8 @@
 
 #include <cuda_runtime.h>
 
+#include <atomic>
+
 #include "options.h"
 
 namespace lfm25 {
@@ -35,6 +37,23 @@ cudaError_t launch_kernel(void (*kernel)(Parameters...), unsigned int blocks, un
     config.attrs = attributes;
     config.numAttrs = count;
     return cudaLaunchKernelEx(&config, kernel, static_cast<Parameters>(arguments)...);
+}
+
+// Dynamic shared memory of a kernel beyond 48 KB, allowed once per device: the call costs as much as a small launch.
+template <auto Kernel>
+cudaError_t allow_shared_memory(size_t bytes) {
+    static std::atomic<uint64_t> done{0};
+    int device = 0;
+    cudaError_t status = cudaGetDevice(&device);
+    const uint64_t bit = uint64_t{1} << (device & 63);
+    if (status != cudaSuccess || (done.load(std::memory_order_relaxed) & bit) != 0) {
+        return status;
+    }
+    status = cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
+    if (status == cudaSuccess) {
+        done.fetch_or(bit, std::memory_order_relaxed);
+    }
+    return status;
 }
 
 }  // namespace lfm25

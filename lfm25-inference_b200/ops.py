@@ -276,31 +276,61 @@ def paged_ragged_attention_splitk_static_lfm2_bf16_into(inputs: FastRaggedAttent
 
 
 # ------------------------------------------------------------------------------- 8-bit paged cache
+#
+# These calls are made for every layer of a step, and a small one is over on the GPU before Python has checked a dozen
+# tensors: the checks format nothing unless they fail, and a launch struct is packed in one go (44 -> 12 us a call).
 
 
-def _typed(name: str, tensor: torch.Tensor, *dtypes) -> torch.Tensor:
-    """A tensor of the expected type on the device of the current stream."""
-    _ensure(tensor.dtype in dtypes, f"8-bit cache: {name} must be {' or '.join(str(d) for d in dtypes)}, got {tensor.dtype}")
-    _ensure(tensor.is_cuda and tensor.device.index == torch.cuda.current_device(),
-            f"8-bit cache: {name} is on {tensor.device}, the current device is cuda:{torch.cuda.current_device()}")
-    return tensor
+def _refuse(message: str):
+    raise Lfm25Error(_abi.ERR_INVALID_ARGUMENT, message)
+
+
+def _current() -> tuple[int, int]:
+    """(device, stream) that a call goes to; without a device (-1, 0), which the library refuses."""
+    try:
+        device = torch.cuda.current_device()
+    except RuntimeError:
+        return -1, 0
+    return device, torch._C._cuda_getCurrentRawStream(device)
 
 
 _U32 = (torch.uint32, torch.int32)       # indices: the same bits
+_I64, _BF16, _F32 = (torch.int64,), (torch.bfloat16,), (torch.float32,)
+_CODES = (torch.uint8, torch.float8_e4m3fn)
 
 
-def _index(name: str, tensor: torch.Tensor, count: int, *dtypes) -> Slice:
-    _ensure(tensor.numel() == count, f"8-bit cache: {name} count mismatch: {tensor.numel()} for {count}")
-    return _slice(_typed(name, tensor, *dtypes))
+def _dense(name: str, tensor: torch.Tensor, dtypes, device: int, count: int = -1) -> tuple[int, int]:
+    """(pointer, elements) of a dense tensor of one of `dtypes` on `device` with `count` elements (-1: any number)."""
+    if tensor.dtype not in dtypes:
+        _refuse(f"8-bit cache: {name} must be {' or '.join(str(d) for d in dtypes)}, got {tensor.dtype}")
+    if tensor.get_device() != device:
+        _refuse(f"8-bit cache: {name} is on {tensor.device}, the current device is cuda:{device}")
+    if not tensor.is_contiguous():
+        _refuse(f"8-bit cache: {name} must be contiguous")
+    elements = tensor.numel()
+    if count >= 0 and elements != count:
+        _refuse(f"8-bit cache: {name} count mismatch: {elements} for {count}")
+    return tensor.data_ptr(), elements
 
 
-def _heads(name: str, tensor: torch.Tensor, head_dim: int) -> tuple[Slice, int]:
-    """Rows [tokens, heads, head_dim] whose heads are dense: the span they cover and their token stride (0: dense)."""
-    _ensure(tensor.dim() == 3 and tensor.shape[2] == head_dim, f"8-bit cache: {name} must have shape [N, heads, {head_dim}]")
-    _ensure(tensor.shape[0] > 0, f"8-bit cache: {name} requires tokens")
-    _ensure(tuple(tensor.stride()[1:]) == (head_dim, 1) or tensor.is_contiguous(), f"8-bit cache: {name} heads must be dense")
-    _typed(name, tensor, torch.bfloat16)
-    return _row_strided_slice(tensor), tensor.stride(0) if tensor.shape[0] > 1 else 0
+def _heads(name: str, tensor: torch.Tensor, head_dim: int, device: int) -> tuple[int, int, int, int, int]:
+    """Rows [tokens, heads, head_dim] whose heads are dense: (pointer, elements that they span, their token stride with 0 for
+    dense, tokens, heads)."""
+    if tensor.dim() != 3 or tensor.shape[2] != head_dim:
+        _refuse(f"8-bit cache: {name} must have shape [N, heads, {head_dim}]")
+    if tensor.dtype != torch.bfloat16:
+        _refuse(f"8-bit cache: {name} must be torch.bfloat16, got {tensor.dtype}")
+    if tensor.get_device() != device:
+        _refuse(f"8-bit cache: {name} is on {tensor.device}, the current device is cuda:{device}")
+    tokens, heads, _ = tensor.shape
+    if tokens == 0:
+        _refuse(f"8-bit cache: {name} requires tokens")
+    if tensor.is_contiguous():
+        return tensor.data_ptr(), tensor.numel(), 0, tokens, heads
+    stride, between, inside = tensor.stride()
+    if inside != 1 or (between != head_dim and heads > 1) or (tokens > 1 and stride < heads * head_dim):
+        _refuse(f"8-bit cache: {name} heads must be dense")
+    return tensor.data_ptr(), (tokens - 1) * stride + heads * head_dim, stride if tokens > 1 else 0, tokens, heads
 
 
 @dataclass
@@ -342,35 +372,40 @@ class E4m3KvArena:
         """Append (see `kv_cache_write_e4m3`)."""
         kv_cache_write_e4m3(key, value, self, physical_slots)
 
-    def _view(self) -> "_abi.E4m3Cache":
-        _ensure(self.key.dim() == 4 and self.key.shape[2] == self.page_size, "8-bit cache: codes must have shape [pages, heads, 16, dim]")
-        _ensure(self.value.shape == self.key.shape, "8-bit cache: key/value shape mismatch")
-        _ensure(tuple(self.key_scales.shape) == tuple(self.key.shape[:2]) and self.value_scales.shape == self.key_scales.shape,
-                "8-bit cache: scales must have shape [pages, heads]")
-        return _abi.E4m3Cache(self.page_size, self.num_pages, self.kv_heads, self.head_dim,
-                              _slice(_typed("key codes", self.key, torch.uint8, torch.float8_e4m3fn)),
-                              _slice(_typed("value codes", self.value, torch.uint8, torch.float8_e4m3fn)),
-                              _slice(_typed("key scales", self.key_scales, torch.float32)),
-                              _slice(_typed("value scales", self.value_scales, torch.float32)))
+    def _fields(self, device: int) -> tuple:
+        """The fields of lfm25_e4m3_cache."""
+        shape = self.key.shape
+        if len(shape) != 4 or shape[2] != self.page_size:
+            _refuse("8-bit cache: codes must have shape [pages, heads, 16, dim]")
+        pages, heads, page_size, dim = shape
+        codes, scales = pages * heads * page_size * dim, pages * heads
+        return (page_size, pages, heads, dim, *_dense("key codes", self.key, _CODES, device),
+                *_dense("value codes", self.value, _CODES, device, codes), *_dense("key scales", self.key_scales, _F32, device, scales),
+                *_dense("value scales", self.value_scales, _F32, device, scales))
 
 
-def _kv_rows(key, value, arena: E4m3KvArena) -> tuple[Slice, Slice, int]:
-    _ensure(key.shape == value.shape and key.dim() == 3 and key.shape[1] == arena.kv_heads,
-            f"8-bit cache: key and value must have shape [N, {arena.kv_heads}, {arena.head_dim}]")
-    key_rows, stride = _heads("key", key, arena.head_dim)
-    value_rows, value_stride = _heads("value", value, arena.head_dim)
-    _ensure(stride == value_stride, "8-bit cache: key and value must share their token stride")
-    return key_rows, value_rows, stride
+def _kv_rows(key, value, arena_fields, device: int) -> tuple:
+    """Key and value rows of an append: (pointer, span) of each, their token stride and number."""
+    heads, dim = arena_fields[2], arena_fields[3]
+    key_pointer, key_span, stride, tokens, key_heads = _heads("key", key, dim, device)
+    value_pointer, value_span, value_stride, value_tokens, value_heads = _heads("value", value, dim, device)
+    if key_heads != heads or value_heads != heads or value_tokens != tokens:
+        _refuse(f"8-bit cache: key and value must have shape [N, {heads}, {dim}]")
+    # a dense tensor has the stride that the other may have spelt out
+    if (stride or heads * dim) != (value_stride or heads * dim):
+        _refuse("8-bit cache: key and value must share their token stride")
+    return key_pointer, key_span, value_pointer, value_span, stride, tokens
 
 
 def kv_cache_write_e4m3(key, value, arena: E4m3KvArena, slot_mapping) -> None:
     """Appends bf16 keys and values [N, kv_heads, head_dim] (rows may be spaced apart) at physical slots i64 [N]; a negative
     slot skips its token.  Tokens of a page stand one behind the other in the batch; a page takes one such run a call.  A run
     that starts a page sets its scales, one that continues it raises them where it has to."""
-    key_rows, value_rows, stride = _kv_rows(key, value, arena)
-    launch = _abi.KvCacheWriteE4m3Launch(arena._view(), key_rows, value_rows,
-                                         _index("slot mapping", slot_mapping, key.shape[0], torch.int64), key.shape[0], stride)
-    check(library().lfm25_kv_cache_write_e4m3(_stream(), launch))
+    device, stream = _current()
+    fields = arena._fields(device)
+    *rows, stride, tokens = _kv_rows(key, value, fields, device)
+    check(library().lfm25_kv_cache_write_e4m3(stream, _abi.KvCacheWriteE4m3Launch.packed(
+        *fields, *rows, *_dense("slot mapping", slot_mapping, _I64, device, tokens), tokens, stride)))
 
 
 def qk_norm_rope_kv_write_e4m3(query, key, value, query_norm, key_norm, inv_freq, position_ids, slot_mapping,
@@ -378,35 +413,43 @@ def qk_norm_rope_kv_write_e4m3(query, key, value, query_norm, key_norm, inv_freq
     """RMS norm and rotation of queries and keys, then the append: `qk_norm_rope_kv_write_arena_decode_bf16` for the 8-bit
     cache, for any head layout and in f32 up to the one rounding of each result.  Queries go to `query_out` (dense), or back to
     where they came from."""
-    key_rows, value_rows, stride = _kv_rows(key, value, arena)
-    query_rows, query_stride = _heads("query", query, arena.head_dim)
+    device, stream = _current()
+    fields = arena._fields(device)
+    dim = fields[3]
+    *rows, stride, tokens = _kv_rows(key, value, fields, device)
+    query_pointer, query_span, query_stride, query_tokens, heads = _heads("query", query, dim, device)
+    if query_tokens != tokens:
+        _refuse("8-bit cache: query token count mismatch")
     query_out = query if query_out is None else query_out
-    _ensure(query_out.shape == query.shape, "8-bit cache: query output shape mismatch")
-    tokens = key.shape[0]
-    _ensure(query.shape[0] == tokens, "8-bit cache: query token count mismatch")
-    launch = _abi.QkNormRopeKvWriteE4m3Launch(
-        arena._view(), query_rows, _slice(_typed("query output", query_out, torch.bfloat16)), key_rows, value_rows,
-        _index("query norm", query_norm, arena.head_dim, torch.bfloat16), _index("key norm", key_norm, arena.head_dim, torch.bfloat16),
-        _index("rotation frequencies", inv_freq, arena.head_dim // 2, torch.float32), _index("positions", position_ids, tokens, *_U32),
-        _index("slot mapping", slot_mapping, tokens, torch.int64), tokens, query.shape[1], query_stride, stride, eps)
-    check(library().lfm25_qk_norm_rope_kv_write_e4m3(_stream(), launch))
+    if query_out.shape != query.shape:
+        _refuse("8-bit cache: query output shape mismatch")
+    check(library().lfm25_qk_norm_rope_kv_write_e4m3(stream, _abi.QkNormRopeKvWriteE4m3Launch.packed(
+        *fields, query_pointer, query_span, *_dense("query output", query_out, _BF16, device), *rows,
+        *_dense("query norm", query_norm, _BF16, device, dim), *_dense("key norm", key_norm, _BF16, device, dim),
+        *_dense("rotation frequencies", inv_freq, _F32, device, dim // 2), *_dense("positions", position_ids, _U32, device, tokens),
+        *_dense("slot mapping", slot_mapping, _I64, device, tokens), tokens, heads, query_stride, stride, eps)))
 
 
-def _attention_e4m3(query, arena, block_tables, request_slots, position_ids, output, window, sinks, scale, maximum_context_tokens,
-                    token_order, segment_offsets):
-    rows, stride = _heads("query", query, arena.head_dim)
-    tokens = query.shape[0]
-    _ensure(output.shape == query.shape, "8-bit cache: output shape mismatch")
-    _ensure(block_tables.dim() == 2, "block tables must have rank 2")
-    _ensure(window >= 0 and sinks >= 0 and maximum_context_tokens >= 0, "window, sinks and context must not be negative")
-    empty = Slice(None, 0)
-    return _abi.PagedAttentionE4m3Launch(
-        arena._view(), rows, _slice(_typed("block tables", block_tables, *_U32)), _index("request slots", request_slots, tokens, *_U32),
-        _index("positions", position_ids, tokens, *_U32), _slice(_typed("output", output, torch.bfloat16)), tokens, query.shape[1],
-        stride, block_tables.shape[1], window, sinks, maximum_context_tokens, arena.head_dim ** -0.5 if scale is None else scale,
-        _order_slice(_typed("token order", token_order, *_U32) if token_order is not None else None, tokens),
-        empty if segment_offsets is None else _slice(_typed("segment offsets", segment_offsets, *_U32)),
-        0 if segment_offsets is None else segment_offsets.numel() - 1)
+def _attention_e4m3(function, query, arena, block_tables, request_slots, position_ids, output, window, sinks, scale,
+                    maximum_context_tokens, token_order, segment_offsets) -> None:
+    device, stream = _current()
+    fields = arena._fields(device)
+    dim = fields[3]
+    pointer, span, stride, tokens, heads = _heads("query", query, dim, device)
+    if output.shape != query.shape:
+        _refuse("8-bit cache: output shape mismatch")
+    if block_tables.dim() != 2:
+        _refuse("block tables must have rank 2")
+    if window < 0 or sinks < 0 or maximum_context_tokens < 0:
+        _refuse("window, sinks and context must not be negative")
+    check(function(stream, _abi.PagedAttentionE4m3Launch.packed(
+        *fields, pointer, span, *_dense("block tables", block_tables, _U32, device),
+        *_dense("request slots", request_slots, _U32, device, tokens), *_dense("positions", position_ids, _U32, device, tokens),
+        *_dense("output", output, _BF16, device), tokens, heads, stride, block_tables.shape[1], window, sinks, maximum_context_tokens,
+        dim ** -0.5 if scale is None else scale,
+        *((0, 0) if token_order is None else _dense("token order", token_order, _U32, device, tokens)),
+        *((0, 0, 0) if segment_offsets is None else
+          (*_dense("segment offsets", segment_offsets, _U32, device), segment_offsets.numel() - 1)))))
 
 
 def paged_attention_e4m3_into(query, arena: E4m3KvArena, block_tables, request_slots, position_ids, output, window: int = 0,
@@ -415,34 +458,41 @@ def paged_attention_e4m3_into(query, arena: E4m3KvArena, block_tables, request_s
     sequence with j > position - window (window 0: all) or j < sinks.  `query` [N, query_heads, head_dim] may be row-strided,
     `scale` defaults to head_dim ** -0.5.  `maximum_context_tokens` (0: not known) only chooses how the work is split.  A token
     without a result (request slot or position outside the tables, an unassigned page) keeps its output row."""
-    check(library().lfm25_paged_attention_e4m3(_stream(), _attention_e4m3(
-        query, arena, block_tables, request_slots, position_ids, output, window, sinks, scale, maximum_context_tokens, token_order, None)))
+    _attention_e4m3(library().lfm25_paged_attention_e4m3, query, arena, block_tables, request_slots, position_ids, output, window, sinks,
+                    scale, maximum_context_tokens, token_order, None)
 
 
 def paged_prompt_attention_e4m3_into(query, arena: E4m3KvArena, block_tables, request_slots, position_ids, segment_offsets, output,
                                      window: int = 0, sinks: int = 0, scale: float | None = None, maximum_context_tokens: int = 0) -> None:
     """The same for portions of prompts whose own keys were appended before: tokens segment_offsets[s] .. segment_offsets[s + 1]
     sit at consecutive positions of one request slot.  Tokens outside every segment keep their output row."""
-    _ensure(segment_offsets.numel() >= 2, "prompt segments are empty")
-    check(library().lfm25_paged_prompt_attention_e4m3(_stream(), _attention_e4m3(
-        query, arena, block_tables, request_slots, position_ids, output, window, sinks, scale, maximum_context_tokens, None,
-        segment_offsets)))
+    if segment_offsets.numel() < 2:
+        _refuse("prompt segments are empty")
+    _attention_e4m3(library().lfm25_paged_prompt_attention_e4m3, query, arena, block_tables, request_slots, position_ids, output, window,
+                    sinks, scale, maximum_context_tokens, None, segment_offsets)
 
 
 def kv_pages_copy(arenas, source_pages, destination_pages) -> None:
     """Copies page source_pages[i] to page destination_pages[i] in every tensor of `arenas` (caches and scales of all layers,
     pages first): one launch for forked sequences and for compaction.  Destinations are distinct and none is a source."""
-    arenas = list(arenas)
-    _ensure(len(arenas) > 0, "page copy requires arenas")
-    table = (_abi.PageArena * len(arenas))()
-    for index, arena in enumerate(arenas):
-        _ensure(arena.dim() >= 1 and arena.shape[0] > 0 and arena.numel() > 0, "page copy arenas are [pages, ...]")
-        _ensure(arena.is_cuda and arena.device.index == torch.cuda.current_device(), "page copy arenas must be on the current device")
-        pages = _slice(arena)
-        table[index] = _abi.PageArena(pages.ptr, arena.numel() // arena.shape[0] * arena.element_size(), arena.shape[0])
-    pairs = source_pages.numel()
-    check(library().lfm25_kv_pages_copy(_stream(), table, len(arenas), _slice(_typed("source pages", source_pages, *_U32)),
-                                        _index("destination pages", destination_pages, pairs, *_U32), pairs))
+    device, stream = _current()
+    table = []
+    for arena in arenas:
+        if arena.get_device() != device:
+            _refuse("page copy arenas must be on the current device")
+        if not arena.is_contiguous():
+            _refuse("page copy arenas must be contiguous")
+        bytes_, pages = arena.nbytes, len(arena) if arena.dim() else 0
+        if pages == 0 or bytes_ == 0:
+            _refuse("page copy arenas are [pages, ...]")
+        table += (arena.data_ptr(), bytes_ // pages, pages)
+    if not table:
+        _refuse("page copy requires arenas")
+    source, pairs = _dense("source pages", source_pages, _U32, device)
+    destination, _ = _dense("destination pages", destination_pages, _U32, device, pairs)
+    count = len(table) // 3
+    check(library().lfm25_kv_pages_copy(stream, (_abi.PageArena * count).from_buffer_copy(_abi.pack_words(table)), count,
+                                        Slice(source, pairs), Slice(destination, pairs), pairs))
 
 
 # ------------------------------------------------------------------------------- FP8 producers
