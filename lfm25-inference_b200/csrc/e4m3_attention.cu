@@ -7,15 +7,17 @@
 //
 // A page (16 keys) is one step of mma.sync m16n8k16 in f16, which holds every E4M3 value:
 //   S = Q K^T     A = the query heads as rows, B = K^T.  The order of the reduction is free, so lane (g, t) of the warp
-//                 takes dimensions 16 t .. 16 t + 15 (of every 64) of the keys 4 (g / 2) + g % 2 and two further on: 16 bytes
-//                 a load, which turn into operands by conversion alone.
-//   O^T += V^T P^T   A = V^T, B = P^T, and the fragment of S is that of P^T.  Lane (g, t) takes the keys 4 t .. 4 t + 3
-//                 (the order of keys that S has) and head_dim / 8 dimensions of each: two bytes of two keys side by side
-//                 are one byte permutation, converted like K.
-// Codes travel from global memory to registers, a few pages ahead of their use; nothing passes through shared memory until
-// the warps are joined.  The query is brought to f16 by a power of two of its own (largest magnitude in [2^11, 2^12)): bf16
-// carries 8 bits, so what is lost lies 2^-36 below the largest element.  Page scales multiply S in front of the exponential
-// and the page's P V behind the MMA, both in f32, where a power of two rounds nothing.
+//                 takes dimensions 16 t .. 16 t + 15 (of every 64) of two keys: 16 bytes a load, which turn into operands by
+//                 conversion alone.
+//   O^T += V^T P^T   A = V^T, B = P^T, and the fragment of S is that of P^T.  Lane (g, t) takes four keys, head_dim / 8
+//                 dimensions of each: two bytes of two keys side by side are one byte permutation, converted like K.
+// Which keys a lane has is free as well (key_of) and chosen, with the place of a row's 16-byte pieces in shared memory, so that
+// both reads are free of bank conflicts.  Pages travel by asynchronous copies into a ring of each warp's own; nobody but the
+// warp waits for them, and nothing polls.
+//
+// The query is brought to f16 by a power of two of its own (largest magnitude in [2^11, 2^12)): bf16 carries 8 bits, so what is
+// lost lies 2^-36 below the largest element.  Page scales multiply S in front of the exponential and the page's P V behind the
+// MMA, both in f32, where a power of two rounds nothing.
 //
 // The maximum that weights refer to is only raised when a score exceeds it by more than 8 (weights are then at most 2^8,
 // which f16 holds): most pages need no exchange between lanes.
@@ -31,8 +33,6 @@ namespace lfm25 {
 
 namespace {
 
-constexpr uint32_t kWarps = 8;
-constexpr uint32_t kThreads = kWarps * 32;
 constexpr float kHeadroom = 8.0f;        // log2 of the largest weight against the reference maximum
 constexpr float kNoResult = -1.0f;       // sum of a share that met an unassigned page
 
@@ -72,27 +72,73 @@ __device__ __forceinline__ void cluster_barrier() {
                  "barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-// One page of one KV head as a lane holds it.
+__device__ __forceinline__ void copy_async_16(uint32_t to, const void* from, uint64_t policy) {
+    asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "l"(policy) : "memory");
+}
+__device__ __forceinline__ void copy_async_4(uint32_t to, const void* from) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <uint32_t PENDING>
+__device__ __forceinline__ void copies_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(PENDING) : "memory");
+}
+__device__ __forceinline__ uint4 load_shared_16(uint32_t address) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(address) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint2 load_shared_8(uint32_t address) {
+    uint2 v;
+    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(address) : "memory");
+    return v;
+}
+
 template <uint32_t DIM>
-struct PageCodes {
-    static constexpr uint32_t C = DIM / 64;
-    uint4 key[2][C];         // [key of the pair][64 dimensions]
-    uint2 value[4][C];       // [key][8 dimensions of 64 C]
-    float key_scale;
-    float value_scale;
+struct Page {
+    static constexpr uint32_t kSide = kPageSize * DIM;         // bytes of K, and of V
+    static constexpr uint32_t kStage = 2 * kSide;
+    // Key of a page that lane (g, t) takes for column 2 t + e of the score tile k, i.e. for the reduction step 8 k + 2 t + e of
+    // P V.  K is read 8 lanes at a time (two keys, e = 0 and 1, times 4 pieces), V 16 lanes at 64 dimensions (four keys, the t,
+    // times two pieces) and 8 at 128 (four keys times two pieces); a row has its 16-byte pieces at piece ^ turn(row).
+    //   64: two rows are 128 bytes.  Neighbours for e; for the t every second pair is swapped, and pieces turn with bit 2.
+    //   128: a row is 128 bytes.  Rows 4 apart for e, 0 2 5 7 for the t: piece ^ row takes eight different values in both.
+    static __device__ __forceinline__ uint32_t key_of(uint32_t k, uint32_t t, uint32_t e) {
+        return DIM == 64 ? 8 * k + 2 * t + (e ^ (t & 1)) : 8 * k + ((2 * t + (t >> 1)) ^ (4 * e));
+    }
+    static __device__ __forceinline__ uint32_t turn(uint32_t row) { return DIM == 64 ? (row >> 1) & 2 : row & 7; }
 };
 
 // HEADS: query heads of the CTA, at most 8 or at most 16
-template <uint32_t DIM, uint32_t HEADS, uint32_t AHEAD>
-__global__ void __launch_bounds__(kThreads, 2)
+template <uint32_t DIM, uint32_t HEADS>
+struct Shape {
+    static constexpr uint32_t kWarps = 8;
+    static constexpr uint32_t kThreads = kWarps * 32;
+    static constexpr uint32_t kStages = DIM == 64 ? 4 : 3;
+    static constexpr uint32_t kPerSm = DIM == 64 && HEADS == 8 ? 3 : 2;
+    static constexpr uint32_t kStride = DIM + 2;               // a head's sums, maximum and sum of weights
+    static constexpr uint32_t kRing = kWarps * kStages * Page<DIM>::kStage;
+    static constexpr uint32_t kMerge = kWarps * HEADS * kStride * 4;          // in the ring's place, once that is done with
+    static constexpr uint32_t kScales = (kRing > kMerge ? kRing : kMerge);    // [warp][stage] of 8 bytes behind it
+    static constexpr uint32_t kJoined = kScales + kWarps * kStages * 8;
+    static constexpr uint32_t kBytes = kJoined + HEADS * kStride * 4 + 16;
+};
+
+template <uint32_t DIM, uint32_t HEADS>
+__global__ void __launch_bounds__(Shape<DIM, HEADS>::kThreads, Shape<DIM, HEADS>::kPerSm)
 e4m3_attention_kernel(const DecodeParams p) {
+    using S = Shape<DIM, HEADS>;
+    using P = Page<DIM>;
+    constexpr uint32_t kWarps = S::kWarps;
+    constexpr uint32_t kStages = S::kStages;
+    constexpr uint32_t STRIDE = S::kStride;
     constexpr uint32_t C = DIM / 64;
     constexpr uint32_t TILES = DIM / 16;         // of 16 dimensions, rows of O^T
     constexpr uint32_t NT = HEADS / 8;           // tiles of 8 heads, columns of O^T
-    extern __shared__ float merge[];             // [kWarps][HEADS][DIM + 2]: sums, then maximum and sum of weights
-    constexpr uint32_t STRIDE = DIM + 2;
-    __shared__ uint32_t unassigned;
-    __shared__ float joined[HEADS * STRIDE];     // this CTA's share, for its cluster
+    extern __shared__ __align__(16) uint8_t decode_smem[];
+    float* merge = reinterpret_cast<float*>(decode_smem);
+    float* joined = reinterpret_cast<float*>(decode_smem + S::kJoined);     // this CTA's share, for its cluster
+    uint32_t* unassigned = reinterpret_cast<uint32_t*>(joined + HEADS * STRIDE);
     const uint32_t lane = threadIdx.x & 31;
     const uint32_t warp = threadIdx.x >> 5;
     const uint32_t g = lane >> 2;
@@ -123,13 +169,28 @@ e4m3_attention_kernel(const DecodeParams p) {
     const uint32_t share_begin = static_cast<uint32_t>(static_cast<uint64_t>(pages.count) * split / p.splits);
     const uint32_t share_end = static_cast<uint32_t>(static_cast<uint64_t>(pages.count) * (split + 1) / p.splits);
     const uint32_t my_pages = share_end - share_begin > warp ? (share_end - share_begin - warp + kWarps - 1) / kWarps : 0;
-    if (threadIdx.x == 0) unassigned = 0;
+    if (threadIdx.x == 0) *unassigned = 0;
     __syncthreads();
 
-    // ---- pages: entries 32 at a time, codes AHEAD pages ahead ----
+    // ---- pages: table entries 32 at a time, codes up to kStages pages ahead ----
+    const uint32_t ring = smem_u32(decode_smem) + warp * kStages * P::kStage;
+    const uint32_t scales = smem_u32(decode_smem + S::kScales) + warp * kStages * 8;
+    const uint64_t policy = l2_evict_first_policy();     // a page is read once a step
+    const uint32_t page_bytes = p.cache.kv_heads * P::kSide;
+    // this lane's pieces of a page are 512 bytes apart, on either side
+    const uint8_t* key_source = p.cache.key_codes + static_cast<size_t>(kv_head) * P::kSide + lane * 16;
+    const uint8_t* value_source = p.cache.value_codes + static_cast<size_t>(kv_head) * P::kSide + lane * 16;
+    const float* scale_source = (lane == 0 ? p.cache.key_scales : p.cache.value_scales) + kv_head;
+    uint32_t place[P::kSide / 512];
+#pragma unroll
+    for (uint32_t i = 0; i < P::kSide / 512; ++i) {
+        const uint32_t piece = i * 32 + lane;
+        const uint32_t row = piece / (DIM / 16);
+        place[i] = row * DIM + (((piece % (DIM / 16)) ^ P::turn(row)) << 4);
+    }
     uint32_t entries = 0;
     uint32_t bad = 0;
-    auto look_up = [&](uint32_t iteration) {          // entry of this warp's page number `iteration`
+    auto fetch = [&](uint32_t iteration) {
         if (iteration % 32 == 0) {
             const uint32_t index = share_begin + warp + (iteration + lane) * kWarps;
             entries = index < share_end ? __ldg(table + pages.logical(index)) : 0;
@@ -138,44 +199,31 @@ e4m3_attention_kernel(const DecodeParams p) {
                 entries = 0;
             }
         }
-        return __shfl_sync(0xffffffffu, entries, iteration % 32);
-    };
-    PageCodes<DIM> held[AHEAD];
-    auto load = [&](PageCodes<DIM>& page, uint32_t iteration) {
-        const size_t tile = static_cast<size_t>(look_up(iteration)) * p.cache.kv_heads + kv_head;
-        const uint8_t* keys = p.cache.key_codes + tile * (kPageSize * DIM) + (4 * (g / 2) + g % 2) * DIM + t * 16;
-        const uint8_t* values = p.cache.value_codes + tile * (kPageSize * DIM) + 4 * t * DIM + g * (DIM / 8);
+        const uint32_t entry = __shfl_sync(0xffffffffu, entries, iteration % 32);
+        const uint32_t stage = iteration % kStages;
+        const uint8_t* key = key_source + static_cast<uint64_t>(entry) * page_bytes;
+        const uint8_t* value = value_source + static_cast<uint64_t>(entry) * page_bytes;
 #pragma unroll
-        for (uint32_t k = 0; k < 2; ++k) {
-#pragma unroll
-            for (uint32_t c = 0; c < C; ++c) page.key[k][c] = __ldcs(reinterpret_cast<const uint4*>(keys + k * 2 * DIM + c * 64));
+        for (uint32_t i = 0; i < P::kSide / 512; ++i) {
+            copy_async_16(ring + stage * P::kStage + place[i], key + i * 512, policy);
+            copy_async_16(ring + stage * P::kStage + P::kSide + place[i], value + i * 512, policy);
         }
-#pragma unroll
-        for (uint32_t k = 0; k < 4; ++k) {
-            if constexpr (C == 1) {
-                page.value[k][0] = __ldcs(reinterpret_cast<const uint2*>(values + k * DIM));
-            } else {
-                const uint4 both = __ldcs(reinterpret_cast<const uint4*>(values + k * DIM));
-                page.value[k][0] = make_uint2(both.x, both.y);
-                page.value[k][C - 1] = make_uint2(both.z, both.w);
-            }
-        }
-        page.key_scale = __ldg(p.cache.key_scales + tile);
-        page.value_scale = __ldg(p.cache.value_scales + tile);
+        if (lane < 2) copy_async_4(scales + stage * 8 + lane * 4, scale_source + static_cast<uint64_t>(entry) * p.cache.kv_heads);
     };
 #pragma unroll
-    for (uint32_t i = 0; i < AHEAD; ++i) {
-        if (i < my_pages) load(held[i], i);
+    for (uint32_t i = 0; i < kStages; ++i) {
+        if (i < my_pages) fetch(i);
+        copies_commit();
     }
 
     // ---- query: rows g and g + 8 of A, dimensions 64 c + 16 t + 4 ks .. + 3 in step (c, ks) ----
-    uint32_t q[2][C][8];
-    float query_factor[2];
+    uint32_t q[NT][C][8];
+    float query_factor[NT];
 #pragma unroll
-    for (uint32_t half = 0; half < 2; ++half) {
+    for (uint32_t half = 0; half < NT; ++half) {
         uint32_t raw[C][8];
         uint32_t largest = 0;
-        const bool there = half < NT && g + 8 * half < heads;
+        const bool there = g + 8 * half < heads;
 #pragma unroll
         for (uint32_t c = 0; c < C; ++c) {
             uint4 part[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
@@ -221,65 +269,102 @@ e4m3_attention_kernel(const DecodeParams p) {
         for (uint32_t i = 0; i < TILES; ++i) out[n][i][0] = out[n][i][1] = make_float2(0.0f, 0.0f);
     }
 
-    auto use = [&](PageCodes<DIM>& page, uint32_t iteration) {
+    // where this lane reads: K of its column (key_of(k, g / 2, g % 2)), V of its keys
+    uint32_t key_at[C];
+    {
+        const uint32_t row = P::key_of(0, g >> 1, g & 1);
+#pragma unroll
+        for (uint32_t c = 0; c < C; ++c) key_at[c] = row * DIM + (((4 * c + t) ^ P::turn(row)) << 4);
+    }
+    uint32_t value_at[2];
+#pragma unroll
+    for (uint32_t e = 0; e < 2; ++e) {
+        const uint32_t row = P::key_of(0, t, e);
+        value_at[e] = P::kSide + row * DIM + (DIM == 64 ? (((g >> 1) ^ P::turn(row)) << 4) + (g & 1) * 8 : (g ^ P::turn(row)) << 4);
+    }
+
+    auto use = [&](uint32_t iteration) {
         const uint32_t base = pages.logical(share_begin + warp + iteration * kWarps) * kPageSize;
-        // ---- scores: [tile of 8 keys][head g: keys 4 t + 2 tile, + 1; head g + 8: the same] ----
-        float s[2][4] = {};
+        const uint32_t stage = ring + iteration % kStages * P::kStage;
+        // ---- scores of two tiles of 8 keys: head g, keys key_of(k, t, 0 and 1); head g + 8, the same ----
+        float s[2][4];
 #pragma unroll
         for (uint32_t k = 0; k < 2; ++k) {
 #pragma unroll
             for (uint32_t c = 0; c < C; ++c) {
-                const uint32_t words[4] = {page.key[k][c].x, page.key[k][c].y, page.key[k][c].z, page.key[k][c].w};
+                const uint4 codes = load_shared_16(stage + key_at[c] + k * 8 * DIM);
+                const uint32_t words[4] = {codes.x, codes.y, codes.z, codes.w};
 #pragma unroll
                 for (uint32_t ks = 0; ks < 4; ++ks) {
-                    mma_f16_16816(s[k], q[0][c][2 * ks], NT > 1 ? q[1][c][2 * ks] : 0u, q[0][c][2 * ks + 1],
-                                  NT > 1 ? q[1][c][2 * ks + 1] : 0u, e4m3x2_to_f16x2(words[ks]), e4m3x2_high_to_f16x2(words[ks]));
+                    const uint32_t a1 = NT > 1 ? q[NT - 1][c][2 * ks] : 0u;
+                    const uint32_t a3 = NT > 1 ? q[NT - 1][c][2 * ks + 1] : 0u;
+                    if (c == 0 && ks == 0) {
+                        mma_f16_16816_first(s[k], q[0][c][0], a1, q[0][c][1], a3, e4m3x2_to_f16x2(words[0]), e4m3x2_high_to_f16x2(words[0]));
+                    } else {
+                        mma_f16_16816(s[k], q[0][c][2 * ks], a1, q[0][c][2 * ks + 1], a3, e4m3x2_to_f16x2(words[ks]),
+                                      e4m3x2_high_to_f16x2(words[ks]));
+                    }
                 }
             }
         }
+        uint2 value[4][C];
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) {
+            const uint32_t at = stage + value_at[i & 1] + (i >> 1) * 8 * DIM;
+            if constexpr (C == 1) {
+                value[i][0] = load_shared_8(at);
+            } else {
+                const uint4 both = load_shared_16(at);
+                value[i][0] = make_uint2(both.x, both.y);
+                value[i][C - 1] = make_uint2(both.z, both.w);
+            }
+        }
+        const uint2 scale_bits = load_shared_8(scales + iteration % kStages * 8);
+        const float key_scale = __uint_as_float(scale_bits.x);
+        const float value_scale = __uint_as_float(scale_bits.y);
         // ---- mask: only pages at an edge of what the token sees have one ----
-        uint32_t seen = 0xfu;                            // of keys base + 4 t ..
+        uint32_t seen = 0xfu;
         const bool whole = base + kPageSize - 1 <= position && (base >= pages.first_key || base + kPageSize <= p.sinks);
         if (!whole) {
             seen = 0;
 #pragma unroll
             for (uint32_t i = 0; i < 4; ++i) {
-                const uint32_t key = base + 4 * t + i;
+                const uint32_t key = base + P::key_of(i >> 1, t, i & 1);
                 if (key <= position && (key >= pages.first_key || key < p.sinks)) {
                     seen |= 1u << i;
                 } else {
                     // whatever lies there, a weight of 0 must not meet a NaN
 #pragma unroll
-                    for (uint32_t c = 0; c < C; ++c) page.value[i][c] = make_uint2(0, 0);
+                    for (uint32_t c = 0; c < C; ++c) value[i][c] = make_uint2(0, 0);
+#pragma unroll
+                    for (uint32_t n = 0; n < NT; ++n) s[i >> 1][2 * n + (i & 1)] = -INFINITY;
                 }
             }
         }
         // ---- weights ----
         uint32_t weights[NT][2];
+        float factor[NT];
+        float most[NT];
         bool above = false;
 #pragma unroll
         for (uint32_t n = 0; n < NT; ++n) {
-            const float factor = page.key_scale * query_factor[n];
-#pragma unroll
-            for (uint32_t i = 0; i < 4; ++i) {
-                float& x = s[i >> 1][2 * n + (i & 1)];
-                x = (seen >> i) & 1 ? x * factor : -INFINITY;
-                above = above || x > maximum[n] + kHeadroom;
-            }
+            factor[n] = key_scale * query_factor[n];
+            // a factor of 0 makes the product with -inf a NaN, which the comparison passes over
+            most[n] = fmaxf(max3(s[0][2 * n], s[0][2 * n + 1], s[1][2 * n]), s[1][2 * n + 1]) * factor[n];
+            above = above || most[n] > maximum[n] + kHeadroom;
         }
         if (__any_sync(0xffffffffu, above)) {
 #pragma unroll
             for (uint32_t n = 0; n < NT; ++n) {
-                float most = fmaxf(fmaxf(s[0][2 * n], s[0][2 * n + 1]), fmaxf(s[1][2 * n], s[1][2 * n + 1]));
-                most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
-                most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
-                most = fmaxf(most, maximum[n]);
+                most[n] = fmaxf(most[n], __shfl_xor_sync(0xffffffffu, most[n], 1));
+                most[n] = fmaxf(most[n], __shfl_xor_sync(0xffffffffu, most[n], 2));
+                most[n] = fmaxf(most[n], maximum[n]);
                 // a row that has seen nothing yet keeps its sums of 0: exp2(-inf - -inf) is no factor
-                const float factor = most == maximum[n] ? 1.0f : fast_exp2(maximum[n] - most);
-                maximum[n] = most;
-                sum[n] *= factor;
-                const float low = __shfl_sync(0xffffffffu, factor, 8 * t);
-                const float high = __shfl_sync(0xffffffffu, factor, 8 * t + 4);
+                const float shrink = most[n] == maximum[n] ? 1.0f : fast_exp2(maximum[n] - most[n]);
+                maximum[n] = most[n];
+                sum[n] *= shrink;
+                const float low = __shfl_sync(0xffffffffu, shrink, 8 * t);
+                const float high = __shfl_sync(0xffffffffu, shrink, 8 * t + 4);
 #pragma unroll
                 for (uint32_t i = 0; i < TILES; ++i) {
 #pragma unroll
@@ -291,8 +376,10 @@ e4m3_attention_kernel(const DecodeParams p) {
         for (uint32_t n = 0; n < NT; ++n) {
             float w[4];
 #pragma unroll
-            for (uint32_t i = 0; i < 4; ++i) {
-                w[i] = (seen >> i) & 1 ? fast_exp2(s[i >> 1][2 * n + (i & 1)] - maximum[n]) : 0.0f;
+            for (uint32_t i = 0; i < 4; ++i) w[i] = fast_exp2(fmaf(s[i >> 1][2 * n + (i & 1)], factor[n], -maximum[n]));
+            if (!whole) {
+#pragma unroll
+                for (uint32_t i = 0; i < 4; ++i) w[i] = (seen >> i) & 1 ? w[i] : 0.0f;
             }
             weights[n][0] = pack_f16x2(w[0], w[1]);
             weights[n][1] = pack_f16x2(w[2], w[3]);
@@ -300,13 +387,12 @@ e4m3_attention_kernel(const DecodeParams p) {
             sum[n] += (w[0] + w[1]) + (w[2] + w[3]);
         }
         // ---- O^T += scale * V^T P^T ----
-        const float scale = page.value_scale;
 #pragma unroll
         for (uint32_t tile = 0; tile < TILES; tile += 2) {
             // dimensions 2 tile .. 2 tile + 3 of this lane's DIM / 8: one byte each of a word
             uint32_t word[4];
 #pragma unroll
-            for (uint32_t k = 0; k < 4; ++k) word[k] = tile & 2 ? page.value[k][tile / 4].y : page.value[k][tile / 4].x;
+            for (uint32_t k = 0; k < 4; ++k) word[k] = tile & 2 ? value[k][tile / 4].y : value[k][tile / 4].x;
             const uint32_t low[2] = {__byte_perm(word[0], word[1], 0x5140), __byte_perm(word[2], word[3], 0x5140)};
             const uint32_t high[2] = {__byte_perm(word[0], word[1], 0x7362), __byte_perm(word[2], word[3], 0x7362)};
 #pragma unroll
@@ -318,28 +404,29 @@ e4m3_attention_kernel(const DecodeParams p) {
                 const uint32_t a3 = e4m3x2_high_to_f16x2(pair[1]);
 #pragma unroll
                 for (uint32_t n = 0; n < NT; ++n) {
-                    float d[4] = {};
-                    mma_f16_16816(d, a0, a1, a2, a3, weights[n][0], weights[n][1]);
+                    float d[4];
+                    mma_f16_16816_first(d, a0, a1, a2, a3, weights[n][0], weights[n][1]);
 #pragma unroll
                     for (uint32_t h = 0; h < 2; ++h) {
                         float2& o = out[n][tile + half][h];
-                        o = make_float2(fmaf(d[2 * h], scale, o.x), fmaf(d[2 * h + 1], scale, o.y));
+                        o = fma_pair(make_float2(d[2 * h], d[2 * h + 1]), value_scale, o);
                     }
                 }
             }
         }
     };
 
-    for (uint32_t iteration = 0; iteration < my_pages; iteration += AHEAD) {
-#pragma unroll
-        for (uint32_t i = 0; i < AHEAD; ++i) {
-            if (iteration + i < my_pages) {
-                use(held[i], iteration + i);
-                if (iteration + i + AHEAD < my_pages) load(held[i], iteration + i + AHEAD);
-            }
-        }
+    for (uint32_t iteration = 0; iteration < my_pages; ++iteration) {
+        copies_wait<kStages - 1>();
+        __syncwarp();                                  // every lane's pieces are there
+        use(iteration);
+        __syncwarp();                                  // and read by all
+        if (iteration + kStages < my_pages) fetch(iteration + kStages);
+        copies_commit();
     }
-    if (__any_sync(0xffffffffu, bad != 0) && lane == 0) unassigned = 1;
+    if (__any_sync(0xffffffffu, bad != 0) && lane == 0) *unassigned = 1;
+    copies_wait<0>();
+    __syncthreads();                                   // the ring's place is free
 
     // ---- join the warps: O^T of lane (g, t) has dimensions DIM / 8 * g + 2 tile + h of the heads 8 n + 2 t, + 1 ----
 #pragma unroll
@@ -361,7 +448,7 @@ e4m3_attention_kernel(const DecodeParams p) {
         }
     }
     __syncthreads();
-    for (uint32_t index = threadIdx.x; index < heads * DIM; index += kThreads) {
+    for (uint32_t index = threadIdx.x; index < heads * DIM; index += S::kThreads) {
         const uint32_t head = index / DIM;
         const uint32_t dim = index % DIM;
         float most = -INFINITY;
@@ -381,9 +468,9 @@ e4m3_attention_kernel(const DecodeParams p) {
             joined[head * STRIDE + dim] = value;
             if (dim == 0) {
                 joined[head * STRIDE + DIM] = most;
-                joined[head * STRIDE + DIM + 1] = unassigned ? kNoResult : total;
+                joined[head * STRIDE + DIM + 1] = *unassigned ? kNoResult : total;
             }
-        } else if (!unassigned) {
+        } else if (*unassigned == 0) {
             p.output[(static_cast<size_t>(token) * p.query_heads + first_head + head) * DIM + dim] = __float2bfloat16_rn(value / total);
         }
     }
@@ -395,7 +482,7 @@ e4m3_attention_kernel(const DecodeParams p) {
     const uint32_t share = (heads * DIM + p.splits - 1) / p.splits;
     const uint32_t end = min((split + 1) * share, heads * DIM);
     const uint32_t own = smem_u32(joined);
-    for (uint32_t index = split * share + threadIdx.x; index < end; index += kThreads) {
+    for (uint32_t index = split * share + threadIdx.x; index < end; index += S::kThreads) {
         const uint32_t head = index / DIM;
         const uint32_t dim = index % DIM;
         float most = -INFINITY;
@@ -419,14 +506,14 @@ e4m3_attention_kernel(const DecodeParams p) {
     cluster_barrier();      // nobody leaves while its share is read
 }
 
-template <uint32_t DIM, uint32_t HEADS, uint32_t AHEAD>
+template <uint32_t DIM, uint32_t HEADS>
 cudaError_t launch_shape(cudaStream_t stream, const DecodeParams& params, uint64_t blocks) {
-    constexpr size_t kShared = sizeof(float) * kWarps * HEADS * (DIM + 2);
-    const cudaError_t status = allow_shared_memory<e4m3_attention_kernel<DIM, HEADS, AHEAD>>(kShared);
+    using S = Shape<DIM, HEADS>;
+    const cudaError_t status = allow_shared_memory<e4m3_attention_kernel<DIM, HEADS>>(S::kBytes);
     if (status != cudaSuccess) {
         return status;
     }
-    return launch_kernel(e4m3_attention_kernel<DIM, HEADS, AHEAD>, static_cast<unsigned int>(blocks), kThreads, kShared, stream,
+    return launch_kernel(e4m3_attention_kernel<DIM, HEADS>, static_cast<unsigned int>(blocks), S::kThreads, S::kBytes, stream,
                          params.splits, params);
 }
 
@@ -459,15 +546,15 @@ cudaError_t launch_e4m3_attention(cudaStream_t stream, const E4m3AttentionLaunch
     }
     const uint64_t pages = (longest + kPageSize - 1) / kPageSize;
     params.splits = 1;
-    while (params.splits < 8 && items * params.splits < 592 && pages >= 2 * params.splits * kWarps) params.splits *= 2;
+    while (params.splits < 8 && items * params.splits < 592 && pages >= 2 * params.splits * 8) params.splits *= 2;
     const uint64_t blocks = items * params.splits;
     if (blocks > 0x7fffffffu) {
         return cudaErrorInvalidConfiguration;
     }
     if (launch.cache.head_dim == 64) {
-        return params.group <= 8 ? launch_shape<64, 8, 3>(stream, params, blocks) : launch_shape<64, 16, 2>(stream, params, blocks);
+        return params.group <= 8 ? launch_shape<64, 8>(stream, params, blocks) : launch_shape<64, 16>(stream, params, blocks);
     }
-    return params.group <= 8 ? launch_shape<128, 8, 2>(stream, params, blocks) : launch_shape<128, 16, 1>(stream, params, blocks);
+    return params.group <= 8 ? launch_shape<128, 8>(stream, params, blocks) : launch_shape<128, 16>(stream, params, blocks);
 }
 
 }  // namespace lfm25

@@ -56,7 +56,16 @@ __device__ __forceinline__ float2 bf16x2_to_float2(uint32_t pair) {
     return make_float2(__uint_as_float(pair << 16), __uint_as_float(pair & 0xffff0000u));
 }
 
-// D(16x8, f32) = A(16x16, f16, row) * B(16x8, f16, col) + C
+// a * b + c for two values at a time, b the same for both
+__device__ __forceinline__ float2 fma_pair(float2 a, float b, float2 c) {
+    float2 out;
+    asm("{\n.reg .b64 x, y, z;\nmov.b64 x, {%2, %3};\nmov.b64 y, {%4, %4};\nmov.b64 z, {%5, %6};\nfma.rn.f32x2 x, x, y, z;\n"
+        "mov.b64 {%0, %1}, x;\n}"
+        : "=f"(out.x), "=f"(out.y) : "f"(a.x), "f"(a.y), "f"(b), "f"(c.x), "f"(c.y));
+    return out;
+}
+
+// D(16x8, f32) += A(16x16, f16, row) * B(16x8, f16, col)
 __device__ __forceinline__ void mma_f16_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                               uint32_t b0, uint32_t b1) {
     asm volatile(
@@ -64,6 +73,16 @@ __device__ __forceinline__ void mma_f16_16816(float (&d)[4], uint32_t a0, uint32
         "{%0, %1, %2, %3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// D(16x8, f32) = A(16x16, f16, row) * B(16x8, f16, col)
+__device__ __forceinline__ void mma_f16_16816_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                                    uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%10, %10, %10, %10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
 }
 
 }  // namespace lfm25
