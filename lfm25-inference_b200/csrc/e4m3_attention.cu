@@ -22,8 +22,14 @@
 // The maximum that weights refer to is only raised when a score exceeds it by more than 8 (weights are then at most 2^8,
 // which f16 holds): most pages need no exchange between lanes.
 //
+// Without its arithmetic the kernel streams at the copy peak (128 tokens at contexts 128..4096: 43.3 us); with it 50.2, bound by the
+// instructions of a page: about 180, 40 of them conversions.  K by the 8-bit MMA instead (its operands as they are, the query in two
+// parts) took as long: that instruction unpacks to f16 itself.
+//
 // Split: with few (token, KV head) pairs the pages of one are shared by the CTAs of a cluster, joined through distributed
 // shared memory: no workspace, so calls never share memory, and one launch.
+#include <type_traits>
+
 #include "e4m3_cache.cuh"
 #include "e4m3_cache.h"
 #include "e4m3_visible.cuh"
@@ -51,7 +57,8 @@ struct DecodeParams {
     uint32_t query_heads;
     uint32_t group;        // query heads of a KV head
     uint32_t chunks;       // of at most 16 of them
-    uint32_t splits;       // CTAs of a cluster
+    uint32_t splits;       // CTAs of a cluster, a power of two
+    uint32_t splits_log2;
     uint32_t window;
     uint32_t sinks;
     float scale_log2;
@@ -74,9 +81,6 @@ __device__ __forceinline__ void cluster_barrier() {
 
 __device__ __forceinline__ void copy_async_16(uint32_t to, const void* from, uint64_t policy) {
     asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "l"(policy) : "memory");
-}
-__device__ __forceinline__ void copy_async_4(uint32_t to, const void* from) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to), "l"(from) : "memory");
 }
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <uint32_t PENDING>
@@ -109,28 +113,37 @@ struct Page {
     static __device__ __forceinline__ uint32_t turn(uint32_t row) { return DIM == 64 ? (row >> 1) & 2 : row & 7; }
 };
 
-// HEADS: query heads of the CTA, at most 8 or at most 16
-template <uint32_t DIM, uint32_t HEADS>
+// HEADS: query heads of the CTA, at most 8 or at most 16; WARPS: 4 or 8
+template <uint32_t DIM, uint32_t HEADS, uint32_t WARPS>
 struct Shape {
-    static constexpr uint32_t kWarps = 8;
+    static constexpr uint32_t kWarps = WARPS;
     static constexpr uint32_t kThreads = kWarps * 32;
-    static constexpr uint32_t kStages = DIM == 64 ? 4 : 3;
-    static constexpr uint32_t kPerSm = DIM == 64 && HEADS == 8 ? 3 : 2;
-    static constexpr uint32_t kStride = DIM + 2;               // a head's sums, maximum and sum of weights
-    static constexpr uint32_t kRing = kWarps * kStages * Page<DIM>::kStage;
+    // Pages that a warp works on side by side, and warps that an SM holds with the registers this takes.  One page is one chain of
+    // dependent instructions, 0.37 us for a warp by itself; two take 0.23 us each.  At 64 dimensions two pages and 16 warps beat one
+    // and 24 (128 tokens at contexts 128..4096: 50.2 against 54.2 us; 16 heads: 39.8 at 12 warps against 44.8), at 128 and up to 8 heads
+    // one and 12 beat two and 8 (100 tokens at contexts 500..5000: 33.9 against 38.2 us), at 128 and 16 heads two beat one at 8
+    // warps each (32.4 against 35.0 us).
+    static constexpr uint32_t kPages = DIM == 128 && HEADS == 8 ? 1 : 2;
+    static constexpr uint32_t kWarpsPerSm = DIM == 64 ? (HEADS == 8 ? 16 : 12) : (HEADS == 8 ? 12 : 8);
+    static constexpr uint32_t kPerSm = kWarpsPerSm / WARPS;
+    static constexpr uint32_t kStages = 3;                     // so many groups of pages on the way
+    static constexpr uint32_t kStride = DIM + 4;               // a head's sums, maximum and sum of weights
+    static constexpr uint32_t kRing = kWarps * kStages * kPages * Page<DIM>::kStage;
     static constexpr uint32_t kMerge = kWarps * HEADS * kStride * 4;          // in the ring's place, once that is done with
-    static constexpr uint32_t kScales = (kRing > kMerge ? kRing : kMerge);    // [warp][stage] of 8 bytes behind it
-    static constexpr uint32_t kJoined = kScales + kWarps * kStages * 8;
+    static constexpr uint32_t kQuery = kRing > kMerge ? kRing : kMerge;       // f16 [HEADS][DIM], then HEADS factors
+    static constexpr uint32_t kJoined = kQuery + HEADS * DIM * 2 + HEADS * 4;
     static constexpr uint32_t kBytes = kJoined + HEADS * kStride * 4 + 16;
 };
 
-template <uint32_t DIM, uint32_t HEADS>
-__global__ void __launch_bounds__(Shape<DIM, HEADS>::kThreads, Shape<DIM, HEADS>::kPerSm)
+template <uint32_t DIM, uint32_t HEADS, uint32_t WARPS>
+__global__ void __launch_bounds__(Shape<DIM, HEADS, WARPS>::kThreads, Shape<DIM, HEADS, WARPS>::kPerSm)
 e4m3_attention_kernel(const DecodeParams p) {
-    using S = Shape<DIM, HEADS>;
+    using S = Shape<DIM, HEADS, WARPS>;
     using P = Page<DIM>;
     constexpr uint32_t kWarps = S::kWarps;
     constexpr uint32_t kStages = S::kStages;
+    constexpr uint32_t NP = S::kPages;
+    constexpr uint32_t kGroup = NP * P::kStage;
     constexpr uint32_t STRIDE = S::kStride;
     constexpr uint32_t C = DIM / 64;
     constexpr uint32_t TILES = DIM / 16;         // of 16 dimensions, rows of O^T
@@ -147,13 +160,16 @@ e4m3_attention_kernel(const DecodeParams p) {
     pdl_wait();
 
     // ---- which token, KV head, heads and share; every early exit is one of the whole cluster ----
-    const uint32_t split = blockIdx.x % p.splits;
-    uint32_t item = blockIdx.x / p.splits;
-    const uint32_t chunk = item % p.chunks;
-    item /= p.chunks;
-    const uint32_t kv_head = item % p.cache.kv_heads;
-    item /= p.cache.kv_heads;
-    const uint32_t token = p.token_order != nullptr ? p.token_order[item] : item;
+    const uint32_t split = blockIdx.x & (p.splits - 1);
+    uint32_t item = blockIdx.x >> p.splits_log2;
+    uint32_t chunk = 0;
+    if (p.chunks > 1) {
+        chunk = item % p.chunks;
+        item /= p.chunks;
+    }
+    const uint32_t rank = item / p.cache.kv_heads;
+    const uint32_t kv_head = item - rank * p.cache.kv_heads;
+    const uint32_t token = p.token_order != nullptr ? p.token_order[rank] : rank;
     if (token >= p.num_tokens) {
         return;
     }
@@ -166,104 +182,134 @@ e4m3_attention_kernel(const DecodeParams p) {
     const uint32_t first_head = kv_head * p.group + chunk * 16;
     const uint32_t heads = min(p.group - chunk * 16, HEADS);
     const VisiblePages pages(position, position, p.window, p.sinks);
-    const uint32_t share_begin = static_cast<uint32_t>(static_cast<uint64_t>(pages.count) * split / p.splits);
-    const uint32_t share_end = static_cast<uint32_t>(static_cast<uint64_t>(pages.count) * (split + 1) / p.splits);
-    const uint32_t my_pages = share_end - share_begin > warp ? (share_end - share_begin - warp + kWarps - 1) / kWarps : 0;
-    if (threadIdx.x == 0) *unassigned = 0;
-    __syncthreads();
+    const uint32_t share_begin = static_cast<uint32_t>(static_cast<uint64_t>(pages.count) * split >> p.splits_log2);
+    const uint32_t share_end = static_cast<uint32_t>(static_cast<uint64_t>(pages.count) * (split + 1) >> p.splits_log2);
+    const uint32_t groups = (share_end - share_begin + NP - 1) / NP;
+    const uint32_t my_groups = groups > warp ? (groups - warp + kWarps - 1) / kWarps : 0;
 
-    // ---- pages: table entries 32 at a time, codes up to kStages pages ahead ----
-    const uint32_t ring = smem_u32(decode_smem) + warp * kStages * P::kStage;
-    const uint32_t scales = smem_u32(decode_smem + S::kScales) + warp * kStages * 8;
+    // ---- pages: table entries and scales 32 pages at a time, a lane each; codes up to kStages pages ahead ----
+    const uint32_t ring = smem_u32(decode_smem) + warp * kStages * kGroup;
     const uint64_t policy = l2_evict_first_policy();     // a page is read once a step
     const uint32_t page_bytes = p.cache.kv_heads * P::kSide;
     // this lane's pieces of a page are 512 bytes apart, on either side
     const uint8_t* key_source = p.cache.key_codes + static_cast<size_t>(kv_head) * P::kSide + lane * 16;
     const uint8_t* value_source = p.cache.value_codes + static_cast<size_t>(kv_head) * P::kSide + lane * 16;
-    const float* scale_source = (lane == 0 ? p.cache.key_scales : p.cache.value_scales) + kv_head;
     uint32_t place[P::kSide / 512];
 #pragma unroll
     for (uint32_t i = 0; i < P::kSide / 512; ++i) {
         const uint32_t piece = i * 32 + lane;
         const uint32_t row = piece / (DIM / 16);
-        place[i] = row * DIM + (((piece % (DIM / 16)) ^ P::turn(row)) << 4);
+        place[i] = ring + row * DIM + (((piece % (DIM / 16)) ^ P::turn(row)) << 4);
     }
+    constexpr uint32_t kBlock = 32 / NP;                   // groups whose entries the lanes hold
+    auto look_up = [&](uint32_t group) -> uint32_t {       // entry of this lane's page of the groups from `group` on
+        const uint32_t index = share_begin + (warp + (group + lane / NP) * kWarps) * NP + lane % NP;
+        return index < share_end ? __ldg(table + pages.logical(index)) : 0;
+    };
+    uint32_t coming = look_up(0);
     uint32_t entries = 0;
     uint32_t bad = 0;
-    auto fetch = [&](uint32_t iteration) {
-        if (iteration % 32 == 0) {
-            const uint32_t index = share_begin + warp + (iteration + lane) * kWarps;
-            entries = index < share_end ? __ldg(table + pages.logical(index)) : 0;
+    uint32_t block = 0;                                  // first group of those whose entries are at hand
+    float scales[2][2];                                  // of these pages and of the ones before, for K and V
+    scales[0][0] = scales[0][1] = 0.0f;
+    uint32_t fill = 0;                                   // ring place of the next group to come, in bytes
+    auto fetch = [&](uint32_t group) {
+        if (group % kBlock == 0) {
+            entries = coming;
+            block = group;
+            coming = look_up(group + kBlock);
             if (entries >= p.cache.num_pages) {
-                bad = 1;                              // page 0 in its place; the token gets no result
+                bad = 1;                                 // page 0 in its place; the token gets no result
                 entries = 0;
             }
+            const uint64_t tile = static_cast<uint64_t>(entries) * p.cache.kv_heads + kv_head;
+            scales[1][0] = scales[0][0];
+            scales[1][1] = scales[0][1];
+            scales[0][0] = __ldg(p.cache.key_scales + tile);
+            scales[0][1] = __ldg(p.cache.value_scales + tile);
         }
-        const uint32_t entry = __shfl_sync(0xffffffffu, entries, iteration % 32);
-        const uint32_t stage = iteration % kStages;
-        const uint8_t* key = key_source + static_cast<uint64_t>(entry) * page_bytes;
-        const uint8_t* value = value_source + static_cast<uint64_t>(entry) * page_bytes;
 #pragma unroll
-        for (uint32_t i = 0; i < P::kSide / 512; ++i) {
-            copy_async_16(ring + stage * P::kStage + place[i], key + i * 512, policy);
-            copy_async_16(ring + stage * P::kStage + P::kSide + place[i], value + i * 512, policy);
+        for (uint32_t j = 0; j < NP; ++j) {              // a page behind the share's last: page 0, masked later
+            const uint64_t offset = static_cast<uint64_t>(__shfl_sync(0xffffffffu, entries, group % kBlock * NP + j)) * page_bytes;
+            const uint8_t* key = key_source + offset;
+            const uint8_t* value = value_source + offset;
+#pragma unroll
+            for (uint32_t i = 0; i < P::kSide / 512; ++i) {
+                copy_async_16(place[i] + fill + j * P::kStage, key + i * 512, policy);
+                copy_async_16(place[i] + fill + j * P::kStage + P::kSide, value + i * 512, policy);
+            }
         }
-        if (lane < 2) copy_async_4(scales + stage * 8 + lane * 4, scale_source + static_cast<uint64_t>(entry) * p.cache.kv_heads);
+        fill = fill + kGroup == kStages * kGroup ? 0 : fill + kGroup;
     };
 #pragma unroll
     for (uint32_t i = 0; i < kStages; ++i) {
-        if (i < my_pages) fetch(i);
+        if (i < my_groups) fetch(i);
         copies_commit();
     }
 
-    // ---- query: rows g and g + 8 of A, dimensions 64 c + 16 t + 4 ks .. + 3 in step (c, ks) ----
-    uint32_t q[NT][C][8];
-    float query_factor[NT];
-#pragma unroll
-    for (uint32_t half = 0; half < NT; ++half) {
-        uint32_t raw[C][8];
-        uint32_t largest = 0;
-        const bool there = g + 8 * half < heads;
-#pragma unroll
-        for (uint32_t c = 0; c < C; ++c) {
-            uint4 part[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
-            if (there) {
-                const uint4* row = reinterpret_cast<const uint4*>(p.query + token * p.query_token_stride +
-                                                                 (first_head + g + 8 * half) * DIM + c * 64 + t * 16);
-                part[0] = row[0];
-                part[1] = row[1];
+    // ---- query, in f16 by a power of two per head, for all warps: 8 elements a thread ----
+    {
+        constexpr uint32_t kLanes = DIM / 8;               // of a head
+        uint8_t* query = decode_smem + S::kQuery;
+        float* factors = reinterpret_cast<float*>(query + HEADS * DIM * 2);
+        for (uint32_t piece = threadIdx.x; piece < HEADS * kLanes; piece += S::kThreads) {   // whole warps, or none of one
+            const uint32_t head = piece / kLanes;
+            uint4 raw = make_uint4(0, 0, 0, 0);
+            if (head < heads) {
+                raw = *reinterpret_cast<const uint4*>(p.query + token * p.query_token_stride + (first_head + head) * DIM + piece % kLanes * 8);
             }
-            const uint32_t words[8] = {part[0].x, part[0].y, part[0].z, part[0].w, part[1].x, part[1].y, part[1].z, part[1].w};
+            const uint32_t words[4] = {raw.x, raw.y, raw.z, raw.w};
+            uint32_t largest = 0;
 #pragma unroll
-            for (uint32_t i = 0; i < 8; ++i) {
-                raw[c][i] = words[i];
+            for (uint32_t i = 0; i < 4; ++i) {
                 const uint32_t low = words[i] & 0x7fffu;
                 const uint32_t high = (words[i] >> 16) & 0x7fffu;
                 largest = max(largest, max(low < 0x7f80u ? low : 0u, high < 0x7f80u ? high : 0u));
             }
+#pragma unroll
+            for (uint32_t delta = kLanes / 2; delta > 0; delta >>= 1) largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, delta));
+            // the power of two that brings the largest into [2^11, 2^12), within what f32 can multiply by
+            const int32_t exponent = min(max(static_cast<int32_t>(largest >> 7) - 127 - 11, -126), 126);
+            const float scale = power_of_two(-exponent);
+            uint32_t halves[4];
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i) {
+                const float2 pair = bf16x2_to_float2(words[i]);
+                halves[i] = pack_f16x2(pair.x * scale, pair.y * scale);
+            }
+            *reinterpret_cast<uint4*>(query + piece * 16) = make_uint4(halves[0], halves[1], halves[2], halves[3]);
+            if (piece % kLanes == 0) factors[head] = power_of_two(exponent) * p.scale_log2;
         }
-        largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
-        largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
-        // the power of two that brings the largest into [2^11, 2^12), within what f32 can multiply by
-        const int32_t exponent = min(max(static_cast<int32_t>(largest >> 7) - 127 - 11, -126), 126);
-        const float factor = power_of_two(-exponent);
-        query_factor[half] = power_of_two(exponent) * p.scale_log2;
+        if (threadIdx.x == 0) *unassigned = 0;
+    }
+    __syncthreads();
+    // rows g and g + 8 of A, dimensions 64 c + 16 t + 4 ks .. + 3 in step (c, ks)
+    uint32_t q[NT][C][8];
+    float query_factor[NT];
+#pragma unroll
+    for (uint32_t n = 0; n < NT; ++n) {
+        const uint32_t row = smem_u32(decode_smem) + S::kQuery + (g + 8 * n) * DIM * 2 + t * 32;
 #pragma unroll
         for (uint32_t c = 0; c < C; ++c) {
 #pragma unroll
-            for (uint32_t i = 0; i < 8; ++i) {
-                const float2 pair = bf16x2_to_float2(raw[c][i]);
-                q[half][c][i] = pack_f16x2(pair.x * factor, pair.y * factor);
+            for (uint32_t h = 0; h < 2; ++h) {
+                const uint4 part = load_shared_16(row + c * 128 + h * 16);
+                q[n][c][4 * h] = part.x;
+                q[n][c][4 * h + 1] = part.y;
+                q[n][c][4 * h + 2] = part.z;
+                q[n][c][4 * h + 3] = part.w;
             }
         }
+        query_factor[n] = reinterpret_cast<const float*>(decode_smem + S::kQuery + HEADS * DIM * 2)[g + 8 * n];
     }
 
     float maximum[NT];          // of head g + 8 n, the reference of its weights (log2 units)
+    float limit[NT];            // above it the reference is raised
     float sum[NT];              // of this lane's weights
     float2 out[NT][TILES][2];   // [tile of heads][tile][row g or g + 8]: heads 2 t and 2 t + 1
 #pragma unroll
     for (uint32_t n = 0; n < NT; ++n) {
-        maximum[n] = -INFINITY;
+        maximum[n] = limit[n] = -INFINITY;
         sum[n] = 0.0f;
 #pragma unroll
         for (uint32_t i = 0; i < TILES; ++i) out[n][i][0] = out[n][i][1] = make_float2(0.0f, 0.0f);
@@ -283,75 +329,82 @@ e4m3_attention_kernel(const DecodeParams p) {
         value_at[e] = P::kSide + row * DIM + (DIM == 64 ? (((g >> 1) ^ P::turn(row)) << 4) + (g & 1) * 8 : (g ^ P::turn(row)) << 4);
     }
 
-    auto use = [&](uint32_t iteration) {
-        const uint32_t base = pages.logical(share_begin + warp + iteration * kWarps) * kPageSize;
-        const uint32_t stage = ring + iteration % kStages * P::kStage;
-        // ---- scores of two tiles of 8 keys: head g, keys key_of(k, t, 0 and 1); head g + 8, the same ----
-        float s[2][4];
+    uint32_t drain = ring;                               // ring place of the next group to use
+    auto use = [&](uint32_t group, uint32_t index, auto masked) {
+        float s[NP][2][4];
+        uint2 value[NP][4][C];
+        float value_scale[NP];
+        float factor[NP][NT];
 #pragma unroll
-        for (uint32_t k = 0; k < 2; ++k) {
+        for (uint32_t j = 0; j < NP; ++j) {
+            const uint32_t stage = drain + j * P::kStage;
+            // ---- scores of two tiles of 8 keys: head g, keys key_of(k, t, 0 and 1); head g + 8, the same ----
+            uint4 codes[2][C];
+#pragma unroll
+            for (uint32_t k = 0; k < 2; ++k) {
+#pragma unroll
+                for (uint32_t c = 0; c < C; ++c) codes[k][c] = load_shared_16(stage + key_at[c] + k * 8 * DIM);
+            }
 #pragma unroll
             for (uint32_t c = 0; c < C; ++c) {
-                const uint4 codes = load_shared_16(stage + key_at[c] + k * 8 * DIM);
-                const uint32_t words[4] = {codes.x, codes.y, codes.z, codes.w};
 #pragma unroll
                 for (uint32_t ks = 0; ks < 4; ++ks) {
-                    const uint32_t a1 = NT > 1 ? q[NT - 1][c][2 * ks] : 0u;
-                    const uint32_t a3 = NT > 1 ? q[NT - 1][c][2 * ks + 1] : 0u;
-                    if (c == 0 && ks == 0) {
-                        mma_f16_16816_first(s[k], q[0][c][0], a1, q[0][c][1], a3, e4m3x2_to_f16x2(words[0]), e4m3x2_high_to_f16x2(words[0]));
-                    } else {
-                        mma_f16_16816(s[k], q[0][c][2 * ks], a1, q[0][c][2 * ks + 1], a3, e4m3x2_to_f16x2(words[ks]),
-                                      e4m3x2_high_to_f16x2(words[ks]));
+#pragma unroll
+                    for (uint32_t k = 0; k < 2; ++k) {
+                        const uint32_t word = ks == 0 ? codes[k][c].x : ks == 1 ? codes[k][c].y : ks == 2 ? codes[k][c].z : codes[k][c].w;
+                        const uint32_t a1 = NT > 1 ? q[NT - 1][c][2 * ks] : 0u;
+                        const uint32_t a3 = NT > 1 ? q[NT - 1][c][2 * ks + 1] : 0u;
+                        if (c == 0 && ks == 0) {
+                            mma_f16_16816_first(s[j][k], q[0][c][0], a1, q[0][c][1], a3, e4m3x2_to_f16x2(word), e4m3x2_high_to_f16x2(word));
+                        } else {
+                            mma_f16_16816(s[j][k], q[0][c][2 * ks], a1, q[0][c][2 * ks + 1], a3, e4m3x2_to_f16x2(word), e4m3x2_high_to_f16x2(word));
+                        }
+                    }
+                }
+            }
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i) {
+                const uint32_t at = stage + value_at[i & 1] + (i >> 1) * 8 * DIM;
+                if constexpr (C == 1) {
+                    value[j][i][0] = load_shared_8(at);
+                } else {
+                    const uint4 both = load_shared_16(at);
+                    value[j][i][0] = make_uint2(both.x, both.y);
+                    value[j][i][C - 1] = make_uint2(both.z, both.w);
+                }
+            }
+            const uint32_t source = group % kBlock * NP + j;
+            const float key_scale = __shfl_sync(0xffffffffu, group >= block ? scales[0][0] : scales[1][0], source);
+            value_scale[j] = __shfl_sync(0xffffffffu, group >= block ? scales[0][1] : scales[1][1], source);
+            // never 0, so that -inf stays what it is (a score is below 2^28: with this factor it is 0)
+#pragma unroll
+            for (uint32_t n = 0; n < NT; ++n) factor[j][n] = fmaxf(key_scale * query_factor[n], 1.1754944e-38f);
+            if constexpr (decltype(masked)::value) {
+                const uint32_t base = pages.logical(index + j) * kPageSize;
+#pragma unroll
+                for (uint32_t i = 0; i < 4; ++i) {
+                    const uint32_t key = base + P::key_of(i >> 1, t, i & 1);
+                    if (index + j >= share_end || key > position || (key < pages.first_key && key >= p.sinks)) {
+                        // whatever lies there, a weight of 0 must not meet a NaN
+#pragma unroll
+                        for (uint32_t c = 0; c < C; ++c) value[j][i][c] = make_uint2(0, 0);
+#pragma unroll
+                        for (uint32_t n = 0; n < NT; ++n) s[j][i >> 1][2 * n + (i & 1)] = -INFINITY;
                     }
                 }
             }
         }
-        uint2 value[4][C];
-#pragma unroll
-        for (uint32_t i = 0; i < 4; ++i) {
-            const uint32_t at = stage + value_at[i & 1] + (i >> 1) * 8 * DIM;
-            if constexpr (C == 1) {
-                value[i][0] = load_shared_8(at);
-            } else {
-                const uint4 both = load_shared_16(at);
-                value[i][0] = make_uint2(both.x, both.y);
-                value[i][C - 1] = make_uint2(both.z, both.w);
-            }
-        }
-        const uint2 scale_bits = load_shared_8(scales + iteration % kStages * 8);
-        const float key_scale = __uint_as_float(scale_bits.x);
-        const float value_scale = __uint_as_float(scale_bits.y);
-        // ---- mask: only pages at an edge of what the token sees have one ----
-        uint32_t seen = 0xfu;
-        const bool whole = base + kPageSize - 1 <= position && (base >= pages.first_key || base + kPageSize <= p.sinks);
-        if (!whole) {
-            seen = 0;
-#pragma unroll
-            for (uint32_t i = 0; i < 4; ++i) {
-                const uint32_t key = base + P::key_of(i >> 1, t, i & 1);
-                if (key <= position && (key >= pages.first_key || key < p.sinks)) {
-                    seen |= 1u << i;
-                } else {
-                    // whatever lies there, a weight of 0 must not meet a NaN
-#pragma unroll
-                    for (uint32_t c = 0; c < C; ++c) value[i][c] = make_uint2(0, 0);
-#pragma unroll
-                    for (uint32_t n = 0; n < NT; ++n) s[i >> 1][2 * n + (i & 1)] = -INFINITY;
-                }
-            }
-        }
-        // ---- weights ----
-        uint32_t weights[NT][2];
-        float factor[NT];
+        // ---- the reference maximum ----
         float most[NT];
         bool above = false;
 #pragma unroll
         for (uint32_t n = 0; n < NT; ++n) {
-            factor[n] = key_scale * query_factor[n];
-            // a factor of 0 makes the product with -inf a NaN, which the comparison passes over
-            most[n] = fmaxf(max3(s[0][2 * n], s[0][2 * n + 1], s[1][2 * n]), s[1][2 * n + 1]) * factor[n];
-            above = above || most[n] > maximum[n] + kHeadroom;
+            most[n] = -INFINITY;
+#pragma unroll
+            for (uint32_t j = 0; j < NP; ++j) {
+                most[n] = fmaxf(most[n], fmaxf(max3(s[j][0][2 * n], s[j][0][2 * n + 1], s[j][1][2 * n]), s[j][1][2 * n + 1]) * factor[j][n]);
+            }
+            above = above || most[n] > limit[n];
         }
         if (__any_sync(0xffffffffu, above)) {
 #pragma unroll
@@ -362,6 +415,7 @@ e4m3_attention_kernel(const DecodeParams p) {
                 // a row that has seen nothing yet keeps its sums of 0: exp2(-inf - -inf) is no factor
                 const float shrink = most[n] == maximum[n] ? 1.0f : fast_exp2(maximum[n] - most[n]);
                 maximum[n] = most[n];
+                limit[n] = most[n] + kHeadroom;
                 sum[n] *= shrink;
                 const float low = __shfl_sync(0xffffffffu, shrink, 8 * t);
                 const float high = __shfl_sync(0xffffffffu, shrink, 8 * t + 4);
@@ -372,56 +426,72 @@ e4m3_attention_kernel(const DecodeParams p) {
                 }
             }
         }
+        // ---- weights ----
+        uint32_t weights[NP][NT][2];
 #pragma unroll
-        for (uint32_t n = 0; n < NT; ++n) {
-            float w[4];
+        for (uint32_t j = 0; j < NP; ++j) {
 #pragma unroll
-            for (uint32_t i = 0; i < 4; ++i) w[i] = fast_exp2(fmaf(s[i >> 1][2 * n + (i & 1)], factor[n], -maximum[n]));
-            if (!whole) {
+            for (uint32_t n = 0; n < NT; ++n) {
+                float w[4];
 #pragma unroll
-                for (uint32_t i = 0; i < 4; ++i) w[i] = (seen >> i) & 1 ? w[i] : 0.0f;
+                for (uint32_t i = 0; i < 4; ++i) w[i] = fast_exp2(fmaf(s[j][i >> 1][2 * n + (i & 1)], factor[j][n], -maximum[n]));
+                weights[j][n][0] = pack_f16x2(w[0], w[1]);
+                weights[j][n][1] = pack_f16x2(w[2], w[3]);
+                // the sum of the weights before their rounding to 11 bits, which averages out over the keys
+                sum[n] += (w[0] + w[1]) + (w[2] + w[3]);
             }
-            weights[n][0] = pack_f16x2(w[0], w[1]);
-            weights[n][1] = pack_f16x2(w[2], w[3]);
-            // the sum of the weights before their rounding to 11 bits, which averages out over the keys
-            sum[n] += (w[0] + w[1]) + (w[2] + w[3]);
         }
         // ---- O^T += scale * V^T P^T ----
 #pragma unroll
-        for (uint32_t tile = 0; tile < TILES; tile += 2) {
-            // dimensions 2 tile .. 2 tile + 3 of this lane's DIM / 8: one byte each of a word
-            uint32_t word[4];
+        for (uint32_t j = 0; j < NP; ++j) {
 #pragma unroll
-            for (uint32_t k = 0; k < 4; ++k) word[k] = tile & 2 ? value[k][tile / 4].y : value[k][tile / 4].x;
-            const uint32_t low[2] = {__byte_perm(word[0], word[1], 0x5140), __byte_perm(word[2], word[3], 0x5140)};
-            const uint32_t high[2] = {__byte_perm(word[0], word[1], 0x7362), __byte_perm(word[2], word[3], 0x7362)};
+            for (uint32_t tile = 0; tile < TILES; tile += 2) {
+                // dimensions 2 tile .. 2 tile + 3 of this lane's DIM / 8: one byte each of a word
+                uint32_t word[4];
 #pragma unroll
-            for (uint32_t half = 0; half < 2; ++half) {
-                const uint32_t* pair = half ? high : low;
-                const uint32_t a0 = e4m3x2_to_f16x2(pair[0]);
-                const uint32_t a1 = e4m3x2_high_to_f16x2(pair[0]);
-                const uint32_t a2 = e4m3x2_to_f16x2(pair[1]);
-                const uint32_t a3 = e4m3x2_high_to_f16x2(pair[1]);
+                for (uint32_t k = 0; k < 4; ++k) word[k] = tile & 2 ? value[j][k][tile / 4].y : value[j][k][tile / 4].x;
+                const uint32_t low[2] = {__byte_perm(word[0], word[1], 0x5140), __byte_perm(word[2], word[3], 0x5140)};
+                const uint32_t high[2] = {__byte_perm(word[0], word[1], 0x7362), __byte_perm(word[2], word[3], 0x7362)};
 #pragma unroll
-                for (uint32_t n = 0; n < NT; ++n) {
-                    float d[4];
-                    mma_f16_16816_first(d, a0, a1, a2, a3, weights[n][0], weights[n][1]);
+                for (uint32_t half = 0; half < 2; ++half) {
+                    const uint32_t* pair = half ? high : low;
+                    const uint32_t a0 = e4m3x2_to_f16x2(pair[0]);
+                    const uint32_t a1 = e4m3x2_high_to_f16x2(pair[0]);
+                    const uint32_t a2 = e4m3x2_to_f16x2(pair[1]);
+                    const uint32_t a3 = e4m3x2_high_to_f16x2(pair[1]);
 #pragma unroll
-                    for (uint32_t h = 0; h < 2; ++h) {
-                        float2& o = out[n][tile + half][h];
-                        o = fma_pair(make_float2(d[2 * h], d[2 * h + 1]), value_scale, o);
+                    for (uint32_t n = 0; n < NT; ++n) {
+                        float d[4];
+                        mma_f16_16816_first(d, a0, a1, a2, a3, weights[j][n][0], weights[j][n][1]);
+#pragma unroll
+                        for (uint32_t h = 0; h < 2; ++h) {
+                            float2& o = out[n][tile + half][h];
+                            o = fma_pair(make_float2(d[2 * h], d[2 * h + 1]), value_scale[j], o);
+                        }
                     }
                 }
             }
         }
     };
 
-    for (uint32_t iteration = 0; iteration < my_pages; ++iteration) {
+    uint32_t index = share_begin + warp * NP;
+    for (uint32_t group = 0; group < my_groups; ++group) {
         copies_wait<kStages - 1>();
         __syncwarp();                                  // every lane's pieces are there
-        use(iteration);
+        const uint32_t first = pages.logical(index) * kPageSize;
+        // Only pages at an edge of what the token sees have a mask.  (A group that is no run of pages has an edge: it holds the last
+        // page of the first tokens, or pages in front of the window's.)
+        const bool whole = index + NP <= share_end && first + NP * kPageSize - 1 <= position &&
+                           (first >= pages.first_key || first + NP * kPageSize <= p.sinks);
+        if (whole) {
+            use(group, index, std::false_type());
+        } else {
+            use(group, index, std::true_type());
+        }
+        index += kWarps * NP;
+        drain = drain + kGroup == ring + kStages * kGroup ? ring : drain + kGroup;
         __syncwarp();                                  // and read by all
-        if (iteration + kStages < my_pages) fetch(iteration + kStages);
+        if (group + kStages < my_groups) fetch(group + kStages);
         copies_commit();
     }
     if (__any_sync(0xffffffffu, bad != 0) && lane == 0) *unassigned = 1;
@@ -438,12 +508,13 @@ e4m3_attention_kernel(const DecodeParams p) {
             mine[(8 * n + g) * STRIDE + DIM] = maximum[n];
             mine[(8 * n + g) * STRIDE + DIM + 1] = sum[n];
         }
+        if (8 * n + 2 * t < heads) {
+            float4* low = reinterpret_cast<float4*>(mine + (8 * n + 2 * t) * STRIDE + (DIM / 8) * g);
+            float4* high = reinterpret_cast<float4*>(mine + (8 * n + 2 * t + 1) * STRIDE + (DIM / 8) * g);
 #pragma unroll
-        for (uint32_t i = 0; i < TILES; ++i) {
-#pragma unroll
-            for (uint32_t h = 0; h < 2; ++h) {
-                mine[(8 * n + 2 * t) * STRIDE + (DIM / 8) * g + 2 * i + h] = out[n][i][h].x;
-                mine[(8 * n + 2 * t + 1) * STRIDE + (DIM / 8) * g + 2 * i + h] = out[n][i][h].y;
+            for (uint32_t i = 0; i < TILES; i += 2) {
+                low[i / 2] = make_float4(out[n][i][0].x, out[n][i][1].x, out[n][i + 1][0].x, out[n][i + 1][1].x);
+                high[i / 2] = make_float4(out[n][i][0].y, out[n][i][1].y, out[n][i + 1][0].y, out[n][i + 1][1].y);
             }
         }
     }
@@ -506,15 +577,39 @@ e4m3_attention_kernel(const DecodeParams p) {
     cluster_barrier();      // nobody leaves while its share is read
 }
 
-template <uint32_t DIM, uint32_t HEADS>
+template <uint32_t DIM, uint32_t HEADS, uint32_t WARPS>
 cudaError_t launch_shape(cudaStream_t stream, const DecodeParams& params, uint64_t blocks) {
-    using S = Shape<DIM, HEADS>;
-    const cudaError_t status = allow_shared_memory<e4m3_attention_kernel<DIM, HEADS>>(S::kBytes);
+    using S = Shape<DIM, HEADS, WARPS>;
+    const cudaError_t status = allow_shared_memory<e4m3_attention_kernel<DIM, HEADS, WARPS>, true>(S::kBytes);
     if (status != cudaSuccess) {
         return status;
     }
-    return launch_kernel(e4m3_attention_kernel<DIM, HEADS>, static_cast<unsigned int>(blocks), S::kThreads, S::kBytes, stream,
+    return launch_kernel(e4m3_attention_kernel<DIM, HEADS, WARPS>, static_cast<unsigned int>(blocks), S::kThreads, S::kBytes, stream,
                          params.splits, params);
+}
+
+// CTAs of 4 warps, their pages shared by a cluster of as many (up to 16) as fill the SMs once, a quarter over, while each warp
+// has 8 pages or more: a cluster costs about as much as 6 pages of one warp (23 padded to 32 tokens through a window of 4096, 2 KV heads of
+// 128: 4 CTAs 18.1, 8 CTAs 14.9, 16 CTAs 24.8 us; 3 tokens at 20480..65536: 4 CTAs 69, 8 CTAs 47, 16 CTAs 36.9 us; 32 tokens at 64..400:
+// 1 CTA 6.5, 2 CTAs 7.5 us).  Where that leaves half of the warps' places free, CTAs of 8 warps (1 token at 8000: 8.2 against 8.9 us;
+// 32 tokens at 64..400: 5.8 against 6.5 us), in clusters of 8 at most, which gain as much as 16.
+template <uint32_t DIM, uint32_t HEADS>
+cudaError_t launch_heads(cudaStream_t stream, DecodeParams params, uint64_t items, uint64_t pages) {
+    using S = Shape<DIM, HEADS, 4>;
+    constexpr uint64_t kSms = 148;
+    constexpr uint64_t kResident = kSms * S::kPerSm;
+    while (params.splits_log2 < 4 && (items << (params.splits_log2 + 1)) <= kResident + kResident / 4 &&
+           pages >= (8ull * 4 << params.splits_log2)) {
+        ++params.splits_log2;
+    }
+    const bool wide = (items << params.splits_log2) * 8 <= kSms * S::kWarpsPerSm;
+    if (wide && params.splits_log2 == 4) params.splits_log2 = 3;
+    params.splits = 1u << params.splits_log2;
+    const uint64_t blocks = items << params.splits_log2;
+    if (blocks > 0x7fffffffu) {
+        return cudaErrorInvalidConfiguration;
+    }
+    return wide ? launch_shape<DIM, HEADS, 8>(stream, params, blocks) : launch_shape<DIM, HEADS, 4>(stream, params, blocks);
 }
 
 }  // namespace
@@ -539,22 +634,19 @@ cudaError_t launch_e4m3_attention(cudaStream_t stream, const E4m3AttentionLaunch
     params.sinks = launch.sinks;
     params.scale_log2 = launch.scale * kLog2e;
     const uint64_t items = static_cast<uint64_t>(launch.num_tokens) * launch.cache.kv_heads * params.chunks;
+    if (items > 0x7fffffffu) {
+        return cudaErrorInvalidConfiguration;
+    }
     // pages of the longest context that a token can see
     uint64_t longest = launch.maximum_context_tokens;
     if (launch.window != 0 && longest > static_cast<uint64_t>(launch.window) + launch.sinks) {
         longest = static_cast<uint64_t>(launch.window) + launch.sinks + kPageSize;
     }
     const uint64_t pages = (longest + kPageSize - 1) / kPageSize;
-    params.splits = 1;
-    while (params.splits < 8 && items * params.splits < 592 && pages >= 2 * params.splits * 8) params.splits *= 2;
-    const uint64_t blocks = items * params.splits;
-    if (blocks > 0x7fffffffu) {
-        return cudaErrorInvalidConfiguration;
-    }
     if (launch.cache.head_dim == 64) {
-        return params.group <= 8 ? launch_shape<64, 8>(stream, params, blocks) : launch_shape<64, 16>(stream, params, blocks);
+        return params.group <= 8 ? launch_heads<64, 8>(stream, params, items, pages) : launch_heads<64, 16>(stream, params, items, pages);
     }
-    return params.group <= 8 ? launch_shape<128, 8>(stream, params, blocks) : launch_shape<128, 16>(stream, params, blocks);
+    return params.group <= 8 ? launch_heads<128, 8>(stream, params, items, pages) : launch_heads<128, 16>(stream, params, items, pages);
 }
 
 }  // namespace lfm25

@@ -39,8 +39,9 @@ cudaError_t launch_kernel(void (*kernel)(Parameters...), unsigned int blocks, un
     return cudaLaunchKernelEx(&config, kernel, static_cast<Parameters>(arguments)...);
 }
 
-// Dynamic shared memory of a kernel beyond 48 KB, allowed once per device: the call costs as much as a small launch.
-template <auto Kernel>
+// Dynamic shared memory of a kernel beyond 48 KB, and clusters of more than 8 CTAs, allowed once per device: the calls cost as much
+// as a small launch.
+template <auto Kernel, bool LargeClusters = false>
 cudaError_t allow_shared_memory(size_t bytes) {
     static std::atomic<uint64_t> done{0};
     int device = 0;
@@ -50,6 +51,9 @@ cudaError_t allow_shared_memory(size_t bytes) {
         return status;
     }
     status = cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
+    if (status == cudaSuccess && LargeClusters) {
+        status = cudaFuncSetAttribute(Kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    }
     if (status == cudaSuccess) {
         done.fetch_or(bit, std::memory_order_relaxed);
     }
