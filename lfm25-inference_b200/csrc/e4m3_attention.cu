@@ -222,11 +222,13 @@ e4m3_attention_kernel(const DecodeParams p) {
                 bad = 1;                                 // page 0 in its place; the token gets no result
                 entries = 0;
             }
+            // a page that is not there is masked, and its scales are 0: a weight of 0 times a stray scale could be NaN
+            const bool exists = share_begin + (warp + (group + lane / NP) * kWarps) * NP + lane % NP < share_end;
             const uint64_t tile = static_cast<uint64_t>(entries) * p.cache.kv_heads + kv_head;
             scales[1][0] = scales[0][0];
             scales[1][1] = scales[0][1];
-            scales[0][0] = __ldg(p.cache.key_scales + tile);
-            scales[0][1] = __ldg(p.cache.value_scales + tile);
+            scales[0][0] = exists ? __ldg(p.cache.key_scales + tile) : 0.0f;
+            scales[0][1] = exists ? __ldg(p.cache.value_scales + tile) : 0.0f;
         }
 #pragma unroll
         for (uint32_t j = 0; j < NP; ++j) {              // a page behind the share's last: page 0, masked later

@@ -1,21 +1,21 @@
 // Attention of prompts over the 8-bit paged cache on the 5th-generation tensor cores (tcgen05 + tensor memory).
 //
-// A CTA owns 128 rows: consecutive tokens of one segment times the query heads of one KV head (32 tokens x 4 heads), or one
-// share of their keys.  Keys come in stages of 64 (4 pages):
+// A CTA owns two tiles of 128 rows: consecutive tokens of one segment times the query heads of one KV head (2 x 32 tokens x 4
+// heads), or one share of their keys.  Keys come in stages of 64 (4 pages), converted once for both tiles:
 //
-//   warps 4-7   pages: E4M3 codes from global memory to registers one stage ahead, converted into the operands of the MMA in
+//   warps 8-11  pages: E4M3 codes from global memory to registers one stage ahead, converted into the operands of the MMA in
 //               shared memory (128-byte swizzle): K to f16 as it is, V to bf16 with its page's scale, both without a rounding
-//   warp 8      one thread issues, per stage, S = Q K^T (kind::f16 on f16 operands) and, once the weights are there,
+//   warp 12     one thread issues, per stage and tile, S = Q K^T (kind::f16 on f16 operands) and, once the weights are there,
 //               O += P V (bf16, P read from tensor memory, V as an MN-major operand); S of the next stage in front of P V of
 //               this one, so that the tensor core works while the softmax does
-//   warps 0-3   one thread a row: tcgen05.ld S, page scales, mask, exp2, weights back over the scores they came from
+//   warps 0-7   one thread a row, four warps a tile: tcgen05.ld S, page scales, mask, exp2, weights back over the scores
 //
 // O stays in tensor memory: the maximum that weights refer to is only raised when a score exceeds it by more than 8 (log2), and
 // only then is O read, scaled and stored.  The query is brought to f16 by a power of two per row, which the scores get back
 // together with the page's scale in the multiply-add in front of the exponential.
 //
-// What bounds it at 64 dimensions is the exponentials (128 rows x 64 keys at 16 a cycle and SM: 512 cycles a stage, the two
-// products 256); 128 dimensions double the products.  Two CTAs share an SM, so that one's softmax fills the other's waits.
+// What bounds it at 64 dimensions is the instructions of softmax and conversion, behind them the exponentials (128 rows x 64 keys
+// at 16 a cycle and SM: 512 cycles a stage and tile; the two products 256).
 //
 // Rows of a mask edge test bits of their own; a NaN among the values is replaced in the operand (a weight of 0 times NaN is
 // NaN) and remembered by key: a row that sees it becomes NaN as a whole.  Few tiles: a cluster shares a tile's keys and joins
@@ -32,14 +32,17 @@ namespace lfm25 {
 
 namespace {
 
-constexpr uint32_t kRows = 128;
+constexpr uint32_t kRows = 128;                            // of a tile
+constexpr uint32_t kTiles = 2;                             // of a CTA
 constexpr uint32_t kPagesPerStage = 4;
 constexpr uint32_t kKeys = kPagesPerStage * kPageSize;     // 64
-constexpr uint32_t kThreads = 288;
-constexpr uint32_t kBuffers = 2;
-constexpr uint32_t kTmemColumns = 256;
-constexpr uint32_t kColumnS = 0;                           // two buffers of 64; weights take the first 32 columns of theirs
-constexpr uint32_t kColumnO = 128;
+constexpr uint32_t kSoftmaxWarps = 4 * kTiles;
+constexpr uint32_t kPageWarps = 4;
+constexpr uint32_t kThreads = (kSoftmaxWarps + kPageWarps + 1) * 32;
+constexpr uint32_t kBuffers = 3;
+constexpr uint32_t kTmemColumns = 512;
+constexpr uint32_t kColumnS = 0;                           // for each tile two buffers of 64; weights take the first 32 columns of theirs
+constexpr uint32_t kColumnO = 256;
 constexpr float kHeadroom = 8.0f;
 constexpr uint32_t kTile = kKeys * 128;                    // 64 keys x 64 dimensions of 2 bytes
 
@@ -62,6 +65,7 @@ struct PromptParams {
     uint32_t chunk_heads;    // query heads of a tile
     uint32_t chunks;
     uint32_t tile_tokens;    // kRows / chunk_heads
+    uint32_t cta_tokens;     // kTiles of that
     uint32_t splits;         // CTAs of a cluster
     uint32_t window;
     uint32_t sinks;
@@ -73,30 +77,63 @@ struct PromptParams {
 template <uint32_t DIM>
 struct Layout {
     static constexpr uint32_t kParts = DIM / 64;
-    static constexpr uint32_t kQ = 0;                                         // [part][row] of 128 bytes
-    static constexpr uint32_t kK = kQ + kParts * kRows * 128;                 // [buffer][part][key]
+    static constexpr uint32_t kQ = 0;                                         // [tile][part][row] of 128 bytes
+    static constexpr uint32_t kK = kQ + kTiles * kParts * kRows * 128;        // [buffer][part][key]
     static constexpr uint32_t kV = kK + kBuffers * kParts * kTile;
     static constexpr uint32_t kControl = kV + kBuffers * kParts * kTile;
-    static constexpr uint32_t kBytes = kControl + 512 + 3 * kRows * 4;
+    static constexpr uint32_t kBytes = kControl + 512 + 3 * kTiles * kRows * 4;
     static constexpr uint32_t kAlloc = kBytes + 1024;
+    static_assert(kControl >= kTiles * kRows * DIM * 4, "the sums that a cluster joins lie where the operands were");
 };
 
 // beside the operands
 struct Control {
-    uint64_t full[kBuffers];       // operands of a stage are there
-    uint64_t empty[kBuffers];      // its P V is done with them
-    uint64_t scores[2];
-    uint64_t weights[2];
-    uint64_t product;              // P V of a stage is complete
-    uint64_t drained;              // after a wait ran out: no MMA is in flight any more
+    uint64_t full[kBuffers];           // operands of a stage are there
+    uint64_t empty[kBuffers];          // both tiles' P V are done with them
+    uint64_t scores[kTiles][2];
+    uint64_t weights[kTiles][2];
+    uint64_t product[kTiles];          // P V of a stage is complete
+    uint64_t drained;                  // after a wait ran out: no MMA is in flight any more
     alignas(16) float key_scales[kBuffers][kPagesPerStage];   // read four at a time
-    alignas(16) unsigned long long nan_keys[kBuffers][4];   // of each page warp: keys of the stage with a NaN among their values
-    uint32_t bad_pages[kBuffers];  // unassigned pages of the stage, one bit each
+    alignas(16) unsigned long long nan_keys[kBuffers][kPageWarps];   // of each page warp: keys with a NaN among their values
+    uint32_t bad_pages[kBuffers];      // unassigned pages of the stage, one bit each
     uint32_t tmem;
     uint32_t abort;
 };
 static_assert(offsetof(Control, key_scales) % 16 == 0, "scales are read 16 bytes at a time");
 static_assert(sizeof(Control) <= 512, "the control block has 512 bytes");
+
+// Two f32 in a register pair, for the packed instructions: operands that many of them share are packed once.
+__device__ __forceinline__ uint64_t pair_of(float low, float high) {
+    uint64_t v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(low), "f"(high));
+    return v;
+}
+__device__ __forceinline__ float2 pair_out(uint64_t v) {
+    float2 out;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(out.x), "=f"(out.y) : "l"(v));
+    return out;
+}
+__device__ __forceinline__ uint64_t pair_fma(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t v;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(a), "l"(b), "l"(c));
+    return v;
+}
+__device__ __forceinline__ uint64_t pair_add(uint64_t a, uint64_t b) {
+    uint64_t v;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
+    return v;
+}
+__device__ __forceinline__ uint64_t pair_mul(uint64_t a, uint64_t b) {
+    uint64_t v;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
+    return v;
+}
+__device__ __forceinline__ uint32_t add_f16x2(uint32_t a, uint32_t b) {
+    uint32_t v;
+    asm("add.rn.f16x2 %0, %1, %2;" : "=r"(v) : "r"(a), "r"(b));
+    return v;
+}
 
 __device__ __forceinline__ void umma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
@@ -135,7 +172,7 @@ __device__ __forceinline__ uint32_t visible_bits(uint32_t base, uint32_t positio
 }
 
 template <uint32_t DIM>
-__global__ void __launch_bounds__(kThreads, 2)
+__global__ void __launch_bounds__(kThreads, 1)
 e4m3_prompt_attention_kernel(const PromptParams p) {
     using L = Layout<DIM>;
     const uint32_t warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
@@ -162,7 +199,7 @@ e4m3_prompt_attention_kernel(const PromptParams p) {
             end = __ldg(p.segment_offsets + segment + 1);
             if (end <= begin || end > p.num_tokens) end = begin = 0;
         }
-        const uint32_t tiles = (end - begin + p.tile_tokens - 1) / p.tile_tokens;
+        const uint32_t tiles = (end - begin + p.cta_tokens - 1) / p.cta_tokens;
         uint32_t upto = tiles;
 #pragma unroll
         for (uint32_t delta = 1; delta < 32; delta <<= 1) {
@@ -183,23 +220,30 @@ e4m3_prompt_attention_kernel(const PromptParams p) {
     if (!found) {
         return;
     }
-    const uint32_t tile_begin = segment_begin + slot * p.tile_tokens;
-    const uint32_t tile_end = min(tile_begin + p.tile_tokens, segment_end);
+    const uint32_t cta_begin = segment_begin + slot * p.cta_tokens;
+    const uint32_t cta_end = min(cta_begin + p.cta_tokens, segment_end);
     const uint32_t table_row = p.request_slots[segment_begin];
     const uint64_t origin = p.position_ids[segment_begin];            // position of the segment's first token
-    const uint64_t first_wide = origin + (tile_begin - segment_begin);
-    const uint64_t most = p.block_table_stride * kPageSize;
-    if (table_row >= p.block_table_rows || first_wide >= most) {
+    const uint64_t first_wide = origin + (cta_begin - segment_begin);
+    const uint64_t most_positions = p.block_table_stride * kPageSize;
+    if (table_row >= p.block_table_rows || first_wide >= most_positions) {
         return;
     }
     const uint32_t first_position = static_cast<uint32_t>(first_wide);
     // tokens behind the end of the table have no result; those in front of it do
-    const uint32_t last_position = static_cast<uint32_t>(min(first_wide + (tile_end - tile_begin), most) - 1);
+    const uint32_t last_position = static_cast<uint32_t>(min(first_wide + (cta_end - cta_begin), most_positions) - 1);
     const VisiblePages pages(first_position, last_position, p.window, p.sinks);
     const uint32_t* __restrict__ table = p.block_tables + static_cast<uint64_t>(table_row) * p.block_table_stride;
     const uint32_t all_stages = (pages.count + kPagesPerStage - 1) / kPagesPerStage;
     const uint32_t begin_stage = static_cast<uint32_t>(static_cast<uint64_t>(all_stages) * split / p.splits);
     const uint32_t stages = static_cast<uint32_t>(static_cast<uint64_t>(all_stages) * (split + 1) / p.splits) - begin_stage;
+    // stages that a tile takes part in: the first one's tokens see less, the second one may have no tokens
+    auto stages_of = [&](uint32_t tile) -> uint32_t {
+        if (tile * p.tile_tokens > last_position - first_position) return 0;
+        const uint32_t last = min(last_position, first_position + (tile + 1) * p.tile_tokens - 1);
+        const uint32_t until = (pages.sink_pages + last / kPageSize - pages.first_page + kPagesPerStage) / kPagesPerStage;
+        return min(until > begin_stage ? until - begin_stage : 0u, stages);
+    };
 
     extern __shared__ uint8_t prompt_smem[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(prompt_smem) + 1023) & ~uintptr_t(1023));
@@ -211,33 +255,36 @@ e4m3_prompt_attention_kernel(const PromptParams p) {
     const uint32_t bar_empty = smem_u32(control->empty);
     const uint32_t bar_scores = smem_u32(control->scores);
     const uint32_t bar_weights = smem_u32(control->weights);
-    const uint32_t bar_product = smem_u32(&control->product);
+    const uint32_t bar_product = smem_u32(control->product);
 
     if (threadIdx.x == 0) {
-        for (uint32_t i = 0; i < 2; ++i) {
-            mbar_init(bar_full + 8 * i, 4);
+        for (uint32_t i = 0; i < kBuffers; ++i) {
+            mbar_init(bar_full + 8 * i, kPageWarps);
             mbar_init(bar_empty + 8 * i, 1);
+        }
+        for (uint32_t i = 0; i < 2 * kTiles; ++i) {
             mbar_init(bar_scores + 8 * i, 1);
             mbar_init(bar_weights + 8 * i, 4);
         }
-        mbar_init(bar_product, 1);
+        for (uint32_t i = 0; i < kTiles; ++i) mbar_init(bar_product + 8 * i, 1);
         mbar_init(smem_u32(&control->drained), 1);
         control->abort = 0;
         fence_barrier_init();
     }
-    if (warp == 8) {
+    if (warp == kSoftmaxWarps + kPageWarps) {
         tmem_allocate(smem_u32(&control->tmem), kTmemColumns);
     }
 
     // ---- rows: this thread's token and head, its query in f16 ----
-    const uint32_t row = threadIdx.x;                    // of the softmax warps
-    const uint32_t row_token = tile_begin + row / p.chunk_heads;
+    const uint32_t tile = (warp / 4) % kTiles;           // of the softmax warps
+    const uint32_t row = threadIdx.x % kRows;            // of the tile
+    const uint32_t row_token = cta_begin + tile * p.tile_tokens + row / p.chunk_heads;
     const uint32_t head = chunk * p.chunk_heads + row % p.chunk_heads;   // of the group
-    const uint64_t row_wide = first_wide + (row_token - tile_begin);
+    const uint64_t row_wide = first_wide + (row_token - cta_begin);
     bool live = false;
     float row_factor = 0.0f;
-    if (warp < 4) {
-        live = row < p.tile_tokens * p.chunk_heads && row_token < tile_end && head < p.group && row_wide < most;
+    if (warp < kSoftmaxWarps) {
+        live = row < p.tile_tokens * p.chunk_heads && row_token < cta_end && head < p.group && row_wide < most_positions;
         if (live) live = p.request_slots[row_token] == table_row && p.position_ids[row_token] == row_wide;
         const __nv_bfloat16* source = p.query + row_token * p.query_token_stride + static_cast<size_t>(kv_head * p.group + head) * DIM;
         // two passes over the row, so that it need not stay in registers
@@ -266,7 +313,7 @@ e4m3_prompt_attention_kernel(const PromptParams p) {
                 const float2 pair = bf16x2_to_float2(words[i]);
                 half[i] = pack_f16x2(pair.x * factor, pair.y * factor);
             }
-            store_shared(base + L::kQ + (c / 8) * (kRows * 128) + row * 128 + (((c % 8) ^ (row & 7)) << 4),
+            store_shared(base + L::kQ + (tile * L::kParts + c / 8) * (kRows * 128) + row * 128 + (((c % 8) ^ (row & 7)) << 4),
                          make_uint4(half[0], half[1], half[2], half[3]));
         }
         fence_proxy_async_smem();
@@ -283,55 +330,58 @@ e4m3_prompt_attention_kernel(const PromptParams p) {
     bool lost = false;           // sees an unassigned page
     bool ok = true;
 
-    if (warp >= 4 && warp < 8) {
+    if (warp >= kSoftmaxWarps && warp < kSoftmaxWarps + kPageWarps) {
         // -------------------------------------------------------------------------------- pages
         constexpr uint32_t kPieces = DIM / 16;                       // of 16 codes, of a key
         constexpr uint32_t kLoads = kKeys * kPieces / 128;           // a thread, for K and for V
-        const uint32_t thread = threadIdx.x - 128;
-        const uint32_t page_warp = warp - 4;
+        constexpr uint32_t kBlock = 32 / kPagesPerStage;             // stages whose table entries the lanes hold
+        const uint32_t page_warp = warp - kSoftmaxWarps;
+        const uint32_t thread = page_warp * 32 + lane;
+        // load i is piece i * 128 + thread: for a warp one page of the stage, and the same place within it in every stage
+        const uint32_t page_bytes = p.cache.kv_heads * kPageSize * DIM;
+        const uint32_t inside = kv_head * kPageSize * DIM + (thread / kPieces) % kPageSize * DIM + thread % kPieces * 16;
+        const uint8_t* key_source = p.cache.key_codes + inside;
+        const uint8_t* value_source = p.cache.value_codes + inside;
+        auto page_of = [&](uint32_t i) -> uint32_t { return (i * 128 + page_warp * 32) / kPieces / kPageSize; };
+        auto look_up = [&](uint32_t stage) -> uint32_t {             // entry of this lane's page of the stages from `stage` on
+            const uint32_t index = (begin_stage + stage) * kPagesPerStage + lane;
+            return index < pages.count ? __ldg(table + pages.logical(index)) : 0;
+        };
         uint4 key_codes[kLoads];
         uint4 value_codes[kLoads];
-        float value_scale[kLoads];
-        float key_scale = 0.0f;
-        uint32_t bad = 0;
+        uint32_t entries = 0;
+        uint32_t coming = look_up(0);
+        uint32_t bad[2] = {0, 0};                                    // of the stages at hand and of those before
+        float key_scale[2] = {0.0f, 0.0f};
+        float value_scale[2] = {0.0f, 0.0f};
         auto load = [&](uint32_t stage) {
-            const uint32_t first = (begin_stage + stage) * kPagesPerStage;
-            bad = 0;
+            if (stage % kBlock == 0) {
+                entries = coming;
+                coming = look_up(stage + kBlock);
+                bad[1] = bad[0];
+                bad[0] = __ballot_sync(0xffffffffu, entries >= p.cache.num_pages);
+                const bool exists = (begin_stage + stage) * kPagesPerStage + lane < pages.count && entries < p.cache.num_pages;
+                if (!exists) entries = 0;      // page 0 in its place, times 0: no row sees it, or those that do get no result
+                const uint64_t at = static_cast<uint64_t>(entries) * p.cache.kv_heads + kv_head;
+                key_scale[1] = key_scale[0];
+                value_scale[1] = value_scale[0];
+                key_scale[0] = exists ? __ldg(p.cache.key_scales + at) : 0.0f;
+                value_scale[0] = exists ? __ldg(p.cache.value_scales + at) : 0.0f;
+            }
 #pragma unroll
             for (uint32_t i = 0; i < kLoads; ++i) {
-                const uint32_t piece = i * 128 + thread;
-                const uint32_t key = piece / kPieces;
-                const uint32_t index = first + key / kPageSize;
-                uint32_t entry = 0xffffffffu;
-                if (index < pages.count) {
-                    entry = __ldg(table + pages.logical(index));
-                    if (entry >= p.cache.num_pages) bad |= 1u << (key / kPageSize);
-                }
-                if (entry < p.cache.num_pages) {
-                    const size_t tile = static_cast<size_t>(entry) * p.cache.kv_heads + kv_head;
-                    const size_t offset = tile * (kPageSize * DIM) + (key % kPageSize) * DIM + (piece % kPieces) * 16;
-                    key_codes[i] = __ldg(reinterpret_cast<const uint4*>(p.cache.key_codes + offset));
-                    value_codes[i] = __ldg(reinterpret_cast<const uint4*>(p.cache.value_codes + offset));
-                    value_scale[i] = __ldg(p.cache.value_scales + tile);
-                } else {
-                    key_codes[i] = value_codes[i] = make_uint4(0, 0, 0, 0);
-                    value_scale[i] = 0.0f;
-                }
-            }
-            if (thread < kPagesPerStage) {
-                const uint32_t index = first + thread;
-                key_scale = 0.0f;
-                if (index < pages.count) {
-                    const uint32_t entry = __ldg(table + pages.logical(index));
-                    if (entry < p.cache.num_pages) {
-                        key_scale = __ldg(p.cache.key_scales + static_cast<size_t>(entry) * p.cache.kv_heads + kv_head);
-                    }
-                }
+                const uint64_t offset = static_cast<uint64_t>(__shfl_sync(0xffffffffu, entries, stage % kBlock * kPagesPerStage + page_of(i))) * page_bytes;
+                key_codes[i] = __ldg(reinterpret_cast<const uint4*>(key_source + offset));
+                value_codes[i] = __ldg(reinterpret_cast<const uint4*>(value_source + offset));
             }
         };
+        // where a piece's 32 bytes go: two pieces of 16 of its key's row
+        const uint32_t turn = (thread / kPieces) & 7;
+        uint32_t buffer = 0;
         if (stages > 0) load(0);
         for (uint32_t stage = 0; stage < stages; ++stage) {
-            const uint32_t buffer = stage % kBuffers;
+            // the block of 8 stages that is at hand may be the next one's already
+            const uint32_t older = stage % kBlock == kBlock - 1 && stage + 1 < stages ? 1 : 0;
             if (stage >= kBuffers) {
                 ok = *abort == 0 && mbar_wait_bounded(bar_empty + 8 * buffer, (stage / kBuffers - 1) & 1, p.wait_limit_ns);
                 if (!__all_sync(0xffffffffu, ok)) {
@@ -339,117 +389,148 @@ e4m3_prompt_attention_kernel(const PromptParams p) {
                     break;
                 }
             }
-            unsigned long long nan_keys = 0;
+            uint4 k_now[kLoads];
+            uint4 v_now[kLoads];
 #pragma unroll
             for (uint32_t i = 0; i < kLoads; ++i) {
-                const uint32_t piece = i * 128 + thread;
-                const uint32_t key = piece / kPieces;
-                const uint32_t dims = piece % kPieces;               // 16 dimensions: two pieces of 16 bytes
-                const uint32_t place = (dims / 4) * kTile + key * 128;
-                const uint32_t at[2] = {place + (((2 * dims % 8) ^ (key & 7)) << 4), place + (((2 * dims % 8 + 1) ^ (key & 7)) << 4)};
-                const uint32_t k_words[4] = {key_codes[i].x, key_codes[i].y, key_codes[i].z, key_codes[i].w};
-                const uint32_t k_base = base + L::kK + buffer * (L::kParts * kTile);
-#pragma unroll
-                for (uint32_t h = 0; h < 2; ++h) {
-                    store_shared(k_base + at[h], make_uint4(e4m3x2_to_f16x2(k_words[2 * h]), e4m3x2_high_to_f16x2(k_words[2 * h]),
-                                                            e4m3x2_to_f16x2(k_words[2 * h + 1]), e4m3x2_high_to_f16x2(k_words[2 * h + 1])));
-                }
-                uint32_t v_words[4] = {value_codes[i].x, value_codes[i].y, value_codes[i].z, value_codes[i].w};
-                uint32_t odd = 0;
-#pragma unroll
-                for (uint32_t w = 0; w < 4; ++w) odd |= (v_words[w] & 0x7f7f7f7fu) + 0x01010101u;
-                odd = (odd & 0x80808080u) != 0;
-                if (__any_sync(0xffffffffu, odd)) {
-                    // codes that are NaN become 0, and their keys are remembered
-                    uint32_t lanes = __ballot_sync(0xffffffffu, odd);
-                    const uint32_t first_key = (i * 128 + (thread & ~31u)) / kPieces;
-                    while (lanes != 0) {
-                        nan_keys |= 1ull << (first_key + (__ffs(lanes) - 1) / kPieces);
-                        lanes &= lanes - 1;
-                    }
-#pragma unroll
-                    for (uint32_t w = 0; w < 4; ++w) {
-                        const uint32_t hit = (((v_words[w] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7;
-                        v_words[w] &= ~(hit * 0xffu);
-                    }
-                }
-                const uint32_t v_base = base + L::kV + buffer * (L::kParts * kTile);
-                const float scale = value_scale[i];
+                k_now[i] = key_codes[i];
+                v_now[i] = value_codes[i];
+            }
+            if (stage + 1 < stages) load(stage + 1);
+            const uint32_t k_base = base + L::kK + buffer * (L::kParts * kTile);
+            const uint32_t v_base = base + L::kV + buffer * (L::kParts * kTile);
+            uint32_t check = 0;                                      // f16 sums of values: NaN where one of them is
+            unsigned long long nan_keys = 0;
+            auto convert_values = [&](uint32_t i, const uint32_t (&words)[4]) {
+                const uint32_t key = (i * 128 + thread) / kPieces;
+                const uint32_t dims = thread % kPieces;              // 16 dimensions
+                const uint32_t place = v_base + (dims / 4) * kTile + key * 128;
+                const float scale = __shfl_sync(0xffffffffu, older ? value_scale[1] : value_scale[0], stage % kBlock * kPagesPerStage + page_of(i));
+                const uint64_t scales = pair_of(scale, scale);
 #pragma unroll
                 for (uint32_t h = 0; h < 2; ++h) {
                     uint32_t pairs[4];
 #pragma unroll
                     for (uint32_t j = 0; j < 4; ++j) {
-                        const uint32_t word = v_words[2 * h + j / 2];
-                        const float2 x = f16x2_to_float2(j % 2 ? e4m3x2_high_to_f16x2(word) : e4m3x2_to_f16x2(word));
-                        pairs[j] = pack_bf16x2(x.x * scale, x.y * scale);
+                        const uint32_t word = words[2 * h + j / 2];
+                        const uint32_t halves = j % 2 ? e4m3x2_high_to_f16x2(word) : e4m3x2_to_f16x2(word);
+                        check = add_f16x2(check, halves);
+                        const float2 x = f16x2_to_float2(halves);
+                        const float2 scaled = pair_out(pair_mul(pair_of(x.x, x.y), scales));
+                        pairs[j] = pack_bf16x2(scaled.x, scaled.y);
                     }
-                    store_shared(v_base + at[h], make_uint4(pairs[0], pairs[1], pairs[2], pairs[3]));
+                    store_shared(place + (((2 * dims % 8 + h) ^ turn) << 4), make_uint4(pairs[0], pairs[1], pairs[2], pairs[3]));
+                }
+            };
+#pragma unroll
+            for (uint32_t i = 0; i < kLoads; ++i) {
+                const uint32_t key = (i * 128 + thread) / kPieces;
+                const uint32_t dims = thread % kPieces;
+                const uint32_t place = k_base + (dims / 4) * kTile + key * 128;
+                const uint32_t words[4] = {k_now[i].x, k_now[i].y, k_now[i].z, k_now[i].w};
+#pragma unroll
+                for (uint32_t h = 0; h < 2; ++h) {
+                    store_shared(place + (((2 * dims % 8 + h) ^ turn) << 4),
+                                 make_uint4(e4m3x2_to_f16x2(words[2 * h]), e4m3x2_high_to_f16x2(words[2 * h]),
+                                            e4m3x2_to_f16x2(words[2 * h + 1]), e4m3x2_high_to_f16x2(words[2 * h + 1])));
+                }
+                const uint32_t v_words[4] = {v_now[i].x, v_now[i].y, v_now[i].z, v_now[i].w};
+                convert_values(i, v_words);
+            }
+            const float2 sums = f16x2_to_float2(check);
+            if (__any_sync(0xffffffffu, isnan(sums.x + sums.y))) {
+                // codes that are NaN become 0, and their keys are remembered
+#pragma unroll
+                for (uint32_t i = 0; i < kLoads; ++i) {
+                    uint32_t words[4] = {v_now[i].x, v_now[i].y, v_now[i].z, v_now[i].w};
+                    uint32_t odd = 0;
+#pragma unroll
+                    for (uint32_t w = 0; w < 4; ++w) {
+                        const uint32_t hit = (((words[w] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7;
+                        odd |= hit;
+                        words[w] &= ~(hit * 0xffu);
+                    }
+                    uint32_t lanes = __ballot_sync(0xffffffffu, odd != 0);
+                    while (lanes != 0) {
+                        nan_keys |= 1ull << ((i * 128 + page_warp * 32 + __ffs(lanes) - 1) / kPieces);
+                        lanes &= lanes - 1;
+                    }
+                    convert_values(i, words);
                 }
             }
-            if (thread < kPagesPerStage) control->key_scales[buffer][thread] = key_scale;
-            if (lane == 0) control->nan_keys[buffer][page_warp] = nan_keys;
-            // bits of all four warps' pages: every warp of 64 dimensions has two pages a load, so one word a warp is joined by
-            // the reader below
-            const uint32_t warp_bad = __reduce_or_sync(0xffffffffu, bad);
-            if (lane == 0) reinterpret_cast<uint8_t*>(&control->bad_pages[buffer])[page_warp] = static_cast<uint8_t>(warp_bad);
-            if (stage + 1 < stages) load(stage + 1);
+            // 4 lanes of the first warp have the stage's key scales
+            if (page_warp == 0 && lane / kPagesPerStage == stage % kBlock) {
+                control->key_scales[buffer][lane % kPagesPerStage] = older ? key_scale[1] : key_scale[0];
+            }
+            if (lane == 0) {
+                control->nan_keys[buffer][page_warp] = nan_keys;
+                if (page_warp == 0) {
+                    control->bad_pages[buffer] = ((older ? bad[1] : bad[0]) >> (stage % kBlock * kPagesPerStage)) & 0xfu;
+                }
+            }
             fence_proxy_async_smem();
             __syncwarp();
-            if (lane == 0 && !(p.selftest_drop != 0 && warp == 4 && stage == 0)) mbar_arrive(bar_full + 8 * buffer);
+            if (lane == 0 && !(p.selftest_drop != 0 && page_warp == 0 && stage == 0)) mbar_arrive(bar_full + 8 * buffer);
+            buffer = buffer + 1 == kBuffers ? 0 : buffer + 1;
         }
         if (!ok && lane == 0 && *abort == 0) {
             *abort = 1;
             record_wait_timeout(p.status, kTagE4m3Prompt, (blockIdx.x << 2) | 1);
         }
-    } else if (warp == 8) {
+    } else if (warp == kSoftmaxWarps + kPageWarps) {
         // -------------------------------------------------------------------------------- MMA issuer
         if (elect_one()) {
             // f32 results of 128 rows; Q K^T: f16, both K-major, 64 keys; P V: bf16, V MN-major, 64 dimensions
             const uint32_t idesc_scores = (1u << 4) | ((kKeys >> 3) << 17) | ((kRows >> 4) << 24);
             const uint32_t idesc_product = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((64u >> 3) << 17) | ((kRows >> 4) << 24);
-            const uint64_t q_desc = smem_descriptor(base + L::kQ);
+            const uint32_t tile_stages[kTiles] = {stages_of(0), stages_of(1)};
             bool running = true;
-            auto issue_scores = [&](uint32_t stage) -> bool {
+            auto issue_scores = [&](uint32_t stage, uint32_t which) -> bool {
                 const uint32_t buffer = stage % kBuffers;
                 if (*abort || !mbar_wait_bounded(bar_full + 8 * buffer, (stage / kBuffers) & 1, p.wait_limit_ns)) {
                     return false;
                 }
                 tcgen05_fence_after();
+                const uint64_t q_desc = smem_descriptor(base + L::kQ + which * (L::kParts * kRows * 128));
                 const uint64_t k_desc = smem_descriptor(base + L::kK + buffer * (L::kParts * kTile));
 #pragma unroll
                 for (uint32_t ks = 0; ks < DIM / 16; ++ks) {   // 16 dimensions: 32 bytes within the swizzled row
-                    umma_ss(tmem + kColumnS + buffer * kKeys, q_desc + (ks / 4) * (kRows * 128 >> 4) + (ks % 4) * 2,
+                    umma_ss(tmem + kColumnS + (2 * which + (stage & 1)) * kKeys, q_desc + (ks / 4) * (kRows * 128 >> 4) + (ks % 4) * 2,
                             k_desc + (ks / 4) * (kTile >> 4) + (ks % 4) * 2, idesc_scores, ks);
                 }
-                umma_commit(bar_scores + 8 * buffer);
+                umma_commit(bar_scores + 8 * (2 * which + (stage & 1)));
                 return true;
             };
-            running = stages == 0 || issue_scores(0);
+            for (uint32_t which = 0; which < kTiles; ++which) {
+                running = running && (tile_stages[which] == 0 || issue_scores(0, which));
+            }
             for (uint32_t stage = 0; stage < stages && running; ++stage) {
                 const uint32_t buffer = stage % kBuffers;
-                // scores of the next stage first.  Their columns are free: the weights in them were consumed by a P V that was
-                // issued before, and MMAs execute in order
-                if (stage + 1 < stages && !issue_scores(stage + 1)) {
-                    running = false;
-                    break;
-                }
-                if (*abort || !mbar_wait_bounded(bar_weights + 8 * buffer, (stage >> 1) & 1, p.wait_limit_ns)) {
-                    running = false;
-                    break;
-                }
-                tcgen05_fence_after();
-#pragma unroll
-                for (uint32_t part = 0; part < L::kParts; ++part) {
-                    const uint64_t v_desc = smem_descriptor(base + L::kV + (buffer * L::kParts + part) * kTile);
-#pragma unroll
-                    for (uint32_t step = 0; step < kPagesPerStage; ++step) {   // 16 keys: 8 columns of weights, 2 KiB of V
-                        umma_ts(tmem + kColumnO + part * 64, tmem + kColumnS + buffer * kKeys + step * 8, v_desc + step * (2048 >> 4),
-                                idesc_product, stage > 0 || step > 0);
+                for (uint32_t which = 0; which < kTiles && running; ++which) {
+                    if (stage >= tile_stages[which]) continue;
+                    // scores of the next stage first.  Their columns are free: the weights in them were consumed by a P V that was
+                    // issued before, and MMAs execute in order
+                    if (stage + 1 < tile_stages[which] && !issue_scores(stage + 1, which)) {
+                        running = false;
+                        break;
                     }
+                    if (*abort || !mbar_wait_bounded(bar_weights + 8 * (2 * which + (stage & 1)), (stage >> 1) & 1, p.wait_limit_ns)) {
+                        running = false;
+                        break;
+                    }
+                    tcgen05_fence_after();
+#pragma unroll
+                    for (uint32_t part = 0; part < L::kParts; ++part) {
+                        const uint64_t v_desc = smem_descriptor(base + L::kV + (buffer * L::kParts + part) * kTile);
+#pragma unroll
+                        for (uint32_t step = 0; step < kPagesPerStage; ++step) {   // 16 keys: 8 columns of weights, 2 KiB of V
+                            umma_ts(tmem + kColumnO + which * DIM + part * 64, tmem + kColumnS + (2 * which + (stage & 1)) * kKeys + step * 8,
+                                    v_desc + step * (2048 >> 4), idesc_product, stage > 0 || step > 0);
+                        }
+                    }
+                    umma_commit(bar_product + 8 * which);
                 }
-                umma_commit(bar_product);
-                umma_commit(bar_empty + 8 * buffer);
+                if (running) umma_commit(bar_empty + 8 * buffer);
             }
             if (!running && *abort == 0) {
                 *abort = 1;
@@ -464,18 +545,20 @@ e4m3_prompt_attention_kernel(const PromptParams p) {
         // -------------------------------------------------------------------------------- softmax
         const uint32_t position = live ? static_cast<uint32_t>(row_wide) : last_position;
         const uint32_t first_key = p.window != 0 && position >= p.window ? position - p.window + 1 : 0;
-        const uint32_t lane_address = tmem + ((warp * 32) << 16);
-        for (uint32_t stage = 0; stage < stages; ++stage) {
-            const uint32_t buffer = stage & 1;
+        const uint32_t lane_address = tmem + ((warp % 4 * 32) << 16);
+        const uint32_t output_columns = lane_address + kColumnO + tile * DIM;
+        const uint32_t my_stages = stages_of(tile);
+        for (uint32_t stage = 0; stage < my_stages; ++stage) {
+            const uint32_t buffer = stage % kBuffers;
             // the scores, and the page warps' own words beside them (complete by then)
-            ok = *abort == 0 && mbar_wait_bounded(bar_scores + 8 * buffer, (stage >> 1) & 1, p.wait_limit_ns) &&
-                 mbar_wait_bounded(bar_full + 8 * buffer, (stage >> 1) & 1, p.wait_limit_ns);
+            ok = *abort == 0 && mbar_wait_bounded(bar_scores + 8 * (2 * tile + (stage & 1)), (stage >> 1) & 1, p.wait_limit_ns) &&
+                 mbar_wait_bounded(bar_full + 8 * buffer, (stage / kBuffers) & 1, p.wait_limit_ns);
             if (!__all_sync(0xffffffffu, ok)) {
                 ok = false;
                 break;
             }
             tcgen05_fence_after();
-            const uint32_t columns = lane_address + kColumnS + buffer * kKeys;
+            const uint32_t columns = lane_address + kColumnS + (2 * tile + (stage & 1)) * kKeys;
             uint32_t raw[4][16];
 #pragma unroll
             for (uint32_t part = 0; part < 4; ++part) tmem_load16_nowait(columns + part * 16, raw[part]);
@@ -503,10 +586,9 @@ e4m3_prompt_attention_kernel(const PromptParams p) {
                 if (odd != 0 || bad != 0) {
                     const unsigned long long seen = bits[0] | (static_cast<unsigned long long>(bits[1]) << 32);
                     poisoned = poisoned || (odd & seen) != 0;
-                    const uint32_t all = (bad | (bad >> 8) | (bad >> 16) | (bad >> 24)) & 0xfu;
 #pragma unroll
                     for (uint32_t sub = 0; sub < kPagesPerStage; ++sub) {
-                        lost = lost || (((all >> sub) & 1) != 0 && ((seen >> (16 * sub)) & 0xffffu) != 0);
+                        lost = lost || (((bad >> sub) & 1) != 0 && ((seen >> (16 * sub)) & 0xffffu) != 0);
                     }
                 }
             }
@@ -538,7 +620,7 @@ e4m3_prompt_attention_kernel(const PromptParams p) {
                 if (raise) reference = most;
                 sum *= shrink;
                 if (stage > 0) {
-                    ok = *abort == 0 && mbar_wait_bounded(bar_product, (stage - 1) & 1, p.wait_limit_ns);
+                    ok = *abort == 0 && mbar_wait_bounded(bar_product + 8 * tile, (stage - 1) & 1, p.wait_limit_ns);
                     if (!__all_sync(0xffffffffu, ok)) {
                         ok = false;
                         break;
@@ -547,43 +629,48 @@ e4m3_prompt_attention_kernel(const PromptParams p) {
 #pragma unroll
                     for (uint32_t c = 0; c < DIM; c += 16) {
                         uint32_t o[16];
-                        tmem_load16(lane_address + kColumnO + c, o);
+                        tmem_load16(output_columns + c, o);
 #pragma unroll
                         for (uint32_t j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * shrink);
-                        tmem_store16(lane_address + kColumnO + c, o);
+                        tmem_store16(output_columns + c, o);
                     }
                 }
             }
             // ---- weights ----
-            const float offset = reference == -INFINITY ? 0.0f : -reference;
-            float2 part_sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+            const float reference_offset = reference == -INFINITY ? 0.0f : -reference;
+            const uint64_t offset = pair_of(reference_offset, reference_offset);
+            uint64_t part_sum[2] = {0, 0};
 #pragma unroll
             for (uint32_t half = 0; half < 2; ++half) {
                 uint32_t packed[16];
 #pragma unroll
-                for (uint32_t pair = 0; pair < 16; ++pair) {
-                    const uint32_t j = half * 32 + pair * 2;
-                    float2 w = fma_two(make_float2(__uint_as_float(raw[j / 16][j % 16]), __uint_as_float(raw[j / 16][j % 16 + 1])),
-                                       factor[j / 16], offset);
-                    w = make_float2(fast_exp2(w.x), fast_exp2(w.y));
-                    if (!fast) {
-                        w.x = (bits[j / 32] >> (j % 32)) & 1 ? w.x : 0.0f;
-                        w.y = (bits[j / 32] >> (j % 32 + 1)) & 1 ? w.y : 0.0f;
+                for (uint32_t sub = 0; sub < 2; ++sub) {
+                    const uint64_t multiplier = pair_of(factor[half * 2 + sub], factor[half * 2 + sub]);
+#pragma unroll
+                    for (uint32_t pair = 0; pair < 8; ++pair) {
+                        const uint32_t j = half * 32 + sub * 16 + pair * 2;
+                        float2 w = pair_out(pair_fma(pair_of(__uint_as_float(raw[j / 16][j % 16]), __uint_as_float(raw[j / 16][j % 16 + 1])),
+                                                     multiplier, offset));
+                        w = make_float2(fast_exp2(w.x), fast_exp2(w.y));
+                        if (!fast) {
+                            w.x = (bits[j / 32] >> (j % 32)) & 1 ? w.x : 0.0f;
+                            w.y = (bits[j / 32] >> (j % 32 + 1)) & 1 ? w.y : 0.0f;
+                        }
+                        packed[sub * 8 + pair] = pack_bf16x2(w.x, w.y);
+                        part_sum[pair & 1] = pair_add(part_sum[pair & 1], pair_of(w.x, w.y));   // unrounded: roundings average out
                     }
-                    packed[pair] = pack_bf16x2(w.x, w.y);
-                    part_sum[pair & 1] = add_two(part_sum[pair & 1], w);   // unrounded: the roundings of many weights average out
                 }
                 tmem_store16(columns + half * 16, packed);
             }
-            part_sum[0] = add_two(part_sum[0], part_sum[1]);
-            sum += part_sum[0].x + part_sum[0].y;
+            const float2 stage_sum = pair_out(pair_add(part_sum[0], part_sum[1]));
+            sum += stage_sum.x + stage_sum.y;
             tmem_store_wait();
             tcgen05_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(bar_weights + 8 * buffer);
+            if (lane == 0) mbar_arrive(bar_weights + 8 * (2 * tile + (stage & 1)));
         }
-        if (ok && stages > 0) {
-            ok = *abort == 0 && mbar_wait_bounded(bar_product, (stages - 1) & 1, p.wait_limit_ns);
+        if (ok && my_stages > 0) {
+            ok = *abort == 0 && mbar_wait_bounded(bar_product + 8 * tile, (my_stages - 1) & 1, p.wait_limit_ns);
             ok = __all_sync(0xffffffffu, ok);
         }
         if (!ok && lane == 0 && *abort == 0) {
@@ -598,7 +685,7 @@ e4m3_prompt_attention_kernel(const PromptParams p) {
 #pragma unroll
             for (uint32_t c = 0; c < DIM; c += 16) {
                 uint32_t o[16];
-                tmem_load16(lane_address + kColumnO + c, o);
+                tmem_load16(output_columns + c, o);
                 if (ok && live && !lost && *abort == 0) {
 #pragma unroll
                     for (uint32_t h = 0; h < 2; ++h) {
@@ -619,25 +706,28 @@ e4m3_prompt_attention_kernel(const PromptParams p) {
     if (p.splits > 1) {
         // ---- join the cluster: unscaled sums, one column of 128 rows behind the other, where the operands were ----
         __syncthreads();                   // nobody writes operands any more, and the MMAs have been waited for
-        float* sums = reinterpret_cast<float*>(smem);
-        if (warp < 4) {
-            const uint32_t lane_address = tmem + ((warp * 32) << 16);
+        float* sums = reinterpret_cast<float*>(smem) + tile * (DIM * kRows);
+        float* joined_row = joined + tile * (3 * kRows) + row;
+        if (warp < kSoftmaxWarps) {
+            const uint32_t columns = tmem + ((warp % 4 * 32) << 16) + kColumnO + tile * DIM;
             const bool valid = ok && !lost && *abort == 0;
+            const bool any = stages_of(tile) > 0;
 #pragma unroll
             for (uint32_t c = 0; c < DIM; c += 16) {
                 uint32_t o[16];
-                tmem_load16(lane_address + kColumnO + c, o);
+                tmem_load16(columns + c, o);
 #pragma unroll
-                for (uint32_t j = 0; j < 16; ++j) sums[(c + j) * kRows + row] = stages > 0 ? __uint_as_float(o[j]) : 0.0f;
+                for (uint32_t j = 0; j < 16; ++j) sums[(c + j) * kRows + row] = any ? __uint_as_float(o[j]) : 0.0f;
             }
-            joined[row] = reference;
-            joined[kRows + row] = sum;
-            joined[2 * kRows + row] = valid ? 1.0f : 0.0f;
+            joined_row[0] = reference;
+            joined_row[kRows] = sum;
+            joined_row[2 * kRows] = valid ? 1.0f : 0.0f;
         }
         __syncwarp();
         cluster_barrier();
-        if (warp < 4) {
-            const uint32_t own = smem_u32(joined) + row * 4;
+        if (warp < kSoftmaxWarps) {
+            const uint32_t own = smem_u32(joined_row);
+            const uint32_t own_sums = smem_u32(sums);
             float most = -INFINITY;
             bool valid = live;
             for (uint32_t r = 0; r < p.splits; ++r) {
@@ -665,7 +755,7 @@ e4m3_prompt_attention_kernel(const PromptParams p) {
                     if (r < p.splits) {
 #pragma unroll
                         for (uint32_t j = 0; j < 8; ++j) {
-                            value[j] = fmaf(load_cluster(base + ((c + j) * kRows + row) * 4, r), weight[r], value[j]);
+                            value[j] = fmaf(load_cluster(own_sums + ((c + j) * kRows + row) * 4, r), weight[r], value[j]);
                         }
                     }
                 }
@@ -684,7 +774,7 @@ e4m3_prompt_attention_kernel(const PromptParams p) {
     }
     tcgen05_fence_before();
     __syncthreads();
-    if (warp == 8) {
+    if (warp == kSoftmaxWarps + kPageWarps) {
         tmem_free(tmem, kTmemColumns);
     }
 }
@@ -721,20 +811,21 @@ cudaError_t launch_e4m3_prompt_attention(cudaStream_t stream, const E4m3Attentio
     params.chunk_heads = params.group < kRows ? params.group : kRows;
     params.chunks = (params.group + params.chunk_heads - 1) / params.chunk_heads;
     params.tile_tokens = kRows / params.chunk_heads;
+    params.cta_tokens = kTiles * params.tile_tokens;
     params.window = launch.window;
     params.sinks = launch.sinks;
     params.scale_log2 = launch.scale * kLog2e;
     params.wait_limit_ns = wait_limit_ns();
     params.selftest_drop = wait_selftest_drop() ? 1 : 0;
     // at most so many tiles: full ones, and one that is not for each segment
-    const uint64_t tiles = launch.num_tokens / params.tile_tokens + launch.num_segments;
+    const uint64_t tiles = launch.num_tokens / params.cta_tokens + launch.num_segments;
     const uint64_t items = tiles * launch.cache.kv_heads * params.chunks;
     uint64_t longest = launch.maximum_context_tokens;
-    if (launch.window != 0 && longest > static_cast<uint64_t>(launch.window) + launch.sinks + params.tile_tokens) {
-        longest = static_cast<uint64_t>(launch.window) + launch.sinks + params.tile_tokens;
+    if (launch.window != 0 && longest > static_cast<uint64_t>(launch.window) + launch.sinks + params.cta_tokens) {
+        longest = static_cast<uint64_t>(launch.window) + launch.sinks + params.cta_tokens;
     }
     params.splits = 1;
-    while (params.splits < 8 && items * params.splits * 2 <= 296 && longest >= 4 * kKeys * params.splits) params.splits *= 2;
+    while (params.splits < 8 && items * params.splits * 2 <= 148 && longest >= 4 * kKeys * params.splits) params.splits *= 2;
     const uint64_t blocks = items * params.splits;
     if (blocks > 0x7fffffffu) {
         return cudaErrorInvalidConfiguration;

@@ -285,6 +285,26 @@ def test_what_is_not_seen_may_hold_anything(device, kind, window, sinks):
 
 
 @pytest.mark.parametrize("kind", ["decode", "prompts"])
+@pytest.mark.parametrize("stray", [float("nan"), float("inf"), -1.0])
+def test_pages_of_nobody_may_hold_anything(device, kind, stray):
+    """A sequence of an odd number of pages next to pages with NaN codes and stray scales, the first page of the pool among them."""
+    rng = np.random.default_rng(17)
+    arena, *cache = random_cache(rng, 8, 2, 64, device)
+    for tensor in (arena.key, arena.value):
+        tensor[[0, 7]] = 0x7F
+    for tensor in (arena.key_scales, arena.value_scales):
+        tensor[[0, 7]] = stray
+    tables = np.array([[1, 2, 3, 4, 5, plain.UNASSIGNED], [6, plain.UNASSIGNED] + [7] * 4])
+    rows, positions = np.arange(2), np.array([70, 3])
+    query = bf16(rng.standard_normal((2, 8, 64)), device)
+    out = torch.zeros_like(query)
+    attention_call(kind, query, arena, to_u32(tables, device), to_u32(rows, device), to_u32(positions, device), out)
+    for part in cache:
+        part.values[[0, 7]] = 0
+    check_attention(out, query, cache, tables, rows, positions, F16_WEIGHTS if kind == "decode" else BF16_WEIGHTS, out)
+
+
+@pytest.mark.parametrize("kind", ["decode", "prompts"])
 def test_unassigned_pages_leave_the_row(device, kind):
     """... of the tokens that see them, and of no others."""
     rng = np.random.default_rng(9)
