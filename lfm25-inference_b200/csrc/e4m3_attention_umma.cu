@@ -5,9 +5,9 @@
 //
 //   warps 8-11  pages: E4M3 codes from global memory to registers one stage ahead, converted into the operands of the MMA in
 //               shared memory (128-byte swizzle): K to f16 as it is, V to bf16 with its page's scale, both without a rounding
-//   warp 12     one thread issues, per stage and tile, S = Q K^T (kind::f16 on f16 operands) and, once the weights are there,
-//               O += P V (bf16, P read from tensor memory, V as an MN-major operand); S of the next stage in front of P V of
-//               this one, so that the tensor core works while the softmax does
+//   warps 12-13 one thread for each tile issues, per stage, S = Q K^T (kind::f16 on f16 operands) and, once the weights are there,
+//               O += P V (bf16, P read from tensor memory, V as an MN-major operand); S of two stages on right behind P V of this
+//               one, so that the tensor core works while the softmax does
 //   warps 0-7   one thread a row, four warps a tile: tcgen05.ld S, page scales, mask, exp2, weights back over the scores
 //
 // O stays in tensor memory: the maximum that weights refer to is only raised when a score exceeds it by more than 8 (log2), and
@@ -21,6 +21,7 @@
 // NaN) and remembered by key: a row that sees it becomes NaN as a whole.  Few tiles: a cluster shares a tile's keys and joins
 // through distributed shared memory.  Every wait is bounded; if one runs out, the tile keeps its output rows.
 #include <cstddef>
+#include <type_traits>
 
 #include "e4m3_cache.cuh"
 #include "e4m3_cache.h"
@@ -38,8 +39,8 @@ constexpr uint32_t kPagesPerStage = 4;
 constexpr uint32_t kKeys = kPagesPerStage * kPageSize;     // 64
 constexpr uint32_t kSoftmaxWarps = 4 * kTiles;
 constexpr uint32_t kPageWarps = 4;
-constexpr uint32_t kThreads = (kSoftmaxWarps + kPageWarps + 1) * 32;
-constexpr uint32_t kBuffers = 3;
+constexpr uint32_t kThreads = (kSoftmaxWarps + kPageWarps + kTiles) * 32;
+constexpr uint32_t kBuffers = 4;
 constexpr uint32_t kTmemColumns = 512;
 constexpr uint32_t kColumnS = 0;                           // for each tile two buffers of 64; weights take the first 32 columns of theirs
 constexpr uint32_t kColumnO = 256;
@@ -92,8 +93,8 @@ struct Control {
     uint64_t empty[kBuffers];          // both tiles' P V are done with them
     uint64_t scores[kTiles][2];
     uint64_t weights[kTiles][2];
-    uint64_t product[kTiles];          // P V of a stage is complete
-    uint64_t drained;                  // after a wait ran out: no MMA is in flight any more
+    uint64_t product[kTiles][2];       // P V of an even / odd stage is complete: one barrier could be two phases behind
+    uint64_t drained[kTiles];          // after a wait ran out: no MMA is in flight any more
     alignas(16) float key_scales[kBuffers][kPagesPerStage];   // read four at a time
     alignas(16) unsigned long long nan_keys[kBuffers][kPageWarps];   // of each page warp: keys with a NaN among their values
     uint32_t bad_pages[kBuffers];      // unassigned pages of the stage, one bit each
@@ -260,14 +261,14 @@ e4m3_prompt_attention_kernel(const PromptParams p) {
     if (threadIdx.x == 0) {
         for (uint32_t i = 0; i < kBuffers; ++i) {
             mbar_init(bar_full + 8 * i, kPageWarps);
-            mbar_init(bar_empty + 8 * i, 1);
+            mbar_init(bar_empty + 8 * i, kTiles);
         }
         for (uint32_t i = 0; i < 2 * kTiles; ++i) {
             mbar_init(bar_scores + 8 * i, 1);
             mbar_init(bar_weights + 8 * i, 4);
+            mbar_init(bar_product + 8 * i, 1);
         }
-        for (uint32_t i = 0; i < kTiles; ++i) mbar_init(bar_product + 8 * i, 1);
-        mbar_init(smem_u32(&control->drained), 1);
+        for (uint32_t i = 0; i < kTiles; ++i) mbar_init(smem_u32(control->drained) + 8 * i, 1);
         control->abort = 0;
         fence_barrier_init();
     }
@@ -477,68 +478,81 @@ e4m3_prompt_attention_kernel(const PromptParams p) {
             *abort = 1;
             record_wait_timeout(p.status, kTagE4m3Prompt, (blockIdx.x << 2) | 1);
         }
-    } else if (warp == kSoftmaxWarps + kPageWarps) {
-        // -------------------------------------------------------------------------------- MMA issuer
+    } else if (warp >= kSoftmaxWarps + kPageWarps) {
+        // -------------------------------------------------------------------------------- MMA issuers, one for each tile
+        const uint32_t which = warp - (kSoftmaxWarps + kPageWarps);
         if (elect_one()) {
             // f32 results of 128 rows; Q K^T: f16, both K-major, 64 keys; P V: bf16, V MN-major, 64 dimensions
-            const uint32_t idesc_scores = (1u << 4) | ((kKeys >> 3) << 17) | ((kRows >> 4) << 24);
-            const uint32_t idesc_product = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((64u >> 3) << 17) | ((kRows >> 4) << 24);
-            const uint32_t tile_stages[kTiles] = {stages_of(0), stages_of(1)};
+            constexpr uint32_t idesc_scores = (1u << 4) | ((kKeys >> 3) << 17) | ((kRows >> 4) << 24);
+            constexpr uint32_t idesc_product = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((64u >> 3) << 17) | ((kRows >> 4) << 24);
+            const uint32_t my_stages = stages_of(which);
+            const uint64_t q_desc = smem_descriptor(base + L::kQ + which * (L::kParts * kRows * 128));
+            const uint64_t k_first = smem_descriptor(base + L::kK);
+            const uint64_t v_first = smem_descriptor(base + L::kV);
+            const uint32_t columns = tmem + kColumnS + 2 * which * kKeys;
+            const uint32_t output_columns = tmem + kColumnO + which * DIM;
+            const uint32_t my_scores = bar_scores + 16 * which;
+            const uint32_t my_weights = bar_weights + 16 * which;
+            const uint32_t my_product = bar_product + 16 * which;
             bool running = true;
-            auto issue_scores = [&](uint32_t stage, uint32_t which) -> bool {
-                const uint32_t buffer = stage % kBuffers;
-                if (*abort || !mbar_wait_bounded(bar_full + 8 * buffer, (stage / kBuffers) & 1, p.wait_limit_ns)) {
+            uint32_t next_buffer = 0;      // of the next scores
+            uint32_t next_parity = 0;
+            auto issue_scores = [&](uint32_t parity) -> bool {
+                if (*abort || !mbar_wait_bounded(bar_full + 8 * next_buffer, next_parity, p.wait_limit_ns)) {
                     return false;
                 }
                 tcgen05_fence_after();
-                const uint64_t q_desc = smem_descriptor(base + L::kQ + which * (L::kParts * kRows * 128));
-                const uint64_t k_desc = smem_descriptor(base + L::kK + buffer * (L::kParts * kTile));
+                const uint64_t k_desc = k_first + next_buffer * (L::kParts * kTile >> 4);
 #pragma unroll
                 for (uint32_t ks = 0; ks < DIM / 16; ++ks) {   // 16 dimensions: 32 bytes within the swizzled row
-                    umma_ss(tmem + kColumnS + (2 * which + (stage & 1)) * kKeys, q_desc + (ks / 4) * (kRows * 128 >> 4) + (ks % 4) * 2,
+                    umma_ss(columns + parity * kKeys, q_desc + (ks / 4) * (kRows * 128 >> 4) + (ks % 4) * 2,
                             k_desc + (ks / 4) * (kTile >> 4) + (ks % 4) * 2, idesc_scores, ks);
                 }
-                umma_commit(bar_scores + 8 * (2 * which + (stage & 1)));
+                umma_commit(my_scores + 8 * parity);
+                if (++next_buffer == kBuffers) {
+                    next_buffer = 0;
+                    next_parity ^= 1;
+                }
                 return true;
             };
-            for (uint32_t which = 0; which < kTiles; ++which) {
-                running = running && (tile_stages[which] == 0 || issue_scores(0, which));
+            for (uint32_t stage = 0; stage < 2 && running; ++stage) {
+                if (stage < my_stages) running = issue_scores(stage);
             }
-            for (uint32_t stage = 0; stage < stages && running; ++stage) {
-                const uint32_t buffer = stage % kBuffers;
-                for (uint32_t which = 0; which < kTiles && running; ++which) {
-                    if (stage >= tile_stages[which]) continue;
-                    // scores of the next stage first.  Their columns are free: the weights in them were consumed by a P V that was
-                    // issued before, and MMAs execute in order
-                    if (stage + 1 < tile_stages[which] && !issue_scores(stage + 1, which)) {
-                        running = false;
-                        break;
-                    }
-                    if (*abort || !mbar_wait_bounded(bar_weights + 8 * (2 * which + (stage & 1)), (stage >> 1) & 1, p.wait_limit_ns)) {
-                        running = false;
-                        break;
-                    }
-                    tcgen05_fence_after();
-#pragma unroll
-                    for (uint32_t part = 0; part < L::kParts; ++part) {
-                        const uint64_t v_desc = smem_descriptor(base + L::kV + (buffer * L::kParts + part) * kTile);
-#pragma unroll
-                        for (uint32_t step = 0; step < kPagesPerStage; ++step) {   // 16 keys: 8 columns of weights, 2 KiB of V
-                            umma_ts(tmem + kColumnO + which * DIM + part * 64, tmem + kColumnS + (2 * which + (stage & 1)) * kKeys + step * 8,
-                                    v_desc + step * (2048 >> 4), idesc_product, stage > 0 || step > 0);
-                        }
-                    }
-                    umma_commit(bar_product + 8 * which);
+            uint32_t buffer = 0;
+            for (uint32_t stage = 0; stage < my_stages && running; ++stage) {
+                const uint32_t parity = stage & 1;
+                if (*abort || !mbar_wait_bounded(my_weights + 8 * parity, (stage >> 1) & 1, p.wait_limit_ns)) {
+                    running = false;
+                    break;
                 }
-                if (running) umma_commit(bar_empty + 8 * buffer);
+                tcgen05_fence_after();
+                const uint64_t v_desc = v_first + buffer * (L::kParts * kTile >> 4);
+#pragma unroll
+                for (uint32_t part = 0; part < L::kParts; ++part) {
+#pragma unroll
+                    for (uint32_t step = 0; step < kPagesPerStage; ++step) {   // 16 keys: 8 columns of weights, 2 KiB of V
+                        umma_ts(output_columns + part * 64, columns + parity * kKeys + step * 8,
+                                v_desc + part * (kTile >> 4) + step * (2048 >> 4), idesc_product, stage > 0 || step > 0);
+                    }
+                }
+                umma_commit(my_product + 8 * parity);
+                umma_commit(bar_empty + 8 * buffer);
+                // Behind it the scores of two stages on: MMAs execute in order, so the weights in their columns have been consumed.
+                if (stage + 2 < my_stages && !issue_scores(parity)) running = false;
+                if (++buffer == kBuffers) buffer = 0;
+            }
+            // stages that only the other tile takes part in
+            for (uint32_t stage = my_stages; stage < stages && running; ++stage) {
+                running = *abort == 0 && mbar_wait_bounded(bar_full + 8 * (stage % kBuffers), (stage / kBuffers) & 1, p.wait_limit_ns);
+                if (running) mbar_arrive(bar_empty + 8 * (stage % kBuffers));
             }
             if (!running && *abort == 0) {
                 *abort = 1;
                 record_wait_timeout(p.status, kTagE4m3Prompt, (blockIdx.x << 2) | 2);
             }
             if (*abort != 0) {
-                umma_commit(smem_u32(&control->drained));
-                (void)mbar_wait_bounded(smem_u32(&control->drained), 0, p.wait_limit_ns);
+                umma_commit(smem_u32(control->drained) + 8 * which);
+                (void)mbar_wait_bounded(smem_u32(control->drained) + 8 * which, 0, p.wait_limit_ns);
             }
         }
     } else {
@@ -592,85 +606,92 @@ e4m3_prompt_attention_kernel(const PromptParams p) {
                     }
                 }
             }
-            tmem_load_wait();
-            // ---- maximum ----
-            if (!fast) {
-                // masked scores, whatever they are, become -inf (the factor is positive or 0, so not by the product)
+            // The rest in two copies: tests of single keys, which the compiler would make predicates of every stage, were a quarter of
+            // all instructions (177 us for eight portions of 512 tokens).
+            auto weigh = [&](auto masked) -> bool {
+                // ---- maximum ----
+                if constexpr (decltype(masked)::value) {
+                    // masked scores, whatever they are, become -inf (the factor is positive or 0, so not by the product)
 #pragma unroll
-                for (uint32_t j = 0; j < kKeys; ++j) {
-                    if (((bits[j / 32] >> (j % 32)) & 1) == 0) raw[j / 16][j % 16] = 0xff800000u;
-                }
-            }
-            float most = -INFINITY;
-#pragma unroll
-            for (uint32_t sub = 0; sub < kPagesPerStage; ++sub) {
-                float a = __uint_as_float(raw[sub][0]);
-                float b = __uint_as_float(raw[sub][1]);
-#pragma unroll
-                for (uint32_t j = 2; j < 16; j += 4) {
-                    a = max3(a, __uint_as_float(raw[sub][j]), __uint_as_float(raw[sub][j + 1]));
-                    if (j + 2 < 16) b = max3(b, __uint_as_float(raw[sub][j + 2]), __uint_as_float(raw[sub][j + 3]));
-                }
-                const float here = fmaxf(a, b);
-                most = fmaxf(most, here * factor[sub]);
-            }
-            const bool raise = most > reference + kHeadroom;
-            if (__any_sync(0xffffffffu, raise)) {
-                const float shrink = !raise ? 1.0f : reference == -INFINITY ? 0.0f : fast_exp2(reference - most);
-                if (raise) reference = most;
-                sum *= shrink;
-                if (stage > 0) {
-                    ok = *abort == 0 && mbar_wait_bounded(bar_product + 8 * tile, (stage - 1) & 1, p.wait_limit_ns);
-                    if (!__all_sync(0xffffffffu, ok)) {
-                        ok = false;
-                        break;
-                    }
-                    tcgen05_fence_after();
-#pragma unroll
-                    for (uint32_t c = 0; c < DIM; c += 16) {
-                        uint32_t o[16];
-                        tmem_load16(output_columns + c, o);
-#pragma unroll
-                        for (uint32_t j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * shrink);
-                        tmem_store16(output_columns + c, o);
+                    for (uint32_t j = 0; j < kKeys; ++j) {
+                        if (((bits[j / 32] >> (j % 32)) & 1) == 0) raw[j / 16][j % 16] = 0xff800000u;
                     }
                 }
-            }
-            // ---- weights ----
-            const float reference_offset = reference == -INFINITY ? 0.0f : -reference;
-            const uint64_t offset = pair_of(reference_offset, reference_offset);
-            uint64_t part_sum[2] = {0, 0};
+                float most = -INFINITY;
 #pragma unroll
-            for (uint32_t half = 0; half < 2; ++half) {
-                uint32_t packed[16];
+                for (uint32_t sub = 0; sub < kPagesPerStage; ++sub) {
+                    float a = __uint_as_float(raw[sub][0]);
+                    float b = __uint_as_float(raw[sub][1]);
 #pragma unroll
-                for (uint32_t sub = 0; sub < 2; ++sub) {
-                    const uint64_t multiplier = pair_of(factor[half * 2 + sub], factor[half * 2 + sub]);
-#pragma unroll
-                    for (uint32_t pair = 0; pair < 8; ++pair) {
-                        const uint32_t j = half * 32 + sub * 16 + pair * 2;
-                        float2 w = pair_out(pair_fma(pair_of(__uint_as_float(raw[j / 16][j % 16]), __uint_as_float(raw[j / 16][j % 16 + 1])),
-                                                     multiplier, offset));
-                        w = make_float2(fast_exp2(w.x), fast_exp2(w.y));
-                        if (!fast) {
-                            w.x = (bits[j / 32] >> (j % 32)) & 1 ? w.x : 0.0f;
-                            w.y = (bits[j / 32] >> (j % 32 + 1)) & 1 ? w.y : 0.0f;
+                    for (uint32_t j = 2; j < 16; j += 4) {
+                        a = max3(a, __uint_as_float(raw[sub][j]), __uint_as_float(raw[sub][j + 1]));
+                        if (j + 2 < 16) b = max3(b, __uint_as_float(raw[sub][j + 2]), __uint_as_float(raw[sub][j + 3]));
+                    }
+                    const float here = fmaxf(a, b);
+                    most = fmaxf(most, here * factor[sub]);
+                }
+                const bool raise = most > reference + kHeadroom;
+                if (__any_sync(0xffffffffu, raise)) {
+                    const float shrink = !raise ? 1.0f : reference == -INFINITY ? 0.0f : fast_exp2(reference - most);
+                    if (raise) reference = most;
+                    sum *= shrink;
+                    if (stage > 0) {
+                        ok = *abort == 0 && mbar_wait_bounded(bar_product + 8 * (2 * tile + ((stage - 1) & 1)), ((stage - 1) >> 1) & 1, p.wait_limit_ns);
+                        if (!__all_sync(0xffffffffu, ok)) {
+                            return false;
                         }
-                        packed[sub * 8 + pair] = pack_bf16x2(w.x, w.y);
-                        part_sum[pair & 1] = pair_add(part_sum[pair & 1], pair_of(w.x, w.y));   // unrounded: roundings average out
+                        tcgen05_fence_after();
+#pragma unroll
+                        for (uint32_t c = 0; c < DIM; c += 16) {
+                            uint32_t o[16];
+                            tmem_load16(output_columns + c, o);
+#pragma unroll
+                            for (uint32_t j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * shrink);
+                            tmem_store16(output_columns + c, o);
+                        }
                     }
                 }
-                tmem_store16(columns + half * 16, packed);
-            }
-            const float2 stage_sum = pair_out(pair_add(part_sum[0], part_sum[1]));
-            sum += stage_sum.x + stage_sum.y;
+                // ---- weights ----
+                const float reference_offset = reference == -INFINITY ? 0.0f : -reference;
+                const uint64_t offset = pair_of(reference_offset, reference_offset);
+                uint64_t part_sum[2] = {0, 0};
+#pragma unroll
+                for (uint32_t half = 0; half < 2; ++half) {
+                    uint32_t packed[16];
+#pragma unroll
+                    for (uint32_t sub = 0; sub < 2; ++sub) {
+                        const uint64_t multiplier = pair_of(factor[half * 2 + sub], factor[half * 2 + sub]);
+#pragma unroll
+                        for (uint32_t pair = 0; pair < 8; ++pair) {
+                            const uint32_t j = half * 32 + sub * 16 + pair * 2;
+                            float2 w = pair_out(pair_fma(pair_of(__uint_as_float(raw[j / 16][j % 16]), __uint_as_float(raw[j / 16][j % 16 + 1])),
+                                                         multiplier, offset));
+                            w = make_float2(fast_exp2(w.x), fast_exp2(w.y));
+                            if constexpr (decltype(masked)::value) {
+                                w.x = (bits[j / 32] >> (j % 32)) & 1 ? w.x : 0.0f;
+                                w.y = (bits[j / 32] >> (j % 32 + 1)) & 1 ? w.y : 0.0f;
+                            }
+                            packed[sub * 8 + pair] = pack_bf16x2(w.x, w.y);
+                            part_sum[pair & 1] = pair_add(part_sum[pair & 1], pair_of(w.x, w.y));   // unrounded: roundings average out
+                        }
+                    }
+                    tmem_store16(columns + half * 16, packed);
+                }
+                const float2 stage_sum = pair_out(pair_add(part_sum[0], part_sum[1]));
+                sum += stage_sum.x + stage_sum.y;
+                return true;
+            };
+            tmem_load_wait();
+            ok = fast ? weigh(std::false_type()) : weigh(std::true_type());
+            if (!ok) break;
             tmem_store_wait();
             tcgen05_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(bar_weights + 8 * (2 * tile + (stage & 1)));
         }
         if (ok && my_stages > 0) {
-            ok = *abort == 0 && mbar_wait_bounded(bar_product + 8 * tile, (my_stages - 1) & 1, p.wait_limit_ns);
+            const uint32_t last = my_stages - 1;
+            ok = *abort == 0 && mbar_wait_bounded(bar_product + 8 * (2 * tile + (last & 1)), (last >> 1) & 1, p.wait_limit_ns);
             ok = __all_sync(0xffffffffu, ok);
         }
         if (!ok && lane == 0 && *abort == 0) {
