@@ -276,59 +276,27 @@ e4m3_prompt_attention_kernel(const PromptParams p) {
         tmem_allocate(smem_u32(&control->tmem), kTmemColumns);
     }
 
-    // ---- rows: this thread's token and head, its query in f16 ----
+    // ---- rows: this thread's token and head ----
     const uint32_t tile = (warp / 4) % kTiles;           // of the softmax warps
     const uint32_t row = threadIdx.x % kRows;            // of the tile
     const uint32_t row_token = cta_begin + tile * p.tile_tokens + row / p.chunk_heads;
     const uint32_t head = chunk * p.chunk_heads + row % p.chunk_heads;   // of the group
     const uint64_t row_wide = first_wide + (row_token - cta_begin);
-    bool live = false;
-    float row_factor = 0.0f;
-    if (warp < kSoftmaxWarps) {
-        live = row < p.tile_tokens * p.chunk_heads && row_token < cta_end && head < p.group && row_wide < most_positions;
-        if (live) live = p.request_slots[row_token] == table_row && p.position_ids[row_token] == row_wide;
-        const __nv_bfloat16* source = p.query + row_token * p.query_token_stride + static_cast<size_t>(kv_head * p.group + head) * DIM;
-        // two passes over the row, so that it need not stay in registers
-        uint32_t largest = 0;
-#pragma unroll
-        for (uint32_t c = 0; c < DIM / 8; ++c) {
-            const uint4 raw = live ? reinterpret_cast<const uint4*>(source)[c] : make_uint4(0, 0, 0, 0);
-            const uint32_t words[4] = {raw.x, raw.y, raw.z, raw.w};
-#pragma unroll
-            for (uint32_t i = 0; i < 4; ++i) {
-                const uint32_t low = words[i] & 0x7fffu;
-                const uint32_t high = (words[i] >> 16) & 0x7fffu;
-                largest = max(largest, max(low < 0x7f80u ? low : 0u, high < 0x7f80u ? high : 0u));
-            }
-        }
-        const int32_t exponent = min(max(static_cast<int32_t>(largest >> 7) - 127 - 11, -126), 126);
-        const float factor = power_of_two(-exponent);
-        row_factor = power_of_two(exponent) * p.scale_log2;
-#pragma unroll
-        for (uint32_t c = 0; c < DIM / 8; ++c) {
-            const uint4 raw = live ? reinterpret_cast<const uint4*>(source)[c] : make_uint4(0, 0, 0, 0);
-            const uint32_t words[4] = {raw.x, raw.y, raw.z, raw.w};
-            uint32_t half[4];
-#pragma unroll
-            for (uint32_t i = 0; i < 4; ++i) {
-                const float2 pair = bf16x2_to_float2(words[i]);
-                half[i] = pack_f16x2(pair.x * factor, pair.y * factor);
-            }
-            store_shared(base + L::kQ + (tile * L::kParts + c / 8) * (kRows * 128) + row * 128 + (((c % 8) ^ (row & 7)) << 4),
-                         make_uint4(half[0], half[1], half[2], half[3]));
-        }
-        fence_proxy_async_smem();
-    }
-    tcgen05_fence_before();
-    __syncthreads();
-    tcgen05_fence_after();
-    const uint32_t tmem = control->tmem;
+    // All threads meet once the barriers, the tensor memory and the queries are there; each role first does what needs none of them.
+    auto meet = [&]() -> uint32_t {
+        tcgen05_fence_before();
+        asm volatile("barrier.sync 1, %0;" ::"n"(kThreads) : "memory");
+        tcgen05_fence_after();
+        return control->tmem;
+    };
+    uint32_t tmem = 0;
 
     // a row's running state (softmax warps)
     float reference = -INFINITY;
     float sum = 0.0f;
     bool poisoned = false;       // sees a NaN value
     bool lost = false;           // sees an unassigned page
+    bool live = false;
     bool ok = true;
 
     if (warp >= kSoftmaxWarps && warp < kSoftmaxWarps + kPageWarps) {
@@ -380,6 +348,7 @@ e4m3_prompt_attention_kernel(const PromptParams p) {
         const uint32_t turn = (thread / kPieces) & 7;
         uint32_t buffer = 0;
         if (stages > 0) load(0);
+        meet();
         for (uint32_t stage = 0; stage < stages; ++stage) {
             // the block of 8 stages that is at hand may be the next one's already
             const uint32_t older = stage % kBlock == kBlock - 1 && stage + 1 < stages ? 1 : 0;
@@ -481,6 +450,7 @@ e4m3_prompt_attention_kernel(const PromptParams p) {
     } else if (warp >= kSoftmaxWarps + kPageWarps) {
         // -------------------------------------------------------------------------------- MMA issuers, one for each tile
         const uint32_t which = warp - (kSoftmaxWarps + kPageWarps);
+        tmem = meet();
         if (elect_one()) {
             // f32 results of 128 rows; Q K^T: f16, both K-major, 64 keys; P V: bf16, V MN-major, 64 dimensions
             constexpr uint32_t idesc_scores = (1u << 4) | ((kKeys >> 3) << 17) | ((kRows >> 4) << 24);
@@ -557,26 +527,73 @@ e4m3_prompt_attention_kernel(const PromptParams p) {
         }
     } else {
         // -------------------------------------------------------------------------------- softmax
+        // ---- queries to f16, by a power of two per row: DIM / 8 lanes a row, 16 bytes each ----
+        live = row < p.tile_tokens * p.chunk_heads && row_token < cta_end && head < p.group && row_wide < most_positions;
+        const uint64_t row_offset = live ? row_token * p.query_token_stride + static_cast<size_t>(kv_head * p.group + head) * DIM : 0;
+        if (live) live = p.request_slots[row_token] == table_row && p.position_ids[row_token] == row_wide;
+        constexpr uint32_t kLanes = DIM / 8;
+        constexpr uint32_t kPasses = kLanes;              // of 32 / kLanes rows
+        uint4 raw_query[kPasses];
+#pragma unroll
+        for (uint32_t pass = 0; pass < kPasses; ++pass) {
+            const uint32_t source = pass * (32 / kLanes) + lane / kLanes;
+            const uint32_t low = __shfl_sync(0xffffffffu, static_cast<uint32_t>(row_offset), source);
+            const uint32_t high = __shfl_sync(0xffffffffu, static_cast<uint32_t>(row_offset >> 32), source);
+            // rows that do not exist read the first query of the batch, and are cleared below
+            raw_query[pass] = *reinterpret_cast<const uint4*>(p.query + ((static_cast<uint64_t>(high) << 32) | low) + lane % kLanes * 8);
+        }
+        const uint32_t live_rows = __ballot_sync(0xffffffffu, live);
+        float row_factor = 0.0f;
+#pragma unroll
+        for (uint32_t pass = 0; pass < kPasses; ++pass) {
+            const uint32_t source = pass * (32 / kLanes) + lane / kLanes;
+            const bool there = (live_rows >> source) & 1;
+            const uint32_t words[4] = {there ? raw_query[pass].x : 0, there ? raw_query[pass].y : 0, there ? raw_query[pass].z : 0,
+                                       there ? raw_query[pass].w : 0};
+            uint32_t largest = 0;
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i) {
+                const uint32_t low = words[i] & 0x7fffu;
+                const uint32_t high = (words[i] >> 16) & 0x7fffu;
+                largest = max(largest, max(low < 0x7f80u ? low : 0u, high < 0x7f80u ? high : 0u));
+            }
+#pragma unroll
+            for (uint32_t delta = kLanes / 2; delta > 0; delta >>= 1) largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, delta));
+            const int32_t exponent = min(max(static_cast<int32_t>(largest >> 7) - 127 - 11, -126), 126);
+            const float factor = power_of_two(-exponent);
+            // the thread of this row is lane `source`: it takes the factor from the first lane that has it
+            const float whole_factor = __shfl_sync(0xffffffffu, power_of_two(exponent) * p.scale_log2, lane % (32 / kLanes) * kLanes);
+            if (lane / (32 / kLanes) == pass) row_factor = whole_factor;
+            uint32_t half[4];
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i) {
+                const float2 pair = bf16x2_to_float2(words[i]);
+                half[i] = pack_f16x2(pair.x * factor, pair.y * factor);
+            }
+            const uint32_t target = warp % 4 * 32 + source;             // row of the tile
+            const uint32_t piece = lane % kLanes;
+            store_shared(base + L::kQ + (tile * L::kParts + piece / 8) * (kRows * 128) + target * 128 + (((piece % 8) ^ (target & 7)) << 4),
+                         make_uint4(half[0], half[1], half[2], half[3]));
+        }
+        fence_proxy_async_smem();
+        tmem = meet();
+
         const uint32_t position = live ? static_cast<uint32_t>(row_wide) : last_position;
         const uint32_t first_key = p.window != 0 && position >= p.window ? position - p.window + 1 : 0;
         const uint32_t lane_address = tmem + ((warp % 4 * 32) << 16);
         const uint32_t output_columns = lane_address + kColumnO + tile * DIM;
         const uint32_t my_stages = stages_of(tile);
+        // weights of the stage before: complete, and handed over
+        auto hand_over = [&](uint32_t stage) {
+            tmem_store_wait();
+            tcgen05_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar_weights + 8 * (2 * tile + (stage & 1)));
+        };
+        uint32_t buffer = 0;
+        uint32_t buffer_parity = 0;
         for (uint32_t stage = 0; stage < my_stages; ++stage) {
-            const uint32_t buffer = stage % kBuffers;
-            // the scores, and the page warps' own words beside them (complete by then)
-            ok = *abort == 0 && mbar_wait_bounded(bar_scores + 8 * (2 * tile + (stage & 1)), (stage >> 1) & 1, p.wait_limit_ns) &&
-                 mbar_wait_bounded(bar_full + 8 * buffer, (stage / kBuffers) & 1, p.wait_limit_ns);
-            if (!__all_sync(0xffffffffu, ok)) {
-                ok = false;
-                break;
-            }
-            tcgen05_fence_after();
-            const uint32_t columns = lane_address + kColumnS + (2 * tile + (stage & 1)) * kKeys;
-            uint32_t raw[4][16];
-#pragma unroll
-            for (uint32_t part = 0; part < 4; ++part) tmem_load16_nowait(columns + part * 16, raw[part]);
-            // ---- what this row sees of the stage ----
+            // ---- what this row sees of the stage, and the page warps' words (there before the scores are) ----
             const uint32_t index = (begin_stage + stage) * kPagesPerStage;
             const uint32_t stage_key = pages.logical(index) * kPageSize;
             const bool together = index + kPagesPerStage <= pages.count && (index >= pages.sink_pages || index + kPagesPerStage <= pages.sink_pages);
@@ -591,6 +608,7 @@ e4m3_prompt_attention_kernel(const PromptParams p) {
                     bits[sub / 2] = sub % 2 ? bits[sub / 2] & ((seen << 16) | 0xffffu) : bits[sub / 2] & (seen | 0xffff0000u);
                 }
             }
+            ok = mbar_wait_bounded(bar_full + 8 * buffer, buffer_parity, p.wait_limit_ns);
             const float4 scales = *reinterpret_cast<const float4*>(control->key_scales[buffer]);
             const float factor[4] = {row_factor * scales.x, row_factor * scales.y, row_factor * scales.z, row_factor * scales.w};
             {
@@ -606,6 +624,21 @@ e4m3_prompt_attention_kernel(const PromptParams p) {
                     }
                 }
             }
+            if (++buffer == kBuffers) {
+                buffer = 0;
+                buffer_parity ^= 1;
+            }
+            ok = ok && mbar_wait_bounded(bar_scores + 8 * (2 * tile + (stage & 1)), (stage >> 1) & 1, p.wait_limit_ns);
+            if (!__all_sync(0xffffffffu, ok)) {
+                ok = false;
+                break;
+            }
+            tcgen05_fence_after();
+            const uint32_t columns = lane_address + kColumnS + (2 * tile + (stage & 1)) * kKeys;
+            uint32_t raw[4][16];
+#pragma unroll
+            for (uint32_t part = 0; part < 4; ++part) tmem_load16_nowait(columns + part * 16, raw[part]);
+            if (stage > 0) hand_over(stage - 1);          // while the scores come
             // The rest in two copies: tests of single keys, which the compiler would make predicates of every stage, were a quarter of
             // all instructions (177 us for eight portions of 512 tokens).
             auto weigh = [&](auto masked) -> bool {
@@ -684,13 +717,10 @@ e4m3_prompt_attention_kernel(const PromptParams p) {
             tmem_load_wait();
             ok = fast ? weigh(std::false_type()) : weigh(std::true_type());
             if (!ok) break;
-            tmem_store_wait();
-            tcgen05_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(bar_weights + 8 * (2 * tile + (stage & 1)));
         }
         if (ok && my_stages > 0) {
             const uint32_t last = my_stages - 1;
+            hand_over(last);
             ok = *abort == 0 && mbar_wait_bounded(bar_product + 8 * (2 * tile + (last & 1)), (last >> 1) & 1, p.wait_limit_ns);
             ok = __all_sync(0xffffffffu, ok);
         }
