@@ -98,6 +98,7 @@ struct Control {
     alignas(16) float key_scales[kBuffers][kPagesPerStage];   // read four at a time
     alignas(16) unsigned long long nan_keys[kBuffers][kPageWarps];   // of each page warp: keys with a NaN among their values
     uint32_t bad_pages[kBuffers];      // unassigned pages of the stage, one bit each
+    uint32_t odd[kBuffers];            // a byte of each page warp: whether any of the two words above is not 0
     uint32_t tmem;
     uint32_t abort;
 };
@@ -433,10 +434,10 @@ e4m3_prompt_attention_kernel(const PromptParams p) {
                 control->key_scales[buffer][lane % kPagesPerStage] = older ? key_scale[1] : key_scale[0];
             }
             if (lane == 0) {
+                const uint32_t stage_bad = ((older ? bad[1] : bad[0]) >> (stage % kBlock * kPagesPerStage)) & 0xfu;
                 control->nan_keys[buffer][page_warp] = nan_keys;
-                if (page_warp == 0) {
-                    control->bad_pages[buffer] = ((older ? bad[1] : bad[0]) >> (stage % kBlock * kPagesPerStage)) & 0xfu;
-                }
+                if (page_warp == 0) control->bad_pages[buffer] = stage_bad;
+                reinterpret_cast<uint8_t*>(&control->odd[buffer])[page_warp] = nan_keys != 0 || stage_bad != 0 ? 1 : 0;
             }
             fence_proxy_async_smem();
             __syncwarp();
@@ -590,38 +591,49 @@ e4m3_prompt_attention_kernel(const PromptParams p) {
             __syncwarp();
             if (lane == 0) mbar_arrive(bar_weights + 8 * (2 * tile + (stage & 1)));
         };
+        // The stages that every row of this warp sees as a whole, in one run: from the last window's first key on, up to the first
+        // position.  (Stages of first tokens only are taken with those that have an edge.)
+        const int32_t least = static_cast<int32_t>(__reduce_min_sync(0xffffffffu, position));
+        const uint32_t edge = __reduce_max_sync(0xffffffffu, first_key);
+        const int32_t shift = static_cast<int32_t>(pages.sink_pages) - static_cast<int32_t>(pages.first_page);   // of list against table
+        const int32_t whole_first = max(static_cast<int32_t>(pages.sink_pages), static_cast<int32_t>((edge + kPageSize - 1) / kPageSize) + shift);
+        const int32_t whole_last = (least + 1 - static_cast<int32_t>(kKeys)) >= 0 ? (least + 1 - static_cast<int32_t>(kKeys)) / static_cast<int32_t>(kPageSize) + shift : -1;
+        const int32_t from = max((whole_first + static_cast<int32_t>(kPagesPerStage) - 1) / static_cast<int32_t>(kPagesPerStage) - static_cast<int32_t>(begin_stage), 0);
+        const int32_t until = whole_last >= 0 ? whole_last / static_cast<int32_t>(kPagesPerStage) + 1 - static_cast<int32_t>(begin_stage) : 0;
+        const uint32_t whole_begin = static_cast<uint32_t>(from);
+        const uint32_t whole_count = static_cast<uint32_t>(max(until - from, 0));
         uint32_t buffer = 0;
         uint32_t buffer_parity = 0;
         for (uint32_t stage = 0; stage < my_stages; ++stage) {
-            // ---- what this row sees of the stage, and the page warps' words (there before the scores are) ----
-            const uint32_t index = (begin_stage + stage) * kPagesPerStage;
-            const uint32_t stage_key = pages.logical(index) * kPageSize;
-            const bool together = index + kPagesPerStage <= pages.count && (index >= pages.sink_pages || index + kPagesPerStage <= pages.sink_pages);
-            const bool whole = together && position >= stage_key + kKeys - 1 && (first_key <= stage_key || p.sinks >= stage_key + kKeys);
-            const bool fast = __all_sync(0xffffffffu, whole);
-            uint32_t bits[2] = {0xffffffffu, 0xffffffffu};
-            if (!fast) {
-#pragma unroll
+            // ---- the page warps' words (there before the scores are) ----
+            const bool fast = stage - whole_begin < whole_count;
+            // the keys of the stage that this row sees, where that is asked for
+            auto seen_keys = [&](uint32_t (&bits)[2]) {
+                const uint32_t index = (begin_stage + stage) * kPagesPerStage;
+                bits[0] = bits[1] = 0;
+#pragma unroll 1
                 for (uint32_t sub = 0; sub < kPagesPerStage; ++sub) {
-                    const uint32_t seen = index + sub < pages.count
-                                              ? visible_bits(pages.logical(index + sub) * kPageSize, position, first_key, p.sinks) : 0u;
-                    bits[sub / 2] = sub % 2 ? bits[sub / 2] & ((seen << 16) | 0xffffu) : bits[sub / 2] & (seen | 0xffff0000u);
+                    if (index + sub < pages.count) {
+                        const uint32_t seen = visible_bits(pages.logical(index + sub) * kPageSize, position, first_key, p.sinks) << (sub % 2 * 16);
+                        if (sub < 2) bits[0] |= seen;
+                        else bits[1] |= seen;
+                    }
                 }
-            }
+            };
             ok = mbar_wait_bounded(bar_full + 8 * buffer, buffer_parity, p.wait_limit_ns);
             const float4 scales = *reinterpret_cast<const float4*>(control->key_scales[buffer]);
             const float factor[4] = {row_factor * scales.x, row_factor * scales.y, row_factor * scales.z, row_factor * scales.w};
-            {
+            if (control->odd[buffer] != 0) {
                 const unsigned long long* nan = control->nan_keys[buffer];
-                const unsigned long long odd = (nan[0] | nan[1]) | (nan[2] | nan[3]);
+                const unsigned long long nan_keys = (nan[0] | nan[1]) | (nan[2] | nan[3]);
                 const uint32_t bad = control->bad_pages[buffer];
-                if (odd != 0 || bad != 0) {
-                    const unsigned long long seen = bits[0] | (static_cast<unsigned long long>(bits[1]) << 32);
-                    poisoned = poisoned || (odd & seen) != 0;
-#pragma unroll
-                    for (uint32_t sub = 0; sub < kPagesPerStage; ++sub) {
-                        lost = lost || (((bad >> sub) & 1) != 0 && ((seen >> (16 * sub)) & 0xffffu) != 0);
-                    }
+                uint32_t bits[2];
+                seen_keys(bits);
+                const unsigned long long seen = bits[0] | (static_cast<unsigned long long>(bits[1]) << 32);
+                poisoned = poisoned || (nan_keys & seen) != 0;
+#pragma unroll 1
+                for (uint32_t sub = 0; sub < kPagesPerStage; ++sub) {
+                    lost = lost || (((bad >> sub) & 1) != 0 && ((seen >> (16 * sub)) & 0xffffu) != 0);
                 }
             }
             if (++buffer == kBuffers) {
@@ -642,6 +654,8 @@ e4m3_prompt_attention_kernel(const PromptParams p) {
             // The rest in two copies: tests of single keys, which the compiler would make predicates of every stage, were a quarter of
             // all instructions (177 us for eight portions of 512 tokens).
             auto weigh = [&](auto masked) -> bool {
+                uint32_t bits[2] = {0, 0};
+                if constexpr (decltype(masked)::value) seen_keys(bits);
                 // ---- maximum ----
                 if constexpr (decltype(masked)::value) {
                     // masked scores, whatever they are, become -inf (the factor is positive or 0, so not by the product)
