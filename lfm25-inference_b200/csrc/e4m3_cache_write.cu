@@ -3,11 +3,13 @@
 // A run is the longest sequence of tokens of the batch, one behind the other, whose slots are one behind the other within a
 // page: one token in a decode step, up to 16 in a prompt.  The unit of work is a run, a KV head and K or V, and belongs to
 // one warp: a scale needs the maximum over the run's 16 x head_dim values at most, which fits the warp's registers, so that
-// every input is read once and nothing but the result is written.  With 8 values (16 bytes) a lane, a row of 64 takes 8
-// lanes and a warp 4 rows at a time.  The run finds itself: every warp looks at the slots of the tokens around its own.
+// every input is read once and nothing but the result is written.  A lane has 4 dimensions of the first half of a head and the 4
+// that they are rotated with, so that a row of 64 takes 8 lanes, a warp 4 rows at a time, and a rotation no exchange.  The run
+// finds itself: every warp looks at the slots of the tokens around its own.
 //
-// The kernel is bound by the chain slots -> values and old scale -> maximum -> codes in a decode step, by bandwidth over
-// long prompts.
+// The kernel is bound by chains of dependent loads (slots -> values and old scale -> maximum -> codes) in a decode step, by
+// bandwidth over long prompts.  Queries have CTAs of their own, which do not wait for slots; all loads of a CTA are under way
+// while it computes its angles.
 //
 // Arithmetic: everything in f32.  With norms, x / sqrt(mean(x^2) + eps) * w is rotated by position * inv_freq[d] in the
 // pairs (d, d + head_dim / 2); the angle is formed and reduced in f64, since in f32 its error grows with the position
@@ -20,8 +22,8 @@ namespace lfm25 {
 
 namespace {
 
-constexpr uint32_t kWarpsMost = 16;
-constexpr uint32_t kSpanMost = 16;                       // tokens of a CTA
+constexpr uint32_t kAhead = 4;                           // query rows that a lane loads ahead
+constexpr uint32_t kSpanMost = 16;                       // tokens of a CTA that looks for runs
 constexpr uint32_t kRowsMost = kSpanMost + kPageSize - 1;   // with the rest of the last run
 
 struct WriteParams {
@@ -39,204 +41,262 @@ struct WriteParams {
     uint64_t query_token_stride;
     uint32_t num_tokens;
     uint32_t query_heads;
+    uint32_t query_blocks;   // CTAs in front that have queries, `query_span` tokens each
+    uint32_t query_span;
     uint32_t span;
     float eps;
 };
 
-__device__ __forceinline__ void unpack(uint4 raw, float (&x)[8]) {
-    const uint32_t words[4] = {raw.x, raw.y, raw.z, raw.w};
-#pragma unroll
-    for (uint32_t i = 0; i < 4; ++i) {
-        const float2 pair = bf16x2_to_float2(words[i]);
-        x[2 * i] = pair.x;
-        x[2 * i + 1] = pair.y;
-    }
+// dimensions 4 i .. 4 i + 3 and, in the upper half, DIM / 2 + 4 i .. of a head, i the lane's place in the row
+struct Values {
+    float low[4];
+    float high[4];
+};
+
+template <uint32_t DIM>
+__device__ __forceinline__ uint4 load_values(const __nv_bfloat16* head, uint32_t place) {
+    const uint2 low = *reinterpret_cast<const uint2*>(head + 4 * place);
+    const uint2 high = *reinterpret_cast<const uint2*>(head + DIM / 2 + 4 * place);
+    return make_uint4(low.x, low.y, high.x, high.y);
 }
 
-// Norm and rotation of a row that LANES lanes hold, 8 values each; `turn` has (cos, sin) of the row's head_dim / 2 angles.
-// Every lane of the warp takes part.
+__device__ __forceinline__ Values unpack(uint4 raw) {
+    const float2 a = bf16x2_to_float2(raw.x);
+    const float2 b = bf16x2_to_float2(raw.y);
+    const float2 c = bf16x2_to_float2(raw.z);
+    const float2 d = bf16x2_to_float2(raw.w);
+    return {{a.x, a.y, b.x, b.y}, {c.x, c.y, d.x, d.y}};
+}
+
+// Norm and rotation of a row that DIM / 8 lanes hold; `turn` has (cos, sin) of the row's DIM / 2 angles.  Every lane of the warp
+// takes part.
 template <uint32_t DIM>
-__device__ __forceinline__ void norm_rope_row(float (&x)[8], const float (&weight)[8], const float2* turn, uint32_t piece,
-                                              float eps) {
-    constexpr uint32_t LANES = DIM / 8;
+__device__ __forceinline__ void norm_rope_row(Values& x, const Values& weight, const float2* turn, uint32_t place, float eps) {
     float sum = 0.0f;
 #pragma unroll
-    for (uint32_t i = 0; i < 8; ++i) sum = fmaf(x[i], x[i], sum);
+    for (uint32_t i = 0; i < 4; ++i) sum = fmaf(x.low[i], x.low[i], fmaf(x.high[i], x.high[i], sum));
 #pragma unroll
-    for (uint32_t delta = LANES / 2; delta > 0; delta >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, delta);
-    const float inverse = 1.0f / sqrtf(sum * (1.0f / DIM) + eps);
-    const bool second = piece >= LANES / 2;
-    const float2* angles = turn + (piece % (LANES / 2)) * 8;
+    for (uint32_t delta = DIM / 16; delta > 0; delta >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, delta);
+    const float inverse = rsqrtf(sum * (1.0f / DIM) + eps);     // 2 units off at most
+    const float4 first = reinterpret_cast<const float4*>(turn + 4 * place)[0];
+    const float4 second = reinterpret_cast<const float4*>(turn + 4 * place)[1];
+    const float cosine[4] = {first.x, first.z, second.x, second.z};
+    const float sine[4] = {first.y, first.w, second.y, second.w};
 #pragma unroll
-    for (uint32_t i = 0; i < 8; ++i) {
-        const float mine = x[i] * inverse * weight[i];
-        const float other = __shfl_xor_sync(0xffffffffu, mine, LANES / 2);
-        const float2 t = angles[i];
-        x[i] = fmaf(mine, t.x, second ? other * t.y : -other * t.y);
+    for (uint32_t i = 0; i < 4; ++i) {
+        const float low = x.low[i] * inverse * weight.low[i];
+        const float high = x.high[i] * inverse * weight.high[i];
+        x.low[i] = fmaf(low, cosine[i], -high * sine[i]);
+        x.high[i] = fmaf(high, cosine[i], low * sine[i]);
     }
 }
 
-template <uint32_t DIM, bool NORM_ROPE>
-__global__ void __launch_bounds__(kWarpsMost * 32)
+__device__ __forceinline__ uint32_t four_codes(const float (&x)[4], float factor) {
+    return e4m3x2(x[0] * factor, x[1] * factor) | (static_cast<uint32_t>(e4m3x2(x[2] * factor, x[3] * factor)) << 16);
+}
+
+// (cos, sin) of position * inv_freq for `rows` tokens from `first` on
+template <uint32_t DIM>
+__device__ __forceinline__ void angles(const WriteParams& p, uint32_t first, uint32_t rows, float2* turns) {
+    for (uint32_t index = threadIdx.x; index < rows * (DIM / 2); index += blockDim.x) {
+        const double angle = static_cast<double>(p.position_ids[first + index / (DIM / 2)]) * static_cast<double>(p.inv_freq[index % (DIM / 2)]);
+        const double turn = rint(angle * 0.15915494309189535);
+        float sine, cosine;
+        sincosf(static_cast<float>(fma(turn, -6.283185307179586, angle)), &sine, &cosine);
+        turns[index] = make_float2(cosine, sine);
+    }
+}
+
+// All queries of `query_span` tokens
+template <uint32_t DIM, uint32_t kWarps>
+__device__ __forceinline__ void write_queries(const WriteParams& p, float2* turns) {
+    constexpr uint32_t LANES = DIM / 8;
+    constexpr uint32_t ROWS = 32 / LANES;
+    const uint32_t lane = threadIdx.x & 31;
+    const uint32_t warp = threadIdx.x >> 5;
+    const uint32_t piece = lane % LANES;
+    const uint32_t begin = blockIdx.x * p.query_span;
+    const uint32_t tokens = min(p.query_span, p.num_tokens - begin);
+    const uint32_t rows = tokens * p.query_heads;
+    uint4 raw[kAhead];
+    uint32_t token_of[kAhead];
+    auto load = [&](uint32_t first) {
+#pragma unroll
+        for (uint32_t i = 0; i < kAhead; ++i) {
+            const uint32_t row = first + i * kWarps * ROWS + lane / LANES;
+            raw[i] = make_uint4(0, 0, 0, 0);
+            token_of[i] = min(row, rows - 1) / p.query_heads;
+            if (row < rows) {
+                raw[i] = load_values<DIM>(p.query + (begin + token_of[i]) * p.query_token_stride + (row - token_of[i] * p.query_heads) * DIM, piece);
+            }
+        }
+    };
+    load(warp * ROWS);
+    const Values weight = unpack(load_values<DIM>(p.query_norm, piece));
+    angles<DIM>(p, begin, tokens, turns);
+    __syncthreads();
+    for (uint32_t first = warp * ROWS; first < rows; first += kAhead * kWarps * ROWS) {
+#pragma unroll
+        for (uint32_t i = 0; i < kAhead; ++i) {
+            if (first + i * kWarps * ROWS < rows) {          // for the whole warp
+                const uint32_t row = first + i * kWarps * ROWS + lane / LANES;
+                Values x = unpack(raw[i]);
+                norm_rope_row<DIM>(x, weight, turns + token_of[i] * (DIM / 2), piece, p.eps);
+                if (row < rows) {
+                    __nv_bfloat16* out = p.query_out + (static_cast<size_t>(begin) * p.query_heads + row) * DIM;
+                    *reinterpret_cast<uint2*>(out + 4 * piece) = make_uint2(pack_bf16x2(x.low[0], x.low[1]), pack_bf16x2(x.low[2], x.low[3]));
+                    *reinterpret_cast<uint2*>(out + DIM / 2 + 4 * piece) =
+                        make_uint2(pack_bf16x2(x.high[0], x.high[1]), pack_bf16x2(x.high[2], x.high[3]));
+                }
+            }
+        }
+        if (first + kAhead * kWarps * ROWS < rows) load(first + kAhead * kWarps * ROWS);
+    }
+}
+
+template <uint32_t DIM, bool NORM_ROPE, uint32_t kWarps>
+__global__ void __launch_bounds__(kWarps * 32, kWarps == 16 ? 1 : DIM == 64 ? 3 : 2)
 e4m3_cache_write_kernel(const WriteParams p) {
     constexpr uint32_t LANES = DIM / 8;            // lanes of a row
     constexpr uint32_t ROWS = 32 / LANES;          // rows of a pass
     constexpr uint32_t PASSES = kPageSize / ROWS;
-    __shared__ float2 turns[NORM_ROPE ? kRowsMost * DIM / 2 : 1];
+    __shared__ __align__(16) float2 turns[NORM_ROPE ? kRowsMost * DIM / 2 : 2];
     const uint32_t lane = threadIdx.x & 31;
     const uint32_t warp = threadIdx.x >> 5;
-    const uint32_t warps = blockDim.x >> 5;
     const uint32_t piece = lane % LANES;
     const uint32_t lane_row = lane / LANES;
     pdl_launch_dependents();
     pdl_wait();
+    if constexpr (NORM_ROPE) {
+        if (blockIdx.x < p.query_blocks) {
+            write_queries<DIM, kWarps>(p, turns);
+            return;
+        }
+    }
 
     // ---- the runs that begin among this CTA's tokens: lane l looks at token begin - 1 + l ----
-    const uint32_t begin = blockIdx.x * p.span;
+    const uint32_t begin = (blockIdx.x - p.query_blocks) * p.span;
     const int64_t mine = static_cast<int64_t>(begin) + lane - 1;
     const int64_t slot = mine >= 0 && mine < p.num_tokens ? p.slot_mapping[mine] : -2;
     const int64_t before = __shfl_up_sync(0xffffffffu, slot, 1);
     const bool valid = slot >= 0 && static_cast<uint64_t>(slot) / kPageSize < p.cache.num_pages;
     const bool continues = valid && slot % kPageSize != 0 && slot == before + 1 && lane > 0;
     const uint32_t continued = __ballot_sync(0xffffffffu, continues);
-    uint32_t leaders = __ballot_sync(0xffffffffu, valid && !continues && lane > 0 && lane <= p.span);
-
-    if (NORM_ROPE) {
-        // angles of all tokens that this CTA's queries and runs have
-        uint32_t rows = min(p.span, p.num_tokens - begin);
-        if (leaders != 0) {
-            const uint32_t last = 31 - __clz(leaders);
-            const uint32_t after = last == 31 ? 0 : __ffs(~(continued >> (last + 1))) - 1;
-            rows = max(rows, last + after);
-        }
-        for (uint32_t index = threadIdx.x; index < rows * (DIM / 2); index += blockDim.x) {
-            const uint32_t row = index / (DIM / 2);
-            const double angle = static_cast<double>(p.position_ids[begin + row]) * static_cast<double>(p.inv_freq[index % (DIM / 2)]);
-            const double turn = rint(angle * 0.15915494309189535);
-            float sine, cosine;
-            sincosf(static_cast<float>(fma(turn, -6.283185307179586, angle)), &sine, &cosine);
-            turns[index] = make_float2(cosine, sine);
-        }
-        __syncthreads();
-
-        // ---- queries: all rows of this CTA's tokens ----
-        float weight[8];
-        unpack(*reinterpret_cast<const uint4*>(p.query_norm + piece * 8), weight);
-        const uint32_t tokens = min(p.span, p.num_tokens - begin);
-        const uint32_t query_rows = tokens * p.query_heads;
-        for (uint32_t first = warp * ROWS; first < query_rows; first += warps * ROWS) {
-            const uint32_t row = first + lane_row;
-            const uint32_t here = min(row, query_rows - 1);
-            const uint32_t token = here / p.query_heads;
-            const uint32_t head = here % p.query_heads;
-            float x[8];
-            unpack(*reinterpret_cast<const uint4*>(p.query + (begin + token) * p.query_token_stride + head * DIM + piece * 8), x);
-            norm_rope_row<DIM>(x, weight, turns + token * (DIM / 2), piece, p.eps);
-            if (row < query_rows) {
-                uint4 out;
-                out.x = pack_bf16x2(x[0], x[1]);
-                out.y = pack_bf16x2(x[2], x[3]);
-                out.z = pack_bf16x2(x[4], x[5]);
-                out.w = pack_bf16x2(x[6], x[7]);
-                *reinterpret_cast<uint4*>(p.query_out + (static_cast<size_t>(begin + token) * p.query_heads + head) * DIM + piece * 8) = out;
-            }
-        }
+    const uint32_t leaders = __ballot_sync(0xffffffffu, valid && !continues && lane > 0 && lane <= p.span);
+    if (leaders == 0) {
+        return;
     }
+    auto run_length = [&](uint32_t leader) -> uint32_t {
+        return 1 + (leader == 31 ? 0 : __ffs(~(continued >> (leader + 1))) - 1);
+    };
 
-    // ---- runs ----
+    // ---- units: K and V of a head for each run ----
     const uint32_t kinds = 2 * p.cache.kv_heads;
     const uint32_t units = __popc(leaders) * kinds;
-    uint32_t skipped = 0;                              // leaders taken off the mask so far
-    for (uint32_t unit = warp; unit < units; unit += warps) {
-        while (skipped < unit / kinds) {
-            leaders &= leaders - 1;
-            ++skipped;
-        }
-        const uint32_t leader = __ffs(leaders) - 1;
-        const uint32_t count = 1 + (leader == 31 ? 0 : __ffs(~(continued >> (leader + 1))) - 1);
+    struct Unit {
+        uint8_t* codes;
+        float* scale;
+        float old_scale;
+        uint32_t count;
+        uint32_t offset;
+        uint32_t first_row;     // of the CTA's rows
+        bool is_value;
+    } next = {};
+    uint4 raw[PASSES];
+    auto load = [&](uint32_t unit) {
+        uint32_t rest = leaders;
+        for (uint32_t skip = unit / kinds; skip > 0; --skip) rest &= rest - 1;
+        const uint32_t leader = __ffs(rest) - 1;
+        next.count = run_length(leader);
         const int64_t first_slot = __shfl_sync(0xffffffffu, slot, leader);
-        const uint32_t first_row = leader - 1;         // of the CTA's rows
+        next.first_row = leader - 1;
         const size_t page = static_cast<size_t>(first_slot) / kPageSize;
-        const uint32_t offset = static_cast<uint32_t>(first_slot % kPageSize);
+        next.offset = static_cast<uint32_t>(first_slot % kPageSize);
         const uint32_t kind = unit % kinds;
-        const bool is_value = kind >= p.cache.kv_heads;
-        const uint32_t head = is_value ? kind - p.cache.kv_heads : kind;
-        const __nv_bfloat16* source = (is_value ? p.value : p.key) + static_cast<size_t>(begin + first_row) * p.kv_token_stride +
-                                      head * DIM + piece * 8;
-        uint8_t* codes = (is_value ? p.cache.value_codes : p.cache.key_codes) + (page * p.cache.kv_heads + head) * (kPageSize * DIM) + piece * 8;
-        float* scale = (is_value ? p.cache.value_scales : p.cache.key_scales) + page * p.cache.kv_heads + head;
-        const float old_scale = offset > 0 ? *scale : 0.0f;
-
-        uint4 raw[PASSES];
+        next.is_value = kind >= p.cache.kv_heads;
+        const uint32_t head = next.is_value ? kind - p.cache.kv_heads : kind;
+        const __nv_bfloat16* source = (next.is_value ? p.value : p.key) + static_cast<size_t>(begin + next.first_row) * p.kv_token_stride +
+                                      head * DIM;
+        next.codes = (next.is_value ? p.cache.value_codes : p.cache.key_codes) + (page * p.cache.kv_heads + head) * (kPageSize * DIM);
+        next.scale = (next.is_value ? p.cache.value_scales : p.cache.key_scales) + page * p.cache.kv_heads + head;
+        next.old_scale = next.offset > 0 ? *next.scale : 0.0f;
 #pragma unroll
         for (uint32_t pass = 0; pass < PASSES; ++pass) {
             const uint32_t row = pass * ROWS + lane_row;
             raw[pass] = make_uint4(0, 0, 0, 0);
-            if (row < count) raw[pass] = *reinterpret_cast<const uint4*>(source + row * p.kv_token_stride);
+            if (row < next.count) raw[pass] = load_values<DIM>(source + row * p.kv_token_stride, piece);
         }
-        float x[PASSES][8];
-        float weight[8];
-        if (NORM_ROPE && !is_value) unpack(*reinterpret_cast<const uint4*>(p.key_norm + piece * 8), weight);
+    };
+    if (warp < units) load(warp);
+    Values weight = {};
+    if constexpr (NORM_ROPE) {
+        weight = unpack(load_values<DIM>(p.key_norm, piece));
+        const uint32_t last = 31 - __clz(leaders);
+        angles<DIM>(p, begin, last - 1 + run_length(last), turns);
+        __syncthreads();
+    }
+    for (uint32_t unit = warp; unit < units; unit += kWarps) {
+        const Unit now = next;
+        Values x[PASSES];
         uint32_t largest = 0;
 #pragma unroll
         for (uint32_t pass = 0; pass < PASSES; ++pass) {
-            unpack(raw[pass], x[pass]);
-            if (NORM_ROPE && !is_value) {
-                const uint32_t row = min(pass * ROWS + lane_row, count - 1);   // rows that do not exist are zeros
-                if (pass * ROWS < count) norm_rope_row<DIM>(x[pass], weight, turns + (first_row + row) * (DIM / 2), piece, p.eps);
-            }
+            if (pass * ROWS < now.count) {
+                x[pass] = unpack(raw[pass]);
+                if (NORM_ROPE && !now.is_value) {
+                    const uint32_t row = min(pass * ROWS + lane_row, now.count - 1);   // rows that do not exist are zeros
+                    norm_rope_row<DIM>(x[pass], weight, turns + (now.first_row + row) * (DIM / 2), piece, p.eps);
+                }
 #pragma unroll
-            for (uint32_t i = 0; i < 8; ++i) {
-                // infinities and NaN do not move the scale: they become the largest code and the NaN code
-                const uint32_t magnitude = __float_as_uint(x[pass][i]) & 0x7fffffffu;
-                largest = max(largest, magnitude < 0x7f800000u ? magnitude : 0u);
+                for (uint32_t i = 0; i < 8; ++i) {
+                    // infinities and NaN do not move the scale: they become the largest code and the NaN code
+                    const uint32_t magnitude = __float_as_uint(i < 4 ? x[pass].low[i % 4] : x[pass].high[i % 4]) & 0x7fffffffu;
+                    largest = max(largest, magnitude < 0x7f800000u ? magnitude : 0u);
+                }
             }
         }
+        if (unit + kWarps < units) load(unit + kWarps);
         largest = __reduce_max_sync(0xffffffffu, largest);
-        const int32_t old_exponent = stored_exponent(old_scale);
+        const int32_t old_exponent = stored_exponent(now.old_scale);
         int32_t exponent = scale_exponent(largest);
-        if (offset > 0) exponent = max(exponent, old_exponent);
+        if (now.offset > 0) exponent = max(exponent, old_exponent);
 
         const float factor = power_of_two(-exponent);
 #pragma unroll
         for (uint32_t pass = 0; pass < PASSES; ++pass) {
             const uint32_t row = pass * ROWS + lane_row;
-            if (row < count) {
-                uint2 out;
-                out.x = e4m3x2(x[pass][0] * factor, x[pass][1] * factor) | (static_cast<uint32_t>(e4m3x2(x[pass][2] * factor, x[pass][3] * factor)) << 16);
-                out.y = e4m3x2(x[pass][4] * factor, x[pass][5] * factor) | (static_cast<uint32_t>(e4m3x2(x[pass][6] * factor, x[pass][7] * factor)) << 16);
-                *reinterpret_cast<uint2*>(codes + (offset + row) * DIM) = out;
+            if (row < now.count) {
+                uint8_t* place = now.codes + (now.offset + row) * DIM + 4 * piece;
+                *reinterpret_cast<uint32_t*>(place) = four_codes(x[pass].low, factor);
+                *reinterpret_cast<uint32_t*>(place + DIM / 2) = four_codes(x[pass].high, factor);
             }
         }
         // what the page holds already goes over to a larger scale
-        if (offset > 0 && exponent > old_exponent) {
+        if (now.offset > 0 && exponent > old_exponent) {
             const float shrink = power_of_two(old_exponent - exponent);
+#pragma unroll 1
+            for (uint32_t row = lane_row; row < now.offset; row += ROWS) {
+                uint2* place = reinterpret_cast<uint2*>(now.codes + row * DIM + 8 * piece);
+                uint2 there = *place;
+                uint32_t* words[2] = {&there.x, &there.y};
 #pragma unroll
-            for (uint32_t pass = 0; pass < PASSES; ++pass) {
-                const uint32_t row = pass * ROWS + lane_row;
-                if (row < offset) {
-                    uint2* place = reinterpret_cast<uint2*>(codes + row * DIM);
-                    uint2 there = *place;
-                    uint32_t* words[2] = {&there.x, &there.y};
-#pragma unroll
-                    for (uint32_t w = 0; w < 2; ++w) {
-                        const float2 low = f16x2_to_float2(e4m3x2_to_f16x2(*words[w]));
-                        const float2 high = f16x2_to_float2(e4m3x2_high_to_f16x2(*words[w]));
-                        *words[w] = e4m3x2(low.x * shrink, low.y * shrink) |
-                                    (static_cast<uint32_t>(e4m3x2(high.x * shrink, high.y * shrink)) << 16);
-                    }
-                    *place = there;
+                for (uint32_t w = 0; w < 2; ++w) {
+                    const float2 low = f16x2_to_float2(e4m3x2_to_f16x2(*words[w]));
+                    const float2 high = f16x2_to_float2(e4m3x2_high_to_f16x2(*words[w]));
+                    *words[w] = e4m3x2(low.x * shrink, low.y * shrink) |
+                                (static_cast<uint32_t>(e4m3x2(high.x * shrink, high.y * shrink)) << 16);
                 }
+                *place = there;
             }
         }
-        if (lane == 0) *scale = power_of_two(exponent);
+        if (lane == 0) *now.scale = power_of_two(exponent);
     }
 }
 
-template <uint32_t DIM>
-cudaError_t launch_dim(cudaStream_t stream, const WriteParams& params, unsigned int blocks, unsigned int threads) {
-    return params.query != nullptr ? launch_kernel(e4m3_cache_write_kernel<DIM, true>, blocks, threads, 0, stream, 1, params)
-                                   : launch_kernel(e4m3_cache_write_kernel<DIM, false>, blocks, threads, 0, stream, 1, params);
+template <uint32_t DIM, uint32_t kWarps>
+cudaError_t launch_dim(cudaStream_t stream, const WriteParams& params, unsigned int blocks) {
+    return params.query != nullptr ? launch_kernel(e4m3_cache_write_kernel<DIM, true, kWarps>, blocks, kWarps * 32, 0, stream, 1, params)
+                                   : launch_kernel(e4m3_cache_write_kernel<DIM, false, kWarps>, blocks, kWarps * 32, 0, stream, 1, params);
 }
 
 }  // namespace
@@ -258,15 +318,33 @@ cudaError_t launch_e4m3_cache_write(cudaStream_t stream, const E4m3WriteLaunch& 
     params.num_tokens = static_cast<uint32_t>(launch.num_tokens);
     params.query_heads = launch.query_heads;
     params.eps = launch.eps;
-    // few tokens: a CTA each, so that a decode step's tokens run side by side; many: 16 to a CTA, which then has the runs of
-    // a page of a prompt, rather than 16 CTAs of which one finds work
-    params.span = launch.num_tokens <= 512 ? 1 : kSpanMost;
-    const uint32_t rows = 256 / launch.cache.head_dim;   // of a warp's pass
-    const uint32_t units = 2 * launch.cache.kv_heads + params.span * launch.query_heads / rows;
-    const unsigned int threads = 32 * (units < kWarpsMost ? units : kWarpsMost);
-    const unsigned int blocks = static_cast<unsigned int>((launch.num_tokens + params.span - 1) / params.span);
-    return launch.cache.head_dim == 64 ? launch_dim<64>(stream, params, blocks, threads)
-                                       : launch_dim<128>(stream, params, blocks, threads);
+    // Tokens of a CTA that looks for runs: as many as leave 4 CTAs an SM.  A decode step's tokens then run side by side (700 tokens
+    // with norms: 16 to a CTA 33.7 us), and the tokens of a long prompt share the search.
+    params.span = 1;
+    while (params.span < kSpanMost && launch.num_tokens / (2 * params.span) >= 4 * 148) params.span *= 2;
+    const size_t run_blocks = (launch.num_tokens + params.span - 1) / params.span;
+    size_t query_blocks = 0;
+    // CTAs of 16 warps while each has an SM to itself, so that the heads of a token are worked on side by side; else of 8
+    uint32_t warps = 16;
+    for (; warps >= 8; warps /= 2) {
+        if (params.query != nullptr) {
+            // as many tokens as a CTA's lanes load at once
+            const uint32_t rows = kAhead * warps * (256 / launch.cache.head_dim);
+            params.query_span = rows / params.query_heads < 1 ? 1 : rows / params.query_heads;
+            if (params.query_span > kSpanMost) params.query_span = kSpanMost;
+            query_blocks = (launch.num_tokens + params.query_span - 1) / params.query_span;
+        }
+        if (warps == 8 || run_blocks + query_blocks <= 148) break;
+    }
+    if (run_blocks + query_blocks > 0x7fffffffu) {
+        return cudaErrorInvalidConfiguration;
+    }
+    params.query_blocks = static_cast<uint32_t>(query_blocks);
+    const unsigned int blocks = static_cast<unsigned int>(run_blocks + query_blocks);
+    if (launch.cache.head_dim == 64) {
+        return warps == 16 ? launch_dim<64, 16>(stream, params, blocks) : launch_dim<64, 8>(stream, params, blocks);
+    }
+    return warps == 16 ? launch_dim<128, 16>(stream, params, blocks) : launch_dim<128, 8>(stream, params, blocks);
 }
 
 }  // namespace lfm25
