@@ -8,8 +8,8 @@
 // finds itself: every warp looks at the slots of the tokens around its own.
 //
 // The kernel is bound by chains of dependent loads (slots -> values and old scale -> maximum -> codes) in a decode step, by
-// bandwidth over long prompts.  Queries have CTAs of their own, which do not wait for slots; all loads of a CTA are under way
-// while it computes its angles.
+// bandwidth over long prompts.  Queries, keys and values have CTAs of their own: queries do not wait for slots, values not for
+// angles, and all loads of a CTA are under way while it computes its angles.
 //
 // Arithmetic: everything in f32.  With norms, x / sqrt(mean(x^2) + eps) * w is rotated by position * inv_freq[d] in the
 // pairs (d, d + head_dim / 2); the angle is formed and reduced in f64, since in f32 its error grows with the position
@@ -22,6 +22,8 @@ namespace lfm25 {
 
 namespace {
 
+constexpr uint32_t kWarps = 8;
+constexpr uint32_t kThreads = kWarps * 32;
 constexpr uint32_t kAhead = 4;                           // query rows that a lane loads ahead
 constexpr uint32_t kSpanMost = 16;                       // tokens of a CTA that looks for runs
 constexpr uint32_t kRowsMost = kSpanMost + kPageSize - 1;   // with the rest of the last run
@@ -43,6 +45,7 @@ struct WriteParams {
     uint32_t query_heads;
     uint32_t query_blocks;   // CTAs in front that have queries, `query_span` tokens each
     uint32_t query_span;
+    uint32_t run_blocks;     // behind them so many with keys, `span` tokens each, and as many with values
     uint32_t span;
     float eps;
 };
@@ -98,7 +101,7 @@ __device__ __forceinline__ uint32_t four_codes(const float (&x)[4], float factor
 // (cos, sin) of position * inv_freq for `rows` tokens from `first` on
 template <uint32_t DIM>
 __device__ __forceinline__ void angles(const WriteParams& p, uint32_t first, uint32_t rows, float2* turns) {
-    for (uint32_t index = threadIdx.x; index < rows * (DIM / 2); index += blockDim.x) {
+    for (uint32_t index = threadIdx.x; index < rows * (DIM / 2); index += kThreads) {
         const double angle = static_cast<double>(p.position_ids[first + index / (DIM / 2)]) * static_cast<double>(p.inv_freq[index % (DIM / 2)]);
         const double turn = rint(angle * 0.15915494309189535);
         float sine, cosine;
@@ -108,7 +111,7 @@ __device__ __forceinline__ void angles(const WriteParams& p, uint32_t first, uin
 }
 
 // All queries of `query_span` tokens
-template <uint32_t DIM, uint32_t kWarps>
+template <uint32_t DIM>
 __device__ __forceinline__ void write_queries(const WriteParams& p, float2* turns) {
     constexpr uint32_t LANES = DIM / 8;
     constexpr uint32_t ROWS = 32 / LANES;
@@ -154,8 +157,8 @@ __device__ __forceinline__ void write_queries(const WriteParams& p, float2* turn
     }
 }
 
-template <uint32_t DIM, bool NORM_ROPE, uint32_t kWarps>
-__global__ void __launch_bounds__(kWarps * 32, kWarps == 16 ? 1 : DIM == 64 ? 3 : 2)
+template <uint32_t DIM, bool NORM_ROPE>
+__global__ void __launch_bounds__(kThreads, DIM == 64 ? 3 : 2)
 e4m3_cache_write_kernel(const WriteParams p) {
     constexpr uint32_t LANES = DIM / 8;            // lanes of a row
     constexpr uint32_t ROWS = 32 / LANES;          // rows of a pass
@@ -169,13 +172,14 @@ e4m3_cache_write_kernel(const WriteParams p) {
     pdl_wait();
     if constexpr (NORM_ROPE) {
         if (blockIdx.x < p.query_blocks) {
-            write_queries<DIM, kWarps>(p, turns);
+            write_queries<DIM>(p, turns);
             return;
         }
     }
 
     // ---- the runs that begin among this CTA's tokens: lane l looks at token begin - 1 + l ----
-    const uint32_t begin = (blockIdx.x - p.query_blocks) * p.span;
+    const bool is_value = blockIdx.x - p.query_blocks >= p.run_blocks;
+    const uint32_t begin = (blockIdx.x - p.query_blocks - (is_value ? p.run_blocks : 0)) * p.span;
     const int64_t mine = static_cast<int64_t>(begin) + lane - 1;
     const int64_t slot = mine >= 0 && mine < p.num_tokens ? p.slot_mapping[mine] : -2;
     const int64_t before = __shfl_up_sync(0xffffffffu, slot, 1);
@@ -190,8 +194,8 @@ e4m3_cache_write_kernel(const WriteParams p) {
         return 1 + (leader == 31 ? 0 : __ffs(~(continued >> (leader + 1))) - 1);
     };
 
-    // ---- units: K and V of a head for each run ----
-    const uint32_t kinds = 2 * p.cache.kv_heads;
+    // ---- units: a head of each run ----
+    const uint32_t kinds = p.cache.kv_heads;
     const uint32_t units = __popc(leaders) * kinds;
     struct Unit {
         uint8_t* codes;
@@ -200,7 +204,6 @@ e4m3_cache_write_kernel(const WriteParams p) {
         uint32_t count;
         uint32_t offset;
         uint32_t first_row;     // of the CTA's rows
-        bool is_value;
     } next = {};
     uint4 raw[PASSES];
     auto load = [&](uint32_t unit) {
@@ -212,13 +215,11 @@ e4m3_cache_write_kernel(const WriteParams p) {
         next.first_row = leader - 1;
         const size_t page = static_cast<size_t>(first_slot) / kPageSize;
         next.offset = static_cast<uint32_t>(first_slot % kPageSize);
-        const uint32_t kind = unit % kinds;
-        next.is_value = kind >= p.cache.kv_heads;
-        const uint32_t head = next.is_value ? kind - p.cache.kv_heads : kind;
-        const __nv_bfloat16* source = (next.is_value ? p.value : p.key) + static_cast<size_t>(begin + next.first_row) * p.kv_token_stride +
+        const uint32_t head = unit % kinds;
+        const __nv_bfloat16* source = (is_value ? p.value : p.key) + static_cast<size_t>(begin + next.first_row) * p.kv_token_stride +
                                       head * DIM;
-        next.codes = (next.is_value ? p.cache.value_codes : p.cache.key_codes) + (page * p.cache.kv_heads + head) * (kPageSize * DIM);
-        next.scale = (next.is_value ? p.cache.value_scales : p.cache.key_scales) + page * p.cache.kv_heads + head;
+        next.codes = (is_value ? p.cache.value_codes : p.cache.key_codes) + (page * p.cache.kv_heads + head) * (kPageSize * DIM);
+        next.scale = (is_value ? p.cache.value_scales : p.cache.key_scales) + page * p.cache.kv_heads + head;
         next.old_scale = next.offset > 0 ? *next.scale : 0.0f;
 #pragma unroll
         for (uint32_t pass = 0; pass < PASSES; ++pass) {
@@ -229,7 +230,7 @@ e4m3_cache_write_kernel(const WriteParams p) {
     };
     if (warp < units) load(warp);
     Values weight = {};
-    if constexpr (NORM_ROPE) {
+    if (NORM_ROPE && !is_value) {
         weight = unpack(load_values<DIM>(p.key_norm, piece));
         const uint32_t last = 31 - __clz(leaders);
         angles<DIM>(p, begin, last - 1 + run_length(last), turns);
@@ -243,7 +244,7 @@ e4m3_cache_write_kernel(const WriteParams p) {
         for (uint32_t pass = 0; pass < PASSES; ++pass) {
             if (pass * ROWS < now.count) {
                 x[pass] = unpack(raw[pass]);
-                if (NORM_ROPE && !now.is_value) {
+                if (NORM_ROPE && !is_value) {
                     const uint32_t row = min(pass * ROWS + lane_row, now.count - 1);   // rows that do not exist are zeros
                     norm_rope_row<DIM>(x[pass], weight, turns + (now.first_row + row) * (DIM / 2), piece, p.eps);
                 }
@@ -293,10 +294,10 @@ e4m3_cache_write_kernel(const WriteParams p) {
     }
 }
 
-template <uint32_t DIM, uint32_t kWarps>
+template <uint32_t DIM>
 cudaError_t launch_dim(cudaStream_t stream, const WriteParams& params, unsigned int blocks) {
-    return params.query != nullptr ? launch_kernel(e4m3_cache_write_kernel<DIM, true, kWarps>, blocks, kWarps * 32, 0, stream, 1, params)
-                                   : launch_kernel(e4m3_cache_write_kernel<DIM, false, kWarps>, blocks, kWarps * 32, 0, stream, 1, params);
+    return params.query != nullptr ? launch_kernel(e4m3_cache_write_kernel<DIM, true>, blocks, kThreads, 0, stream, 1, params)
+                                   : launch_kernel(e4m3_cache_write_kernel<DIM, false>, blocks, kThreads, 0, stream, 1, params);
 }
 
 }  // namespace
@@ -318,33 +319,27 @@ cudaError_t launch_e4m3_cache_write(cudaStream_t stream, const E4m3WriteLaunch& 
     params.num_tokens = static_cast<uint32_t>(launch.num_tokens);
     params.query_heads = launch.query_heads;
     params.eps = launch.eps;
-    // Tokens of a CTA that looks for runs: as many as leave 4 CTAs an SM.  A decode step's tokens then run side by side (700 tokens
-    // with norms: 16 to a CTA 33.7 us), and the tokens of a long prompt share the search.
+    // Tokens of a CTA that looks for runs: as many as leave 2 CTAs an SM with keys and 2 with values.  A decode step's tokens
+    // then run side by side, and the tokens of a long prompt share the search (3800 tokens: 8 to a CTA 16.0 us, 4 to a CTA 17.3 us;
+    // 700 tokens: 2 to a CTA 8.3 us, 1 to a CTA 9.3 us).
     params.span = 1;
-    while (params.span < kSpanMost && launch.num_tokens / (2 * params.span) >= 4 * 148) params.span *= 2;
+    while (params.span < kSpanMost && launch.num_tokens / (2 * params.span) >= 2 * 148) params.span *= 2;
     const size_t run_blocks = (launch.num_tokens + params.span - 1) / params.span;
     size_t query_blocks = 0;
-    // CTAs of 16 warps while each has an SM to itself, so that the heads of a token are worked on side by side; else of 8
-    uint32_t warps = 16;
-    for (; warps >= 8; warps /= 2) {
-        if (params.query != nullptr) {
-            // as many tokens as a CTA's lanes load at once
-            const uint32_t rows = kAhead * warps * (256 / launch.cache.head_dim);
-            params.query_span = rows / params.query_heads < 1 ? 1 : rows / params.query_heads;
-            if (params.query_span > kSpanMost) params.query_span = kSpanMost;
-            query_blocks = (launch.num_tokens + params.query_span - 1) / params.query_span;
-        }
-        if (warps == 8 || run_blocks + query_blocks <= 148) break;
+    if (params.query != nullptr) {
+        // as many tokens as a CTA's lanes load at once
+        const uint32_t rows = kAhead * kWarps * (256 / launch.cache.head_dim);
+        params.query_span = rows / params.query_heads < 1 ? 1 : rows / params.query_heads;
+        if (params.query_span > kSpanMost) params.query_span = kSpanMost;
+        query_blocks = (launch.num_tokens + params.query_span - 1) / params.query_span;
     }
-    if (run_blocks + query_blocks > 0x7fffffffu) {
+    if (2 * run_blocks + query_blocks > 0x7fffffffu) {
         return cudaErrorInvalidConfiguration;
     }
     params.query_blocks = static_cast<uint32_t>(query_blocks);
-    const unsigned int blocks = static_cast<unsigned int>(run_blocks + query_blocks);
-    if (launch.cache.head_dim == 64) {
-        return warps == 16 ? launch_dim<64, 16>(stream, params, blocks) : launch_dim<64, 8>(stream, params, blocks);
-    }
-    return warps == 16 ? launch_dim<128, 16>(stream, params, blocks) : launch_dim<128, 8>(stream, params, blocks);
+    params.run_blocks = static_cast<uint32_t>(run_blocks);
+    const unsigned int blocks = static_cast<unsigned int>(2 * run_blocks + query_blocks);
+    return launch.cache.head_dim == 64 ? launch_dim<64>(stream, params, blocks) : launch_dim<128>(stream, params, blocks);
 }
 
 }  // namespace lfm25
