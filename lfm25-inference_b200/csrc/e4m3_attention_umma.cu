@@ -507,13 +507,15 @@ e4m3_prompt_attention_kernel(const PromptParams p) {
                     }
                 }
                 umma_commit(my_product + 8 * parity);
-                umma_commit(bar_empty + 8 * buffer);
+                // Only where the buffer is filled once more: an arrival that nobody waits for may come when the CTA has gone, and
+                // its shared memory with it.
+                if (stage + kBuffers < stages) umma_commit(bar_empty + 8 * buffer);
                 // Behind it the scores of two stages on: MMAs execute in order, so the weights in their columns have been consumed.
                 if (stage + 2 < my_stages && !issue_scores(parity)) running = false;
                 if (++buffer == kBuffers) buffer = 0;
             }
             // stages that only the other tile takes part in
-            for (uint32_t stage = my_stages; stage < stages && running; ++stage) {
+            for (uint32_t stage = my_stages; stage + kBuffers < stages && running; ++stage) {
                 running = *abort == 0 && mbar_wait_bounded(bar_full + 8 * (stage % kBuffers), (stage / kBuffers) & 1, p.wait_limit_ns);
                 if (running) mbar_arrive(bar_empty + 8 * (stage % kBuffers));
             }
