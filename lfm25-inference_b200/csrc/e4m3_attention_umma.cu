@@ -14,8 +14,10 @@
 // only then is O read, scaled and stored.  The query is brought to f16 by a power of two per row, which the scores get back
 // together with the page's scale in the multiply-add in front of the exponential.
 //
-// What bounds it at 64 dimensions is the instructions of softmax and conversion, behind them the exponentials (128 rows x 64 keys
-// at 16 a cycle and SM: 512 cycles a stage and tile; the two products 256).
+// Eight portions of 512 tokens at depths of 0 to 3584, 32 heads on 8 of 64: 166 us, 0.41 PFLOP/s, where the exponentials alone (16 a
+// cycle and SM) need 60.  No unit is busy for as much as half of that time.  What bounds it is the chain of a stage through its
+// roles, some 2400 cycles in which a softmax warp waits 500 for scores and pages, weighs for 1300 and hands over for 240, and
+// 10,000 cycles at the ends of a CTA: without the exponentials it takes 160 us, without the loads of pages 159.
 //
 // Rows of a mask edge test bits of their own; a NaN among the values is replaced in the operand (a weight of 0 times NaN is
 // NaN) and remembered by key: a row that sees it becomes NaN as a whole.  Few tiles: a cluster shares a tile's keys and joins
@@ -891,8 +893,11 @@ cudaError_t launch_e4m3_prompt_attention(cudaStream_t stream, const E4m3Attentio
     if (launch.window != 0 && longest > static_cast<uint64_t>(launch.window) + launch.sinks + params.cta_tokens) {
         longest = static_cast<uint64_t>(launch.window) + launch.sinks + params.cta_tokens;
     }
+    // Shares of the keys as long as all CTAs run at once and each has a few stages (37 tokens behind 8000, 8 KV heads: 1 share 152,
+    // 2 84, 4 49, 8 32.6 us; 64 behind 500: 18.8, 17.7, 15.5, 16.7; 64 behind 200: 13.6, 15.2; 2 x 64 behind 4000, where 8 shares
+    // are 256 CTAs: 4 shares 31.4, 8 44.9).
     params.splits = 1;
-    while (params.splits < 8 && items * params.splits * 2 <= 148 && longest >= 4 * kKeys * params.splits) params.splits *= 2;
+    while (params.splits < 8 && items * params.splits * 2 <= 148 && longest >= (2 * params.splits + 4) * kKeys) params.splits *= 2;
     const uint64_t blocks = items * params.splits;
     if (blocks > 0x7fffffffu) {
         return cudaErrorInvalidConfiguration;
