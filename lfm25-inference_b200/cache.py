@@ -39,6 +39,7 @@ class KvPageAllocator:
 
     def __init__(self, total_pages: int, page_size: int = 16):
         self._handle = ctypes.c_void_p()
+        self._page_size = page_size
         check(library().lfm25_kv_allocator_create(total_pages, page_size, ctypes.byref(self._handle)))
 
     def try_reserve_tokens(self, maximum_tokens: int) -> int:
@@ -77,7 +78,7 @@ class KvPageAllocator:
         full pages are shared, a partly filled last one gets a page of its own.  Returns (source pages, destination pages) to be
         copied with `ops.kv_pages_copy` before either sequence is appended to; no counterpart in the reference."""
         pair = np.zeros(2, dtype=np.uint32)
-        if -(-tokens // 16) > source_table.size:
+        if -(-tokens // self._page_size) > source_table.size:
             raise KvAllocationError(_abi.KV_SEQUENCE_CAPACITY_EXCEEDED)
         copies = self._moves(library().lfm25_kv_allocator_fork_sequence(
             self._handle, tokens, _table_pointer(source_table), _table_pointer(block_table), block_table.size, _table_pointer(pair)))

@@ -198,6 +198,16 @@ def test_release_behind_a_window(tokens, window, sinks, kept):
     assert pages_in_use(allocator) == 0
 
 
+def test_fork_of_pages_of_32_tokens():
+    allocator = KvPageAllocator(5, 32)
+    first, second = table(2), table(2)
+    allocator.grow_sequence(0, 50, first)
+    source, destination = allocator.fork_sequence(50, first, second)
+    assert source.tolist() == [first[1]] and destination.tolist() == [second[1]] and second[0] == first[0]
+    with pytest.raises(KvAllocationError):
+        allocator.fork_sequence(65, first, table(4))           # more than the source's table holds
+
+
 def test_fork_of_a_sequence_behind_a_window():
     allocator = KvPageAllocator(12)
     first, second = table(), table()
