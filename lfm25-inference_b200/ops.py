@@ -482,10 +482,10 @@ def kv_pages_copy(arenas, source_pages, destination_pages) -> None:
             _refuse("page copy arenas must be on the current device")
         if not arena.is_contiguous():
             _refuse("page copy arenas must be contiguous")
-        bytes_, pages = arena.nbytes, len(arena) if arena.dim() else 0
-        if pages == 0 or bytes_ == 0:
+        shape = arena.shape
+        if not shape or 0 in shape:
             _refuse("page copy arenas are [pages, ...]")
-        table += (arena.data_ptr(), bytes_ // pages, pages)
+        table += (arena.data_ptr(), arena.nbytes // shape[0], shape[0])
     if not table:
         _refuse("page copy requires arenas")
     source, pairs = _dense("source pages", source_pages, _U32, device)
