@@ -3,21 +3,24 @@
 // A CTA owns two tiles of 128 rows: consecutive tokens of one segment times the query heads of one KV head (2 x 32 tokens x 4
 // heads), or one share of their keys.  Keys come in stages of 64 (4 pages), converted once for both tiles:
 //
-//   warps 8-11  pages: E4M3 codes from global memory to registers one stage ahead, converted into the operands of the MMA in
-//               shared memory (128-byte swizzle): K to f16 as it is, V to bf16 with its page's scale, both without a rounding
-//   warps 12-13 one thread for each tile issues, per stage, S = Q K^T (kind::f16 on f16 operands) and, once the weights are there,
-//               O += P V (bf16, P read from tensor memory, V as an MN-major operand); S of two stages on right behind P V of this
-//               one, so that the tensor core works while the softmax does
-//   warps 0-7   one thread a row, four warps a tile: tcgen05.ld S, page scales, mask, exp2, weights back over the scores
+//   page warps (4)      E4M3 codes by asynchronous copies two stages ahead, then converted into the operands of the MMA in shared
+//                       memory (128-byte swizzle): K to f16 as it is, V to bf16 with its page's scale, both without a rounding
+//   issuing warps (2)   one for each tile, per stage S = Q K^T (kind::f16 on f16 operands) and, once the weights are there, O += P V
+//                       (bf16, P read from tensor memory, V as an MN-major operand); S of two stages on right behind P V of this
+//                       one, so that the tensor core works while the softmax does
+//   softmax warps (16)  one thread a row, four warps a tile, and at 64 dimensions two such sets that take stages by turns, each with
+//                       a maximum, sum and O of its own, joined at the end: tcgen05.ld S, page scales, mask, exp2, weights back
+//                       over the scores.  (At 128 dimensions tensor memory holds one O for each tile, and there is one set.)
 //
 // O stays in tensor memory: the maximum that weights refer to is only raised when a score exceeds it by more than 8 (log2), and
 // only then is O read, scaled and stored.  The query is brought to f16 by a power of two per row, which the scores get back
 // together with the page's scale in the multiply-add in front of the exponential.
 //
-// Eight portions of 512 tokens at depths of 0 to 3584, 32 heads on 8 of 64: 166 us, 0.41 PFLOP/s, where the exponentials alone (16 a
-// cycle and SM) need 60.  No unit is busy for as much as half of that time.  What bounds it is the chain of a stage through its
-// roles, some 2400 cycles in which a softmax warp waits 500 for scores and pages, weighs for 1300 and hands over for 240, and
-// 10,000 cycles at the ends of a CTA: without the exponentials it takes 160 us, without the loads of pages 159.
+// Eight portions of 512 tokens at depths of 0 to 3584, 32 heads on 8 of 64: 145 us, 0.47 PFLOP/s, where the exponentials alone (16 a
+// cycle and SM) need 60.  What bounds it is the chain of a stage through its roles, 1900 cycles: no unit is busy for much more than
+// half of that, page warps as long as softmax warps, and 11,000 cycles go to the ends of a CTA.  One set of softmax warps takes 156 us (166
+// with codes in registers one stage ahead); without its exponentials the kernel takes 139, without conversions 146, without both 133.
+// Eight page warps leave 72 registers a thread: 151 us.
 //
 // Rows of a mask edge test bits of their own; a NaN among the values is replaced in the operand (a weight of 0 times NaN is
 // NaN) and remembered by key: a row that sees it becomes NaN as a whole.  Few tiles: a cluster shares a tile's keys and joins
@@ -39,12 +42,10 @@ constexpr uint32_t kRows = 128;                            // of a tile
 constexpr uint32_t kTiles = 2;                             // of a CTA
 constexpr uint32_t kPagesPerStage = 4;
 constexpr uint32_t kKeys = kPagesPerStage * kPageSize;     // 64
-constexpr uint32_t kSoftmaxWarps = 4 * kTiles;
 constexpr uint32_t kPageWarps = 4;
-constexpr uint32_t kThreads = (kSoftmaxWarps + kPageWarps + kTiles) * 32;
-constexpr uint32_t kBuffers = 4;
+constexpr uint32_t kBuffersMost = 4;
 constexpr uint32_t kTmemColumns = 512;
-constexpr uint32_t kColumnS = 0;                           // for each tile two buffers of 64; weights take the first 32 columns of theirs
+constexpr uint32_t kColumnS = 0;                           // for each tile two buffers of 64; weights of 32 keys take the first 16 columns of theirs
 constexpr uint32_t kColumnO = 256;
 constexpr float kHeadroom = 8.0f;
 constexpr uint32_t kTile = kKeys * 128;                    // 64 keys x 64 dimensions of 2 bytes
@@ -80,27 +81,37 @@ struct PromptParams {
 template <uint32_t DIM>
 struct Layout {
     static constexpr uint32_t kParts = DIM / 64;
+    // softmax warps of a tile take stages by turns, in sets of 4, each with an O of its own where tensor memory has room for two
+    static constexpr uint32_t kSets = DIM == 64 ? 2 : 1;
+    static constexpr uint32_t kSoftmaxWarps = 4 * kTiles * kSets;
+    static constexpr uint32_t kThreads = (kSoftmaxWarps + kPageWarps + kTiles) * 32;
+    static constexpr uint32_t kRowWords = 4 + 3 * kSets;                      // maximum, sum, result; factor; the first three of each set
+    static constexpr uint32_t kBuffers = DIM == 64 ? 4 : 3;                   // of operands
+    static constexpr uint32_t kAhead = 2;                                     // stages of codes under way
+    static constexpr uint32_t kCodes = 2 * kKeys * DIM;                       // bytes of a stage
     static constexpr uint32_t kQ = 0;                                         // [tile][part][row] of 128 bytes
     static constexpr uint32_t kK = kQ + kTiles * kParts * kRows * 128;        // [buffer][part][key]
     static constexpr uint32_t kV = kK + kBuffers * kParts * kTile;
-    static constexpr uint32_t kControl = kV + kBuffers * kParts * kTile;
-    static constexpr uint32_t kBytes = kControl + 512 + 3 * kTiles * kRows * 4;
+    static constexpr uint32_t kRaw = kV + kBuffers * kParts * kTile;          // [stage][K, V][piece]
+    static constexpr uint32_t kControl = kRaw + kAhead * kCodes;
+    static constexpr uint32_t kBytes = kControl + 512 + kRowWords * kTiles * kRows * 4;
     static constexpr uint32_t kAlloc = kBytes + 1024;
+    static_assert(kColumnO + kTiles * kSets * DIM <= kTmemColumns, "tensor memory has 512 columns");
     static_assert(kControl >= kTiles * kRows * DIM * 4, "the sums that a cluster joins lie where the operands were");
 };
 
 // beside the operands
 struct Control {
-    uint64_t full[kBuffers];           // operands of a stage are there
-    uint64_t empty[kBuffers];          // both tiles' P V are done with them
+    uint64_t full[kBuffersMost];           // operands of a stage are there
+    uint64_t empty[kBuffersMost];          // both tiles' P V are done with them
     uint64_t scores[kTiles][2];
     uint64_t weights[kTiles][2];
     uint64_t product[kTiles][2];       // P V of an even / odd stage is complete: one barrier could be two phases behind
     uint64_t drained[kTiles];          // after a wait ran out: no MMA is in flight any more
-    alignas(16) float key_scales[kBuffers][kPagesPerStage];   // read four at a time
-    alignas(16) unsigned long long nan_keys[kBuffers][kPageWarps];   // of each page warp: keys with a NaN among their values
-    uint32_t bad_pages[kBuffers];      // unassigned pages of the stage, one bit each
-    uint32_t odd[kBuffers];            // a byte of each page warp: whether any of the two words above is not 0
+    alignas(16) float key_scales[kBuffersMost][kPagesPerStage];   // read four at a time
+    alignas(16) unsigned long long nan_keys[kBuffersMost][kPageWarps];   // of each page warp: keys with a NaN among their values
+    uint32_t bad_pages[kBuffersMost];      // unassigned pages of the stage, one bit each
+    uint32_t odd[kBuffersMost];            // a byte of each page warp: whether any of the two words above is not 0
     uint32_t tmem;
     uint32_t abort;
 };
@@ -151,9 +162,43 @@ __device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t b, uint
         "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
         : "memory");
 }
+// Columns of this thread's lane of tensor memory.  Load and wait are one statement: nothing the compiler knows of keeps the first
+// use of a register, and with it the end of its life, behind a wait that is a statement of its own.
+__device__ __forceinline__ void load_columns(uint32_t address, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(address)
+        : "memory");
+}
+__device__ __forceinline__ void load_columns(uint32_t address, uint32_t (&a)[16], uint32_t (&b)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(a[0]), "=r"(a[1]), "=r"(a[2]), "=r"(a[3]), "=r"(a[4]), "=r"(a[5]), "=r"(a[6]), "=r"(a[7]), "=r"(a[8]),
+          "=r"(a[9]), "=r"(a[10]), "=r"(a[11]), "=r"(a[12]), "=r"(a[13]), "=r"(a[14]), "=r"(a[15]), "=r"(b[0]), "=r"(b[1]),
+          "=r"(b[2]), "=r"(b[3]), "=r"(b[4]), "=r"(b[5]), "=r"(b[6]), "=r"(b[7]), "=r"(b[8]), "=r"(b[9]), "=r"(b[10]),
+          "=r"(b[11]), "=r"(b[12]), "=r"(b[13]), "=r"(b[14]), "=r"(b[15])
+        : "r"(address)
+        : "memory");
+}
 __device__ __forceinline__ void store_shared(uint32_t address, uint4 v) {
     asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(address), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
+__device__ __forceinline__ uint4 load_shared(uint32_t address) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(address) : "memory");
+    return v;
+}
+__device__ __forceinline__ void copy_async(uint32_t shared, const void* global) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(shared), "l"(global) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <uint32_t LEFT>
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory"); }
 __device__ __forceinline__ void cluster_barrier() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n"
                  "barrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -176,9 +221,13 @@ __device__ __forceinline__ uint32_t visible_bits(uint32_t base, uint32_t positio
 }
 
 template <uint32_t DIM>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(Layout<DIM>::kThreads, 1)
 e4m3_prompt_attention_kernel(const PromptParams p) {
     using L = Layout<DIM>;
+    constexpr uint32_t kSoftmaxWarps = L::kSoftmaxWarps;
+    constexpr uint32_t kThreads = L::kThreads;
+    constexpr uint32_t kSets = L::kSets;
+    constexpr uint32_t kBuffers = L::kBuffers;
     const uint32_t warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
     const uint32_t lane = threadIdx.x & 31;
     pdl_launch_dependents();
@@ -228,6 +277,25 @@ e4m3_prompt_attention_kernel(const PromptParams p) {
     const uint32_t cta_end = min(cta_begin + p.cta_tokens, segment_end);
     const uint32_t table_row = p.request_slots[segment_begin];
     const uint64_t origin = p.position_ids[segment_begin];            // position of the segment's first token
+
+    // ---- rows: this thread's token and head.  Their loads are under way together with those of the segment ----
+    const uint32_t tile = (warp / 4) % kTiles;           // of the softmax warps
+    const uint32_t set = warp / (4 * kTiles);
+    const uint32_t row = threadIdx.x % kRows;            // of the tile
+    const uint32_t row_token = cta_begin + tile * p.tile_tokens + row / p.chunk_heads;
+    const uint32_t head = chunk * p.chunk_heads + row % p.chunk_heads;   // of the group
+    const size_t out_row = (static_cast<size_t>(row_token) * p.query_heads + kv_head * p.group + head) * DIM;
+    constexpr uint32_t kLanes = DIM / 8;                 // of a row of queries, 16 bytes each
+    constexpr uint32_t kPasses = kLanes / kSets;         // of 32 / kLanes rows; the sets share them
+    bool live = warp < kSoftmaxWarps && row < p.tile_tokens * p.chunk_heads && row_token < cta_end && head < p.group;
+    uint32_t row_slot = 0;
+    uint32_t row_position = 0;
+    if (warp < kSoftmaxWarps) {
+        if (live) {
+            row_slot = p.request_slots[row_token];
+            row_position = p.position_ids[row_token];
+        }
+    }
     const uint64_t first_wide = origin + (cta_begin - segment_begin);
     const uint64_t most_positions = p.block_table_stride * kPageSize;
     if (table_row >= p.block_table_rows || first_wide >= most_positions) {
@@ -254,7 +322,7 @@ e4m3_prompt_attention_kernel(const PromptParams p) {
     const uint32_t base = smem_u32(smem);
     Control* control = reinterpret_cast<Control*>(smem + L::kControl);
     volatile uint32_t* abort = &control->abort;
-    float* joined = reinterpret_cast<float*>(smem + L::kControl + 512);   // maximum, sum, result of each row
+    float* row_words = reinterpret_cast<float*>(smem + L::kControl + 512);
     const uint32_t bar_full = smem_u32(control->full);
     const uint32_t bar_empty = smem_u32(control->empty);
     const uint32_t bar_scores = smem_u32(control->scores);
@@ -279,12 +347,9 @@ e4m3_prompt_attention_kernel(const PromptParams p) {
         tmem_allocate(smem_u32(&control->tmem), kTmemColumns);
     }
 
-    // ---- rows: this thread's token and head ----
-    const uint32_t tile = (warp / 4) % kTiles;           // of the softmax warps
-    const uint32_t row = threadIdx.x % kRows;            // of the tile
-    const uint32_t row_token = cta_begin + tile * p.tile_tokens + row / p.chunk_heads;
-    const uint32_t head = chunk * p.chunk_heads + row % p.chunk_heads;   // of the group
     const uint64_t row_wide = first_wide + (row_token - cta_begin);
+    live = live && row_wide < most_positions && row_slot == table_row && row_position == row_wide;
+    float* own_words = row_words + tile * (L::kRowWords * kRows) + row;
     // All threads meet once the barriers, the tensor memory and the queries are there; each role first does what needs none of them.
     auto meet = [&]() -> uint32_t {
         tcgen05_fence_before();
@@ -299,8 +364,9 @@ e4m3_prompt_attention_kernel(const PromptParams p) {
     float sum = 0.0f;
     bool poisoned = false;       // sees a NaN value
     bool lost = false;           // sees an unassigned page
-    bool live = false;
     bool ok = true;
+    bool valid = false;
+    float weight[kSets];         // of each set's sums
 
     if (warp >= kSoftmaxWarps && warp < kSoftmaxWarps + kPageWarps) {
         // -------------------------------------------------------------------------------- pages
@@ -319,8 +385,7 @@ e4m3_prompt_attention_kernel(const PromptParams p) {
             const uint32_t index = (begin_stage + stage) * kPagesPerStage + lane;
             return index < pages.count ? __ldg(table + pages.logical(index)) : 0;
         };
-        uint4 key_codes[kLoads];
-        uint4 value_codes[kLoads];
+        const uint32_t raw = base + L::kRaw + thread * 16;           // each thread reads what it has copied itself
         uint32_t entries = 0;
         uint32_t coming = look_up(0);
         uint32_t bad[2] = {0, 0};                                    // of the stages at hand and of those before
@@ -343,18 +408,21 @@ e4m3_prompt_attention_kernel(const PromptParams p) {
 #pragma unroll
             for (uint32_t i = 0; i < kLoads; ++i) {
                 const uint64_t offset = static_cast<uint64_t>(__shfl_sync(0xffffffffu, entries, stage % kBlock * kPagesPerStage + page_of(i))) * page_bytes;
-                key_codes[i] = __ldg(reinterpret_cast<const uint4*>(key_source + offset));
-                value_codes[i] = __ldg(reinterpret_cast<const uint4*>(value_source + offset));
+                copy_async(raw + stage % L::kAhead * L::kCodes + i * 2048, key_source + offset);
+                copy_async(raw + stage % L::kAhead * L::kCodes + (kLoads + i) * 2048, value_source + offset);
             }
         };
         // where a piece's 32 bytes go: two pieces of 16 of its key's row
         const uint32_t turn = (thread / kPieces) & 7;
         uint32_t buffer = 0;
-        if (stages > 0) load(0);
+        for (uint32_t stage = 0; stage < L::kAhead; ++stage) {
+            if (stage < stages) load(stage);
+            copies_commit();
+        }
         meet();
         for (uint32_t stage = 0; stage < stages; ++stage) {
             // the block of 8 stages that is at hand may be the next one's already
-            const uint32_t older = stage % kBlock == kBlock - 1 && stage + 1 < stages ? 1 : 0;
+            const uint32_t older = min(stage + L::kAhead, stages) - 1 >= (stage / kBlock + 1) * kBlock ? 1 : 0;
             if (stage >= kBuffers) {
                 ok = *abort == 0 && mbar_wait_bounded(bar_empty + 8 * buffer, (stage / kBuffers - 1) & 1, p.wait_limit_ns);
                 if (!__all_sync(0xffffffffu, ok)) {
@@ -362,14 +430,14 @@ e4m3_prompt_attention_kernel(const PromptParams p) {
                     break;
                 }
             }
+            copies_wait<L::kAhead - 1>();
             uint4 k_now[kLoads];
             uint4 v_now[kLoads];
 #pragma unroll
             for (uint32_t i = 0; i < kLoads; ++i) {
-                k_now[i] = key_codes[i];
-                v_now[i] = value_codes[i];
+                k_now[i] = load_shared(raw + stage % L::kAhead * L::kCodes + i * 2048);
+                v_now[i] = load_shared(raw + stage % L::kAhead * L::kCodes + (kLoads + i) * 2048);
             }
-            if (stage + 1 < stages) load(stage + 1);
             const uint32_t k_base = base + L::kK + buffer * (L::kParts * kTile);
             const uint32_t v_base = base + L::kV + buffer * (L::kParts * kTile);
             uint32_t check = 0;                                      // f16 sums of values: NaN where one of them is
@@ -445,7 +513,11 @@ e4m3_prompt_attention_kernel(const PromptParams p) {
             __syncwarp();
             if (lane == 0 && !(p.selftest_drop != 0 && page_warp == 0 && stage == 0)) mbar_arrive(bar_full + 8 * buffer);
             buffer = buffer + 1 == kBuffers ? 0 : buffer + 1;
+            // into the place of the codes that have just been converted
+            if (stage + L::kAhead < stages) load(stage + L::kAhead);
+            copies_commit();
         }
+        copies_wait<0>();
         if (!ok && lane == 0 && *abort == 0) {
             *abort = 1;
             record_wait_timeout(p.status, kTagE4m3Prompt, (blockIdx.x << 2) | 1);
@@ -454,27 +526,31 @@ e4m3_prompt_attention_kernel(const PromptParams p) {
         // -------------------------------------------------------------------------------- MMA issuers, one for each tile
         const uint32_t which = warp - (kSoftmaxWarps + kPageWarps);
         tmem = meet();
-        if (elect_one()) {
-            // f32 results of 128 rows; Q K^T: f16, both K-major, 64 keys; P V: bf16, V MN-major, 64 dimensions
-            constexpr uint32_t idesc_scores = (1u << 4) | ((kKeys >> 3) << 17) | ((kRows >> 4) << 24);
-            constexpr uint32_t idesc_product = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((64u >> 3) << 17) | ((kRows >> 4) << 24);
-            const uint32_t my_stages = stages_of(which);
-            const uint64_t q_desc = smem_descriptor(base + L::kQ + which * (L::kParts * kRows * 128));
-            const uint64_t k_first = smem_descriptor(base + L::kK);
-            const uint64_t v_first = smem_descriptor(base + L::kV);
-            const uint32_t columns = tmem + kColumnS + 2 * which * kKeys;
-            const uint32_t output_columns = tmem + kColumnO + which * DIM;
-            const uint32_t my_scores = bar_scores + 16 * which;
-            const uint32_t my_weights = bar_weights + 16 * which;
-            const uint32_t my_product = bar_product + 16 * which;
-            bool running = true;
-            uint32_t next_buffer = 0;      // of the next scores
-            uint32_t next_parity = 0;
-            auto issue_scores = [&](uint32_t parity) -> bool {
-                if (*abort || !mbar_wait_bounded(bar_full + 8 * next_buffer, next_parity, p.wait_limit_ns)) {
-                    return false;
-                }
-                tcgen05_fence_after();
+        // The warp stays together: all lanes wait, one of them issues.
+        // f32 results of 128 rows; Q K^T: f16, both K-major, 64 keys; P V: bf16, V MN-major, 64 dimensions
+        constexpr uint32_t idesc_scores = (1u << 4) | ((kKeys >> 3) << 17) | ((kRows >> 4) << 24);
+        constexpr uint32_t idesc_product = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((64u >> 3) << 17) | ((kRows >> 4) << 24);
+        const uint32_t my_stages = stages_of(which);
+        const uint64_t q_desc = smem_descriptor(base + L::kQ + which * (L::kParts * kRows * 128));
+        const uint64_t k_first = smem_descriptor(base + L::kK);
+        const uint64_t v_first = smem_descriptor(base + L::kV);
+        const uint32_t columns = tmem + kColumnS + 2 * which * kKeys;
+        const uint32_t output_columns = tmem + kColumnO + which * DIM;
+        const uint32_t my_scores = bar_scores + 16 * which;
+        const uint32_t my_weights = bar_weights + 16 * which;
+        const uint32_t my_product = bar_product + 16 * which;
+        uint32_t next_buffer = 0;      // of the next scores
+        uint32_t next_parity = 0;
+        auto wait_for = [&](uint32_t barrier, uint32_t parity) -> bool {
+            const bool came = *abort == 0 && mbar_wait_bounded(barrier, parity, p.wait_limit_ns);
+            return __all_sync(0xffffffffu, came);
+        };
+        auto issue_scores = [&](uint32_t parity) -> bool {
+            if (!wait_for(bar_full + 8 * next_buffer, next_parity)) {
+                return false;
+            }
+            tcgen05_fence_after();
+            if (elect_one()) {
                 const uint64_t k_desc = k_first + next_buffer * (L::kParts * kTile >> 4);
 #pragma unroll
                 for (uint32_t ks = 0; ks < DIM / 16; ++ks) {   // 16 dimensions: 32 bytes within the swizzled row
@@ -482,76 +558,76 @@ e4m3_prompt_attention_kernel(const PromptParams p) {
                             k_desc + (ks / 4) * (kTile >> 4) + (ks % 4) * 2, idesc_scores, ks);
                 }
                 umma_commit(my_scores + 8 * parity);
-                if (++next_buffer == kBuffers) {
-                    next_buffer = 0;
-                    next_parity ^= 1;
-                }
-                return true;
-            };
-            for (uint32_t stage = 0; stage < 2 && running; ++stage) {
-                if (stage < my_stages) running = issue_scores(stage);
             }
-            uint32_t buffer = 0;
-            for (uint32_t stage = 0; stage < my_stages && running; ++stage) {
-                const uint32_t parity = stage & 1;
-                if (*abort || !mbar_wait_bounded(my_weights + 8 * parity, (stage >> 1) & 1, p.wait_limit_ns)) {
-                    running = false;
-                    break;
-                }
-                tcgen05_fence_after();
+            __syncwarp();
+            if (++next_buffer == kBuffers) {
+                next_buffer = 0;
+                next_parity ^= 1;
+            }
+            return true;
+        };
+        for (uint32_t stage = 0; stage < 2 && ok; ++stage) {
+            if (stage < my_stages) ok = issue_scores(stage);
+        }
+        uint32_t buffer = 0;
+        for (uint32_t stage = 0; stage < my_stages && ok; ++stage) {
+            const uint32_t parity = stage & 1;
+            ok = wait_for(my_weights + 8 * parity, (stage >> 1) & 1);
+            if (!ok) break;
+            tcgen05_fence_after();
+            if (elect_one()) {
                 const uint64_t v_desc = v_first + buffer * (L::kParts * kTile >> 4);
 #pragma unroll
                 for (uint32_t part = 0; part < L::kParts; ++part) {
 #pragma unroll
                     for (uint32_t step = 0; step < kPagesPerStage; ++step) {   // 16 keys: 8 columns of weights, 2 KiB of V
-                        umma_ts(output_columns + part * 64, columns + parity * kKeys + step * 8,
-                                v_desc + part * (kTile >> 4) + step * (2048 >> 4), idesc_product, stage > 0 || step > 0);
+                        umma_ts(output_columns + stage % kSets * (kTiles * DIM) + part * 64, columns + parity * kKeys + step / 2 * 32 + step % 2 * 8,
+                                v_desc + part * (kTile >> 4) + step * (2048 >> 4), idesc_product, stage >= kSets || step > 0);
                     }
                 }
                 umma_commit(my_product + 8 * parity);
                 // Only where the buffer is filled once more: an arrival that nobody waits for may come when the CTA has gone, and
                 // its shared memory with it.
                 if (stage + kBuffers < stages) umma_commit(bar_empty + 8 * buffer);
-                // Behind it the scores of two stages on: MMAs execute in order, so the weights in their columns have been consumed.
-                if (stage + 2 < my_stages && !issue_scores(parity)) running = false;
-                if (++buffer == kBuffers) buffer = 0;
             }
-            // stages that only the other tile takes part in
-            for (uint32_t stage = my_stages; stage + kBuffers < stages && running; ++stage) {
-                running = *abort == 0 && mbar_wait_bounded(bar_full + 8 * (stage % kBuffers), (stage / kBuffers) & 1, p.wait_limit_ns);
-                if (running) mbar_arrive(bar_empty + 8 * (stage % kBuffers));
-            }
-            if (!running && *abort == 0) {
-                *abort = 1;
-                record_wait_timeout(p.status, kTagE4m3Prompt, (blockIdx.x << 2) | 2);
-            }
-            if (*abort != 0) {
-                umma_commit(smem_u32(control->drained) + 8 * which);
-                (void)mbar_wait_bounded(smem_u32(control->drained) + 8 * which, 0, p.wait_limit_ns);
-            }
+            __syncwarp();
+            // Behind it the scores of two stages on: MMAs execute in order, so the weights in their columns have been consumed.
+            if (stage + 2 < my_stages) ok = issue_scores(parity);
+            if (++buffer == kBuffers) buffer = 0;
+        }
+        // stages that only the other tile takes part in
+        for (uint32_t stage = my_stages; stage + kBuffers < stages && ok; ++stage) {
+            ok = wait_for(bar_full + 8 * (stage % kBuffers), (stage / kBuffers) & 1);
+            if (ok && lane == 0) mbar_arrive(bar_empty + 8 * (stage % kBuffers));
+            __syncwarp();
+        }
+        if (!ok && lane == 0 && *abort == 0) {
+            *abort = 1;
+            record_wait_timeout(p.status, kTagE4m3Prompt, (blockIdx.x << 2) | 2);
+        }
+        __syncwarp();
+        if (__any_sync(0xffffffffu, *abort != 0)) {
+            if (elect_one()) umma_commit(smem_u32(control->drained) + 8 * which);
+            __syncwarp();
+            (void)mbar_wait_bounded(smem_u32(control->drained) + 8 * which, 0, p.wait_limit_ns);
         }
     } else {
         // -------------------------------------------------------------------------------- softmax
-        // ---- queries to f16, by a power of two per row: DIM / 8 lanes a row, 16 bytes each ----
-        live = row < p.tile_tokens * p.chunk_heads && row_token < cta_end && head < p.group && row_wide < most_positions;
+        // ---- queries to f16, by a power of two per row ----
         const uint64_t row_offset = live ? row_token * p.query_token_stride + static_cast<size_t>(kv_head * p.group + head) * DIM : 0;
-        if (live) live = p.request_slots[row_token] == table_row && p.position_ids[row_token] == row_wide;
-        constexpr uint32_t kLanes = DIM / 8;
-        constexpr uint32_t kPasses = kLanes;              // of 32 / kLanes rows
         uint4 raw_query[kPasses];
 #pragma unroll
         for (uint32_t pass = 0; pass < kPasses; ++pass) {
-            const uint32_t source = pass * (32 / kLanes) + lane / kLanes;
+            const uint32_t source = (set * kPasses + pass) * (32 / kLanes) + lane / kLanes;
             const uint32_t low = __shfl_sync(0xffffffffu, static_cast<uint32_t>(row_offset), source);
             const uint32_t high = __shfl_sync(0xffffffffu, static_cast<uint32_t>(row_offset >> 32), source);
             // rows that do not exist read the first query of the batch, and are cleared below
             raw_query[pass] = *reinterpret_cast<const uint4*>(p.query + ((static_cast<uint64_t>(high) << 32) | low) + lane % kLanes * 8);
         }
         const uint32_t live_rows = __ballot_sync(0xffffffffu, live);
-        float row_factor = 0.0f;
 #pragma unroll
         for (uint32_t pass = 0; pass < kPasses; ++pass) {
-            const uint32_t source = pass * (32 / kLanes) + lane / kLanes;
+            const uint32_t source = (set * kPasses + pass) * (32 / kLanes) + lane / kLanes;
             const bool there = (live_rows >> source) & 1;
             const uint32_t words[4] = {there ? raw_query[pass].x : 0, there ? raw_query[pass].y : 0, there ? raw_query[pass].z : 0,
                                        there ? raw_query[pass].w : 0};
@@ -566,9 +642,6 @@ e4m3_prompt_attention_kernel(const PromptParams p) {
             for (uint32_t delta = kLanes / 2; delta > 0; delta >>= 1) largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, delta));
             const int32_t exponent = min(max(static_cast<int32_t>(largest >> 7) - 127 - 11, -126), 126);
             const float factor = power_of_two(-exponent);
-            // the thread of this row is lane `source`: it takes the factor from the first lane that has it
-            const float whole_factor = __shfl_sync(0xffffffffu, power_of_two(exponent) * p.scale_log2, lane % (32 / kLanes) * kLanes);
-            if (lane / (32 / kLanes) == pass) row_factor = whole_factor;
             uint32_t half[4];
 #pragma unroll
             for (uint32_t i = 0; i < 4; ++i) {
@@ -577,18 +650,20 @@ e4m3_prompt_attention_kernel(const PromptParams p) {
             }
             const uint32_t target = warp % 4 * 32 + source;             // row of the tile
             const uint32_t piece = lane % kLanes;
+            if (piece == 0) row_words[(tile * L::kRowWords + 3) * kRows + target] = power_of_two(exponent) * p.scale_log2;
             store_shared(base + L::kQ + (tile * L::kParts + piece / 8) * (kRows * 128) + target * 128 + (((piece % 8) ^ (target & 7)) << 4),
                          make_uint4(half[0], half[1], half[2], half[3]));
         }
         fence_proxy_async_smem();
         tmem = meet();
 
+        const float row_factor = own_words[3 * kRows];
         const uint32_t position = live ? static_cast<uint32_t>(row_wide) : last_position;
         const uint32_t first_key = p.window != 0 && position >= p.window ? position - p.window + 1 : 0;
         const uint32_t lane_address = tmem + ((warp % 4 * 32) << 16);
-        const uint32_t output_columns = lane_address + kColumnO + tile * DIM;
+        const uint32_t output_columns = lane_address + kColumnO + (set * kTiles + tile) * DIM;
         const uint32_t my_stages = stages_of(tile);
-        // weights of the stage before: complete, and handed over
+        // weights complete, and handed over
         auto hand_over = [&](uint32_t stage) {
             tmem_store_wait();
             tcgen05_fence_before();
@@ -606,9 +681,9 @@ e4m3_prompt_attention_kernel(const PromptParams p) {
         const int32_t until = whole_last >= 0 ? whole_last / static_cast<int32_t>(kPagesPerStage) + 1 - static_cast<int32_t>(begin_stage) : 0;
         const uint32_t whole_begin = static_cast<uint32_t>(from);
         const uint32_t whole_count = static_cast<uint32_t>(max(until - from, 0));
-        uint32_t buffer = 0;
+        uint32_t buffer = set;
         uint32_t buffer_parity = 0;
-        for (uint32_t stage = 0; stage < my_stages; ++stage) {
+        for (uint32_t stage = set; stage < my_stages; stage += kSets) {
             // ---- the page warps' words (there before the scores are) ----
             const bool fast = stage - whole_begin < whole_count;
             // the keys of the stage that this row sees, where that is asked for
@@ -640,8 +715,9 @@ e4m3_prompt_attention_kernel(const PromptParams p) {
                     lost = lost || (((bad >> sub) & 1) != 0 && ((seen >> (16 * sub)) & 0xffffu) != 0);
                 }
             }
-            if (++buffer == kBuffers) {
-                buffer = 0;
+            buffer += kSets;
+            if (buffer >= kBuffers) {
+                buffer -= kBuffers;
                 buffer_parity ^= 1;
             }
             ok = ok && mbar_wait_bounded(bar_scores + 8 * (2 * tile + (stage & 1)), (stage >> 1) & 1, p.wait_limit_ns);
@@ -651,94 +727,102 @@ e4m3_prompt_attention_kernel(const PromptParams p) {
             }
             tcgen05_fence_after();
             const uint32_t columns = lane_address + kColumnS + (2 * tile + (stage & 1)) * kKeys;
-            uint32_t raw[4][16];
-#pragma unroll
-            for (uint32_t part = 0; part < 4; ++part) tmem_load16_nowait(columns + part * 16, raw[part]);
-            if (stage > 0) hand_over(stage - 1);          // while the scores come
-            // The rest in two copies: tests of single keys, which the compiler would make predicates of every stage, were a quarter of
-            // all instructions (177 us for eight portions of 512 tokens).
+            // In two copies: tests of single keys, which the compiler would make predicates of every stage, were a quarter of all
+            // instructions.
             auto weigh = [&](auto masked) -> bool {
+                constexpr bool kMasked = decltype(masked)::value;
                 uint32_t bits[2] = {0, 0};
-                if constexpr (decltype(masked)::value) seen_keys(bits);
+                if constexpr (kMasked) seen_keys(bits);
+                // 32 keys at a time, the first ones twice: all scores at once leave no registers for this many warps
+                uint32_t raw[2][16];
+                auto fetch = [&](uint32_t half) {
+                    load_columns(columns + half * 32, raw[0], raw[1]);
+                };
                 // ---- maximum ----
-                if constexpr (decltype(masked)::value) {
-                    // masked scores, whatever they are, become -inf (the factor is positive or 0, so not by the product)
-#pragma unroll
-                    for (uint32_t j = 0; j < kKeys; ++j) {
-                        if (((bits[j / 32] >> (j % 32)) & 1) == 0) raw[j / 16][j % 16] = 0xff800000u;
-                    }
-                }
                 float most = -INFINITY;
 #pragma unroll
-                for (uint32_t sub = 0; sub < kPagesPerStage; ++sub) {
-                    float a = __uint_as_float(raw[sub][0]);
-                    float b = __uint_as_float(raw[sub][1]);
+                for (uint32_t half = 0; half < 2; ++half) {
+                    fetch(half);
+                    if constexpr (kMasked) {
+                        // masked scores, whatever they are, become -inf (the factor is positive or 0, so not by the product)
 #pragma unroll
-                    for (uint32_t j = 2; j < 16; j += 4) {
-                        a = max3(a, __uint_as_float(raw[sub][j]), __uint_as_float(raw[sub][j + 1]));
-                        if (j + 2 < 16) b = max3(b, __uint_as_float(raw[sub][j + 2]), __uint_as_float(raw[sub][j + 3]));
+                        for (uint32_t j = 0; j < 32; ++j) {
+                            if (((bits[half] >> j) & 1) == 0) raw[j / 16][j % 16] = 0xff800000u;
+                        }
                     }
-                    const float here = fmaxf(a, b);
-                    most = fmaxf(most, here * factor[sub]);
+#pragma unroll
+                    for (uint32_t sub = 0; sub < 2; ++sub) {
+                        float a = __uint_as_float(raw[sub][0]);
+                        float b = __uint_as_float(raw[sub][1]);
+#pragma unroll
+                        for (uint32_t j = 2; j < 16; j += 4) {
+                            a = max3(a, __uint_as_float(raw[sub][j]), __uint_as_float(raw[sub][j + 1]));
+                            if (j + 2 < 16) b = max3(b, __uint_as_float(raw[sub][j + 2]), __uint_as_float(raw[sub][j + 3]));
+                        }
+                        const float here = fmaxf(a, b);
+                        most = fmaxf(most, here * factor[half * 2 + sub]);
+                    }
                 }
                 const bool raise = most > reference + kHeadroom;
                 if (__any_sync(0xffffffffu, raise)) {
                     const float shrink = !raise ? 1.0f : reference == -INFINITY ? 0.0f : fast_exp2(reference - most);
                     if (raise) reference = most;
                     sum *= shrink;
-                    if (stage > 0) {
-                        ok = *abort == 0 && mbar_wait_bounded(bar_product + 8 * (2 * tile + ((stage - 1) & 1)), ((stage - 1) >> 1) & 1, p.wait_limit_ns);
+                    if (stage >= kSets) {
+                        const uint32_t before = stage - kSets;
+                        ok = *abort == 0 && mbar_wait_bounded(bar_product + 8 * (2 * tile + (before & 1)), (before >> 1) & 1, p.wait_limit_ns);
                         if (!__all_sync(0xffffffffu, ok)) {
                             return false;
                         }
                         tcgen05_fence_after();
-#pragma unroll
+#pragma unroll 1
                         for (uint32_t c = 0; c < DIM; c += 16) {
                             uint32_t o[16];
-                            tmem_load16(output_columns + c, o);
+                            load_columns(output_columns + c, o);
 #pragma unroll
                             for (uint32_t j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * shrink);
                             tmem_store16(output_columns + c, o);
                         }
                     }
                 }
-                // ---- weights ----
+                // ---- weights, of the keys at hand first ----
                 const float reference_offset = reference == -INFINITY ? 0.0f : -reference;
                 const uint64_t offset = pair_of(reference_offset, reference_offset);
                 uint64_t part_sum[2] = {0, 0};
 #pragma unroll
-                for (uint32_t half = 0; half < 2; ++half) {
+                for (uint32_t turn = 0; turn < 2; ++turn) {
+                    const uint32_t half = 1 - turn;
+                    if (turn == 1) fetch(half);
                     uint32_t packed[16];
 #pragma unroll
                     for (uint32_t sub = 0; sub < 2; ++sub) {
                         const uint64_t multiplier = pair_of(factor[half * 2 + sub], factor[half * 2 + sub]);
 #pragma unroll
                         for (uint32_t pair = 0; pair < 8; ++pair) {
-                            const uint32_t j = half * 32 + sub * 16 + pair * 2;
-                            float2 w = pair_out(pair_fma(pair_of(__uint_as_float(raw[j / 16][j % 16]), __uint_as_float(raw[j / 16][j % 16 + 1])),
+                            const uint32_t j = sub * 16 + pair * 2;
+                            float2 w = pair_out(pair_fma(pair_of(__uint_as_float(raw[sub][pair * 2]), __uint_as_float(raw[sub][pair * 2 + 1])),
                                                          multiplier, offset));
                             w = make_float2(fast_exp2(w.x), fast_exp2(w.y));
-                            if constexpr (decltype(masked)::value) {
-                                w.x = (bits[j / 32] >> (j % 32)) & 1 ? w.x : 0.0f;
-                                w.y = (bits[j / 32] >> (j % 32 + 1)) & 1 ? w.y : 0.0f;
+                            if constexpr (kMasked) {
+                                w.x = (bits[half] >> j) & 1 ? w.x : 0.0f;
+                                w.y = (bits[half] >> (j + 1)) & 1 ? w.y : 0.0f;
                             }
                             packed[sub * 8 + pair] = pack_bf16x2(w.x, w.y);
                             part_sum[pair & 1] = pair_add(part_sum[pair & 1], pair_of(w.x, w.y));   // unrounded: roundings average out
                         }
                     }
-                    tmem_store16(columns + half * 16, packed);
+                    tmem_store16(columns + half * 32, packed);
                 }
                 const float2 stage_sum = pair_out(pair_add(part_sum[0], part_sum[1]));
                 sum += stage_sum.x + stage_sum.y;
                 return true;
             };
-            tmem_load_wait();
             ok = fast ? weigh(std::false_type()) : weigh(std::true_type());
             if (!ok) break;
+            hand_over(stage);
         }
-        if (ok && my_stages > 0) {
-            const uint32_t last = my_stages - 1;
-            hand_over(last);
+        if (ok && my_stages > set) {
+            const uint32_t last = my_stages - 1 - (my_stages - 1 - set) % kSets;      // of this set
             ok = *abort == 0 && mbar_wait_bounded(bar_product + 8 * (2 * tile + (last & 1)), (last >> 1) & 1, p.wait_limit_ns);
             ok = __all_sync(0xffffffffu, ok);
         }
@@ -748,93 +832,115 @@ e4m3_prompt_attention_kernel(const PromptParams p) {
         }
         tcgen05_fence_after();
         if (poisoned) sum = __int_as_float(0x7fc00000);
-        const size_t out_row = (static_cast<size_t>(row_token) * p.query_heads + kv_head * p.group + head) * DIM;
-        if (p.splits == 1) {
-            const float inverse = 1.0f / sum;
+        valid = ok && !lost && *abort == 0;
+        // ---- the sets' results together ----
+        if constexpr (kSets > 1) {
+            own_words[(4 + 3 * set) * kRows] = reference;
+            own_words[(5 + 3 * set) * kRows] = sum;
+            own_words[(6 + 3 * set) * kRows] = valid ? 1.0f : 0.0f;
+            asm volatile("barrier.sync 2, %0;" ::"n"(kSoftmaxWarps * 32) : "memory");
+            reference = fmaxf(own_words[4 * kRows], own_words[7 * kRows]);
+            valid = own_words[6 * kRows] != 0.0f && own_words[9 * kRows] != 0.0f;
+            const float offset = reference == -INFINITY ? 0.0f : reference;
+            sum = 0.0f;
 #pragma unroll
-            for (uint32_t c = 0; c < DIM; c += 16) {
+            for (uint32_t i = 0; i < kSets; ++i) {
+                weight[i] = fast_exp2(own_words[(4 + 3 * i) * kRows] - offset);
+                sum = fmaf(own_words[(5 + 3 * i) * kRows], weight[i], sum);
+            }
+        } else {
+            weight[0] = 1.0f;
+        }
+    }
+
+    __syncwarp();
+    if (p.splits > 1) {
+        // nobody writes operands any more, and the products have been waited for: the sums for the cluster lie there, one column of
+        // 128 rows behind the other
+        __syncthreads();
+    }
+    if (warp < kSoftmaxWarps) {
+        if (p.splits > 1) {
+            own_words[0] = reference;
+            own_words[kRows] = sum;
+            own_words[2 * kRows] = valid ? 1.0f : 0.0f;
+        }
+        // each set has its share of the dimensions
+        constexpr uint32_t kShare = DIM / kSets;
+        const uint32_t my_stages = stages_of(tile);
+        const uint32_t columns = tmem + ((warp % 4 * 32) << 16) + kColumnO + tile * DIM;
+        float* sums = reinterpret_cast<float*>(smem) + tile * (DIM * kRows) + row;
+        const float inverse = 1.0f / sum;
+#pragma unroll
+        for (uint32_t c = set * kShare; c < (set + 1) * kShare; c += 16) {
+            float value[16] = {};
+#pragma unroll
+            for (uint32_t i = 0; i < kSets; ++i) {
                 uint32_t o[16];
-                tmem_load16(output_columns + c, o);
-                if (ok && live && !lost && *abort == 0) {
+                __syncwarp();                  // the whole warp loads, also where only some rows are stored
+                load_columns(columns + i * kTiles * DIM + c, o);
+                if (my_stages > i) {           // else there are no sums
 #pragma unroll
-                    for (uint32_t h = 0; h < 2; ++h) {
-                        uint32_t pairs[4];
+                    for (uint32_t j = 0; j < 16; ++j) value[j] = fmaf(__uint_as_float(o[j]), weight[i], value[j]);
+                }
+            }
+            if (p.splits > 1) {
 #pragma unroll
-                        for (uint32_t j = 0; j < 4; ++j) {
-                            pairs[j] = pack_bf16x2(__uint_as_float(o[h * 8 + 2 * j]) * inverse, __uint_as_float(o[h * 8 + 2 * j + 1]) * inverse);
-                        }
-                        *reinterpret_cast<uint4*>(p.output + out_row + c + h * 8) = make_uint4(pairs[0], pairs[1], pairs[2], pairs[3]);
-                    }
+                for (uint32_t j = 0; j < 16; ++j) sums[(c + j) * kRows] = value[j];
+            } else if (live && valid) {
+#pragma unroll
+                for (uint32_t h = 0; h < 2; ++h) {
+                    uint32_t pairs[4];
+#pragma unroll
+                    for (uint32_t j = 0; j < 4; ++j) pairs[j] = pack_bf16x2(value[h * 8 + 2 * j] * inverse, value[h * 8 + 2 * j + 1] * inverse);
+                    *reinterpret_cast<uint4*>(p.output + out_row + c + h * 8) = make_uint4(pairs[0], pairs[1], pairs[2], pairs[3]);
                 }
             }
         }
     }
 
-    // single-lane roles meet their warps again in front of the CTA's barrier
-    __syncwarp();
     if (p.splits > 1) {
-        // ---- join the cluster: unscaled sums, one column of 128 rows behind the other, where the operands were ----
-        __syncthreads();                   // nobody writes operands any more, and the MMAs have been waited for
-        float* sums = reinterpret_cast<float*>(smem) + tile * (DIM * kRows);
-        float* joined_row = joined + tile * (3 * kRows) + row;
-        if (warp < kSoftmaxWarps) {
-            const uint32_t columns = tmem + ((warp % 4 * 32) << 16) + kColumnO + tile * DIM;
-            const bool valid = ok && !lost && *abort == 0;
-            const bool any = stages_of(tile) > 0;
-#pragma unroll
-            for (uint32_t c = 0; c < DIM; c += 16) {
-                uint32_t o[16];
-                tmem_load16(columns + c, o);
-#pragma unroll
-                for (uint32_t j = 0; j < 16; ++j) sums[(c + j) * kRows + row] = any ? __uint_as_float(o[j]) : 0.0f;
-            }
-            joined_row[0] = reference;
-            joined_row[kRows] = sum;
-            joined_row[2 * kRows] = valid ? 1.0f : 0.0f;
-        }
+        // ---- join the cluster ----
         __syncwarp();
         cluster_barrier();
         if (warp < kSoftmaxWarps) {
-            const uint32_t own = smem_u32(joined_row);
-            const uint32_t own_sums = smem_u32(sums);
+            const uint32_t own = smem_u32(own_words);
+            const uint32_t own_sums = base + (tile * (DIM * kRows) + row) * 4;
+            float weight[8];
+            float part_sum[8];
             float most = -INFINITY;
-            bool valid = live;
-            for (uint32_t r = 0; r < p.splits; ++r) {
-                most = fmaxf(most, load_cluster(own, r));
-                valid = valid && load_cluster(own + 2 * kRows * 4, r) != 0.0f;
+            bool complete = live;
+#pragma unroll
+            for (uint32_t r = 0; r < 8; ++r) {         // all loads under way at once
+                weight[r] = r < p.splits ? load_cluster(own, r) : -INFINITY;
+                part_sum[r] = r < p.splits ? load_cluster(own + kRows * 4, r) : 0.0f;
+                const float holds = r < p.splits ? load_cluster(own + 2 * kRows * 4, r) : 1.0f;
+                complete = complete & (holds != 0.0f);
+                most = fmaxf(most, weight[r]);
             }
             const float offset = most == -INFINITY ? 0.0f : most;
             float total = 0.0f;
-            float weight[8];
 #pragma unroll
             for (uint32_t r = 0; r < 8; ++r) {
-                weight[r] = 0.0f;
-                if (r < p.splits) {
-                    weight[r] = fast_exp2(load_cluster(own, r) - offset);
-                    total = fmaf(load_cluster(own + kRows * 4, r), weight[r], total);
-                }
+                weight[r] = fast_exp2(weight[r] - offset);
+                total = fmaf(part_sum[r], weight[r], total);
             }
             const float inverse = 1.0f / total;
             const uint32_t share = DIM / p.splits;       // 8 dimensions or more
-            const size_t out_row = (static_cast<size_t>(row_token) * p.query_heads + kv_head * p.group + head) * DIM;
-            for (uint32_t c = split * share; c < (split + 1) * share; c += 8) {
-                float value[8] = {};
+            for (uint32_t c = split * share + set * 4; c < (split + 1) * share; c += 4 * kSets) {
+                float value[4] = {};
 #pragma unroll
                 for (uint32_t r = 0; r < 8; ++r) {
                     if (r < p.splits) {
 #pragma unroll
-                        for (uint32_t j = 0; j < 8; ++j) {
-                            value[j] = fmaf(load_cluster(own_sums + ((c + j) * kRows + row) * 4, r), weight[r], value[j]);
+                        for (uint32_t j = 0; j < 4; ++j) {
+                            value[j] = fmaf(load_cluster(own_sums + ((c + j) * kRows) * 4, r), weight[r], value[j]);
                         }
                     }
                 }
-                if (valid) {
-                    uint4 out;
-                    out.x = pack_bf16x2(value[0] * inverse, value[1] * inverse);
-                    out.y = pack_bf16x2(value[2] * inverse, value[3] * inverse);
-                    out.z = pack_bf16x2(value[4] * inverse, value[5] * inverse);
-                    out.w = pack_bf16x2(value[6] * inverse, value[7] * inverse);
-                    *reinterpret_cast<uint4*>(p.output + out_row + c) = out;
+                if (complete) {
+                    *reinterpret_cast<uint2*>(p.output + out_row + c) = make_uint2(pack_bf16x2(value[0] * inverse, value[1] * inverse),
+                                                                                  pack_bf16x2(value[2] * inverse, value[3] * inverse));
                 }
             }
         }
@@ -854,7 +960,7 @@ cudaError_t launch_dim(cudaStream_t stream, const PromptParams& params, uint64_t
     if (status != cudaSuccess) {
         return status;
     }
-    return launch_kernel(e4m3_prompt_attention_kernel<DIM>, static_cast<unsigned int>(blocks), kThreads, Layout<DIM>::kAlloc, stream,
+    return launch_kernel(e4m3_prompt_attention_kernel<DIM>, static_cast<unsigned int>(blocks), Layout<DIM>::kThreads, Layout<DIM>::kAlloc, stream,
                          params.splits, params);
 }
 
@@ -893,9 +999,9 @@ cudaError_t launch_e4m3_prompt_attention(cudaStream_t stream, const E4m3Attentio
     if (launch.window != 0 && longest > static_cast<uint64_t>(launch.window) + launch.sinks + params.cta_tokens) {
         longest = static_cast<uint64_t>(launch.window) + launch.sinks + params.cta_tokens;
     }
-    // Shares of the keys as long as all CTAs run at once and each has a few stages (37 tokens behind 8000, 8 KV heads: 1 share 152,
-    // 2 84, 4 49, 8 32.6 us; 64 behind 500: 18.8, 17.7, 15.5, 16.7; 64 behind 200: 13.6, 15.2; 2 x 64 behind 4000, where 8 shares
-    // are 256 CTAs: 4 shares 31.4, 8 44.9).
+    // Shares of the keys as long as all CTAs run at once and each has a few stages (with one set of softmax warps: 37 tokens behind
+    // 8000, 8 KV heads: 1 share 152, 2 84, 4 49, 8 32.6 us; 64 behind 500: 18.8, 17.7, 15.5, 16.7; 64 behind 200: 13.6, 15.2;
+    // 2 x 64 behind 4000, where 8 shares are 256 CTAs: 4 shares 31.4, 8 44.9).
     params.splits = 1;
     while (params.splits < 8 && items * params.splits * 2 <= 148 && longest >= (2 * params.splits + 4) * kKeys) params.splits *= 2;
     const uint64_t blocks = items * params.splits;
