@@ -16,7 +16,7 @@
 // only then is O read, scaled and stored.  The query is brought to f16 by a power of two per row, which the scores get back
 // together with the page's scale in the multiply-add in front of the exponential.
 //
-// Eight portions of 512 tokens at depths of 0 to 3584, 32 heads on 8 of 64: 145 us, 0.47 PFLOP/s, where the exponentials alone (16 a
+// Eight portions of 512 tokens at depths of 0 to 3584, 32 heads on 8 of 64: 142 us, 0.49 PFLOP/s, where the exponentials alone (16 a
 // cycle and SM) need 60.  What bounds it is the chain of a stage through its roles, 1900 cycles: no unit is busy for much more than
 // half of that, page warps as long as softmax warps, and 11,000 cycles go to the ends of a CTA.  One set of softmax warps takes 156 us (166
 // with codes in registers one stage ahead); without its exponentials the kernel takes 139, without conversions 146, without both 133.
@@ -85,7 +85,7 @@ struct Layout {
     static constexpr uint32_t kSets = DIM == 64 ? 2 : 1;
     static constexpr uint32_t kSoftmaxWarps = 4 * kTiles * kSets;
     static constexpr uint32_t kThreads = (kSoftmaxWarps + kPageWarps + kTiles) * 32;
-    static constexpr uint32_t kRowWords = 4 + 3 * kSets;                      // maximum, sum, result; factor; the first three of each set
+    static constexpr uint32_t kRowWords = 3 + 3 * kSets;                      // of a row: maximum, sum, factor; of each set maximum, sum, whether they hold
     static constexpr uint32_t kBuffers = DIM == 64 ? 4 : 3;                   // of operands
     static constexpr uint32_t kAhead = 2;                                     // stages of codes under way
     static constexpr uint32_t kCodes = 2 * kKeys * DIM;                       // bytes of a stage
@@ -287,14 +287,12 @@ e4m3_prompt_attention_kernel(const PromptParams p) {
     const size_t out_row = (static_cast<size_t>(row_token) * p.query_heads + kv_head * p.group + head) * DIM;
     constexpr uint32_t kLanes = DIM / 8;                 // of a row of queries, 16 bytes each
     constexpr uint32_t kPasses = kLanes / kSets;         // of 32 / kLanes rows; the sets share them
-    bool live = warp < kSoftmaxWarps && row < p.tile_tokens * p.chunk_heads && row_token < cta_end && head < p.group;
+    const bool inside = warp < kSoftmaxWarps && row < p.tile_tokens * p.chunk_heads && row_token < cta_end && head < p.group;
     uint32_t row_slot = 0;
     uint32_t row_position = 0;
-    if (warp < kSoftmaxWarps) {
-        if (live) {
-            row_slot = p.request_slots[row_token];
-            row_position = p.position_ids[row_token];
-        }
+    if (inside) {
+        row_slot = p.request_slots[row_token];
+        row_position = p.position_ids[row_token];
     }
     const uint64_t first_wide = origin + (cta_begin - segment_begin);
     const uint64_t most_positions = p.block_table_stride * kPageSize;
@@ -307,8 +305,8 @@ e4m3_prompt_attention_kernel(const PromptParams p) {
     const VisiblePages pages(first_position, last_position, p.window, p.sinks);
     const uint32_t* __restrict__ table = p.block_tables + static_cast<uint64_t>(table_row) * p.block_table_stride;
     const uint32_t all_stages = (pages.count + kPagesPerStage - 1) / kPagesPerStage;
-    const uint32_t begin_stage = static_cast<uint32_t>(static_cast<uint64_t>(all_stages) * split / p.splits);
-    const uint32_t stages = static_cast<uint32_t>(static_cast<uint64_t>(all_stages) * (split + 1) / p.splits) - begin_stage;
+    const uint32_t begin_stage = all_stages * split / p.splits;               // less than 2^26 stages, at most 8 shares
+    const uint32_t stages = all_stages * (split + 1) / p.splits - begin_stage;
     // stages that a tile takes part in: the first one's tokens see less, the second one may have no tokens
     auto stages_of = [&](uint32_t tile) -> uint32_t {
         if (tile * p.tile_tokens > last_position - first_position) return 0;
@@ -348,7 +346,6 @@ e4m3_prompt_attention_kernel(const PromptParams p) {
     }
 
     const uint64_t row_wide = first_wide + (row_token - cta_begin);
-    live = live && row_wide < most_positions && row_slot == table_row && row_position == row_wide;
     float* own_words = row_words + tile * (L::kRowWords * kRows) + row;
     // All threads meet once the barriers, the tensor memory and the queries are there; each role first does what needs none of them.
     auto meet = [&]() -> uint32_t {
@@ -364,6 +361,7 @@ e4m3_prompt_attention_kernel(const PromptParams p) {
     float sum = 0.0f;
     bool poisoned = false;       // sees a NaN value
     bool lost = false;           // sees an unassigned page
+    bool live = false;           // has a result
     bool ok = true;
     bool valid = false;
     float weight[kSets];         // of each set's sums
@@ -614,7 +612,7 @@ e4m3_prompt_attention_kernel(const PromptParams p) {
     } else {
         // -------------------------------------------------------------------------------- softmax
         // ---- queries to f16, by a power of two per row ----
-        const uint64_t row_offset = live ? row_token * p.query_token_stride + static_cast<size_t>(kv_head * p.group + head) * DIM : 0;
+        const uint64_t row_offset = inside ? row_token * p.query_token_stride + static_cast<size_t>(kv_head * p.group + head) * DIM : 0;
         uint4 raw_query[kPasses];
 #pragma unroll
         for (uint32_t pass = 0; pass < kPasses; ++pass) {
@@ -624,23 +622,34 @@ e4m3_prompt_attention_kernel(const PromptParams p) {
             // rows that do not exist read the first query of the batch, and are cleared below
             raw_query[pass] = *reinterpret_cast<const uint4*>(p.query + ((static_cast<uint64_t>(high) << 32) | low) + lane % kLanes * 8);
         }
+        live = inside && row_wide < most_positions && row_slot == table_row && row_position == row_wide;
         const uint32_t live_rows = __ballot_sync(0xffffffffu, live);
+        uint32_t largest[kPasses];                        // exchanges of all passes side by side
 #pragma unroll
         for (uint32_t pass = 0; pass < kPasses; ++pass) {
             const uint32_t source = (set * kPasses + pass) * (32 / kLanes) + lane / kLanes;
-            const bool there = (live_rows >> source) & 1;
-            const uint32_t words[4] = {there ? raw_query[pass].x : 0, there ? raw_query[pass].y : 0, there ? raw_query[pass].z : 0,
-                                       there ? raw_query[pass].w : 0};
-            uint32_t largest = 0;
+            if (((live_rows >> source) & 1) == 0) raw_query[pass] = make_uint4(0, 0, 0, 0);
+            const uint32_t words[4] = {raw_query[pass].x, raw_query[pass].y, raw_query[pass].z, raw_query[pass].w};
+            largest[pass] = 0;
 #pragma unroll
             for (uint32_t i = 0; i < 4; ++i) {
                 const uint32_t low = words[i] & 0x7fffu;
                 const uint32_t high = (words[i] >> 16) & 0x7fffu;
-                largest = max(largest, max(low < 0x7f80u ? low : 0u, high < 0x7f80u ? high : 0u));
+                largest[pass] = max(largest[pass], max(low < 0x7f80u ? low : 0u, high < 0x7f80u ? high : 0u));
             }
+        }
 #pragma unroll
-            for (uint32_t delta = kLanes / 2; delta > 0; delta >>= 1) largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, delta));
-            const int32_t exponent = min(max(static_cast<int32_t>(largest >> 7) - 127 - 11, -126), 126);
+        for (uint32_t delta = kLanes / 2; delta > 0; delta >>= 1) {
+            uint32_t other[kPasses];
+#pragma unroll
+            for (uint32_t pass = 0; pass < kPasses; ++pass) other[pass] = __shfl_xor_sync(0xffffffffu, largest[pass], delta);
+#pragma unroll
+            for (uint32_t pass = 0; pass < kPasses; ++pass) largest[pass] = max(largest[pass], other[pass]);
+        }
+#pragma unroll
+        for (uint32_t pass = 0; pass < kPasses; ++pass) {
+            const uint32_t words[4] = {raw_query[pass].x, raw_query[pass].y, raw_query[pass].z, raw_query[pass].w};
+            const int32_t exponent = min(max(static_cast<int32_t>(largest[pass] >> 7) - 127 - 11, -126), 126);
             const float factor = power_of_two(-exponent);
             uint32_t half[4];
 #pragma unroll
@@ -648,16 +657,16 @@ e4m3_prompt_attention_kernel(const PromptParams p) {
                 const float2 pair = bf16x2_to_float2(words[i]);
                 half[i] = pack_f16x2(pair.x * factor, pair.y * factor);
             }
-            const uint32_t target = warp % 4 * 32 + source;             // row of the tile
+            const uint32_t target = warp % 4 * 32 + (set * kPasses + pass) * (32 / kLanes) + lane / kLanes;   // row of the tile
             const uint32_t piece = lane % kLanes;
-            if (piece == 0) row_words[(tile * L::kRowWords + 3) * kRows + target] = power_of_two(exponent) * p.scale_log2;
+            if (piece == 0) row_words[(tile * L::kRowWords + 2) * kRows + target] = power_of_two(exponent) * p.scale_log2;
             store_shared(base + L::kQ + (tile * L::kParts + piece / 8) * (kRows * 128) + target * 128 + (((piece % 8) ^ (target & 7)) << 4),
                          make_uint4(half[0], half[1], half[2], half[3]));
         }
         fence_proxy_async_smem();
         tmem = meet();
 
-        const float row_factor = own_words[3 * kRows];
+        const float row_factor = own_words[2 * kRows];
         const uint32_t position = live ? static_cast<uint32_t>(row_wide) : last_position;
         const uint32_t first_key = p.window != 0 && position >= p.window ? position - p.window + 1 : 0;
         const uint32_t lane_address = tmem + ((warp % 4 * 32) << 16);
@@ -835,18 +844,18 @@ e4m3_prompt_attention_kernel(const PromptParams p) {
         valid = ok && !lost && *abort == 0;
         // ---- the sets' results together ----
         if constexpr (kSets > 1) {
-            own_words[(4 + 3 * set) * kRows] = reference;
-            own_words[(5 + 3 * set) * kRows] = sum;
-            own_words[(6 + 3 * set) * kRows] = valid ? 1.0f : 0.0f;
+            own_words[(3 + 3 * set) * kRows] = reference;
+            own_words[(4 + 3 * set) * kRows] = sum;
+            own_words[(5 + 3 * set) * kRows] = valid ? 1.0f : 0.0f;
             asm volatile("barrier.sync 2, %0;" ::"n"(kSoftmaxWarps * 32) : "memory");
-            reference = fmaxf(own_words[4 * kRows], own_words[7 * kRows]);
-            valid = own_words[6 * kRows] != 0.0f && own_words[9 * kRows] != 0.0f;
+            reference = fmaxf(own_words[3 * kRows], own_words[6 * kRows]);
+            valid = own_words[5 * kRows] != 0.0f && own_words[8 * kRows] != 0.0f;
             const float offset = reference == -INFINITY ? 0.0f : reference;
             sum = 0.0f;
 #pragma unroll
             for (uint32_t i = 0; i < kSets; ++i) {
-                weight[i] = fast_exp2(own_words[(4 + 3 * i) * kRows] - offset);
-                sum = fmaf(own_words[(5 + 3 * i) * kRows], weight[i], sum);
+                weight[i] = fast_exp2(own_words[(3 + 3 * i) * kRows] - offset);
+                sum = fmaf(own_words[(4 + 3 * i) * kRows], weight[i], sum);
             }
         } else {
             weight[0] = 1.0f;
@@ -862,8 +871,7 @@ e4m3_prompt_attention_kernel(const PromptParams p) {
     if (warp < kSoftmaxWarps) {
         if (p.splits > 1) {
             own_words[0] = reference;
-            own_words[kRows] = sum;
-            own_words[2 * kRows] = valid ? 1.0f : 0.0f;
+            own_words[kRows] = valid ? sum : -1.0f;      // a sum is never negative
         }
         // each set has its share of the dimensions
         constexpr uint32_t kShare = DIM / kSets;
@@ -871,6 +879,7 @@ e4m3_prompt_attention_kernel(const PromptParams p) {
         const uint32_t columns = tmem + ((warp % 4 * 32) << 16) + kColumnO + tile * DIM;
         float* sums = reinterpret_cast<float*>(smem) + tile * (DIM * kRows) + row;
         const float inverse = 1.0f / sum;
+        const uint32_t staged = base + L::kQ + tile * (L::kParts * kRows * 128);      // the tile's queries are not needed any more
 #pragma unroll
         for (uint32_t c = set * kShare; c < (set + 1) * kShare; c += 16) {
             float value[16] = {};
@@ -887,13 +896,31 @@ e4m3_prompt_attention_kernel(const PromptParams p) {
             if (p.splits > 1) {
 #pragma unroll
                 for (uint32_t j = 0; j < 16; ++j) sums[(c + j) * kRows] = value[j];
-            } else if (live && valid) {
+            } else {
 #pragma unroll
                 for (uint32_t h = 0; h < 2; ++h) {
                     uint32_t pairs[4];
 #pragma unroll
                     for (uint32_t j = 0; j < 4; ++j) pairs[j] = pack_bf16x2(value[h * 8 + 2 * j] * inverse, value[h * 8 + 2 * j + 1] * inverse);
-                    *reinterpret_cast<uint4*>(p.output + out_row + c + h * 8) = make_uint4(pairs[0], pairs[1], pairs[2], pairs[3]);
+                    store_shared(staged + row * (DIM * 2) + (((c / 8 + h) ^ (row & 7)) << 4), make_uint4(pairs[0], pairs[1], pairs[2], pairs[3]));
+                }
+            }
+        }
+        if (p.splits == 1) {
+            // rows of this warp, by whole lines (one row a lane is 32 lines a store; 7 portions at heads of 128: 26.0 us instead of 24.7)
+            constexpr uint32_t kPieces = kShare / 8;     // of a row's share
+            __syncwarp();
+            const uint32_t written = __ballot_sync(0xffffffffu, live && valid);
+#pragma unroll
+            for (uint32_t pass = 0; pass < kPieces; ++pass) {
+                const uint32_t source = pass * (32 / kPieces) + lane / kPieces;
+                const uint32_t piece = set * kPieces + lane % kPieces;
+                const uint32_t low = __shfl_sync(0xffffffffu, static_cast<uint32_t>(out_row), source);
+                const uint32_t high = __shfl_sync(0xffffffffu, static_cast<uint32_t>(static_cast<uint64_t>(out_row) >> 32), source);
+                const uint32_t target = warp % 4 * 32 + source;
+                const uint4 out = load_shared(staged + target * (DIM * 2) + ((piece ^ (target & 7)) << 4));
+                if ((written >> source) & 1) {
+                    *reinterpret_cast<uint4*>(p.output + ((static_cast<uint64_t>(high) << 32) | low) + piece * 8) = out;
                 }
             }
         }
@@ -914,8 +941,7 @@ e4m3_prompt_attention_kernel(const PromptParams p) {
             for (uint32_t r = 0; r < 8; ++r) {         // all loads under way at once
                 weight[r] = r < p.splits ? load_cluster(own, r) : -INFINITY;
                 part_sum[r] = r < p.splits ? load_cluster(own + kRows * 4, r) : 0.0f;
-                const float holds = r < p.splits ? load_cluster(own + 2 * kRows * 4, r) : 1.0f;
-                complete = complete & (holds != 0.0f);
+                complete = complete & !(part_sum[r] < 0.0f);
                 most = fmaxf(most, weight[r]);
             }
             const float offset = most == -INFINITY ? 0.0f : most;
