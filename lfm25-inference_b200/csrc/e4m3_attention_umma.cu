@@ -20,7 +20,7 @@
 // cycle and SM) need 60.  What bounds it is the chain of a stage through its roles, 1900 cycles: no unit is busy for much more than
 // half of that, page warps as long as softmax warps, and 11,000 cycles go to the ends of a CTA.  One set of softmax warps takes 156 us (166
 // with codes in registers one stage ahead); without its exponentials the kernel takes 139, without conversions 146, without both 133.
-// Eight page warps leave 72 registers a thread: 151 us.
+// Eight page warps leave 72 registers a thread: 146 us.
 //
 // Rows of a mask edge test bits of their own; a NaN among the values is replaced in the operand (a weight of 0 times NaN is
 // NaN) and remembered by key: a row that sees it becomes NaN as a whole.  Few tiles: a cluster shares a tile's keys and joins
