@@ -594,7 +594,8 @@ cudaError_t launch_shape(cudaStream_t stream, const DecodeParams& params, uint64
 // has 8 pages or more: a cluster costs about as much as 6 pages of one warp (23 padded to 32 tokens through a window of 4096, 2 KV heads of
 // 128: 4 CTAs 18.1, 8 CTAs 14.9, 16 CTAs 24.8 us; 3 tokens at 20480..65536: 4 CTAs 69, 8 CTAs 47, 16 CTAs 36.9 us; 32 tokens at 64..400:
 // 1 CTA 6.5, 2 CTAs 7.5 us).  Where that leaves half of the warps' places free, CTAs of 8 warps (1 token at 8000: 8.2 against 8.9 us;
-// 32 tokens at 64..400: 5.8 against 6.5 us), in clusters of 8 at most, which gain as much as 16.
+// 32 tokens at 64..400: 5.8 against 6.5 us).  8 of those rather than 16 CTAs up to 48 pages a warp (4 tokens at 8000..16000: 16.7 us
+// against 19.8 with 16 of 4 warps; 2 at 30000: 23.2 against 25.2 with 16 of 8), beyond that 16 (1 at 65536: 24.6 against 30.7 us).
 template <uint32_t DIM, uint32_t HEADS>
 cudaError_t launch_heads(cudaStream_t stream, DecodeParams params, uint64_t items, uint64_t pages) {
     using S = Shape<DIM, HEADS, 4>;
@@ -604,8 +605,9 @@ cudaError_t launch_heads(cudaStream_t stream, DecodeParams params, uint64_t item
            pages >= (8ull * 4 << params.splits_log2)) {
         ++params.splits_log2;
     }
-    const bool wide = (items << params.splits_log2) * 8 <= kSms * S::kWarpsPerSm;
-    if (wide && params.splits_log2 == 4) params.splits_log2 = 3;
+    auto wide_fits = [&](uint32_t splits_log2) { return (items << splits_log2) * 8 <= kSms * S::kWarpsPerSm; };
+    if (params.splits_log2 == 4 && wide_fits(3) && pages < 48 * 8 * 8) params.splits_log2 = 3;
+    const bool wide = wide_fits(params.splits_log2);
     params.splits = 1u << params.splits_log2;
     const uint64_t blocks = items << params.splits_log2;
     if (blocks > 0x7fffffffu) {
