@@ -247,6 +247,40 @@ def test_prompt_attention(device, heads, kv_heads, dim, segments, window, sinks)
     check_attention(out, query, cache, tables, nobody, positions, BF16_WEIGHTS, before, window=window, sinks=sinks)
 
 
+@pytest.mark.parametrize("heads,kv_heads,dim", [(32, 8, 64), (32, 8, 128)])
+def test_prompt_attention_of_more_tiles_than_run_at_once(device, heads, kv_heads, dim):
+    """Six portions, 240 CTAs; every 41st token is compared, twice: behind other kernels and behind the call itself."""
+    rng = np.random.default_rng(dim)
+    segments = ((0, 300), (17, 301), (400, 290), (800, 257), (64, 320), (1200, 300))
+    contexts = [prefix + count for prefix, count in segments]
+    pool = pool_of(contexts)
+    arena, *cache = random_cache(rng, pool, kv_heads, dim, device)
+    tables = tables_of(rng, contexts, pool)
+    rows = np.concatenate([np.full(count, row) for row, (_, count) in enumerate(segments)])
+    positions = np.concatenate([np.arange(prefix, prefix + count) for prefix, count in segments])
+    query = bf16(rng.standard_normal((len(rows), heads, dim)) * 0.5, device)
+    arguments = [to_u32(values, device) for values in (tables, rows, positions, np.concatenate(([0], np.cumsum([c for _, c in segments]))))]
+    some = np.arange(5, len(rows), 41)
+    outs = [torch.zeros_like(query) for _ in range(3)]
+    for out in outs:
+        ops.paged_prompt_attention_e4m3_into(query, arena, *arguments, out)
+    check_attention(outs[0][some], query[some], cache, tables, rows[some], positions[some], BF16_WEIGHTS, outs[0][some])
+    assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
+
+
+@pytest.mark.parametrize("contexts", [(60001,), (9000, 16500, 12345, 8191)])
+def test_decode_attention_of_few_long_contexts(device, contexts):
+    rng = np.random.default_rng(len(contexts))
+    pool = pool_of(contexts)
+    arena, *cache = random_cache(rng, pool, 8, 64, device)
+    tables = tables_of(rng, contexts, pool)
+    rows, positions = np.arange(len(contexts)), np.array(contexts) - 1
+    query = bf16(rng.standard_normal((len(rows), 32, 64)) * 0.5, device)
+    out = torch.zeros_like(query)
+    ops.paged_attention_e4m3_into(query, arena, to_u32(tables, device), to_u32(rows, device), to_u32(positions, device), out)
+    check_attention(out, query, cache, tables, rows, positions, F16_WEIGHTS, out)
+
+
 def attention_call(kind, query, arena, tables, rows, positions, out, **rule):
     if kind == "decode":
         ops.paged_attention_e4m3_into(query, arena, tables, rows, positions, out, **rule)
