@@ -23,8 +23,6 @@ namespace lfm25 {
 
 namespace {
 
-constexpr uint32_t kWarps = 8;
-constexpr uint32_t kThreads = kWarps * 32;
 constexpr uint32_t kAhead = 4;                           // query rows that a lane loads ahead
 constexpr uint32_t kSpanMost = 16;                       // tokens of a CTA that looks for runs
 constexpr uint32_t kRowsMost = kSpanMost + kPageSize - 1;   // with the rest of the last run
@@ -100,9 +98,9 @@ __device__ __forceinline__ uint32_t four_codes(const float (&x)[4], float factor
 }
 
 // (cos, sin) of position * inv_freq for `rows` tokens from `first` on
-template <uint32_t DIM>
+template <uint32_t DIM, uint32_t kWarps>
 __device__ __forceinline__ void angles(const WriteParams& p, uint32_t first, uint32_t rows, float2* turns) {
-    for (uint32_t index = threadIdx.x; index < rows * (DIM / 2); index += kThreads) {
+    for (uint32_t index = threadIdx.x; index < rows * (DIM / 2); index += kWarps * 32) {
         const double angle = static_cast<double>(p.position_ids[first + index / (DIM / 2)]) * static_cast<double>(p.inv_freq[index % (DIM / 2)]);
         const double turn = rint(angle * 0.15915494309189535);
         float sine, cosine;
@@ -112,7 +110,7 @@ __device__ __forceinline__ void angles(const WriteParams& p, uint32_t first, uin
 }
 
 // All queries of `query_span` tokens
-template <uint32_t DIM>
+template <uint32_t DIM, uint32_t kWarps>
 __device__ __forceinline__ void write_queries(const WriteParams& p, float2* turns) {
     constexpr uint32_t LANES = DIM / 8;
     constexpr uint32_t ROWS = 32 / LANES;
@@ -137,7 +135,7 @@ __device__ __forceinline__ void write_queries(const WriteParams& p, float2* turn
     };
     load(warp * ROWS);
     const Values weight = unpack(load_values<DIM>(p.query_norm, piece));
-    angles<DIM>(p, begin, tokens, turns);
+    angles<DIM, kWarps>(p, begin, tokens, turns);
     __syncthreads();
     for (uint32_t first = warp * ROWS; first < rows; first += kAhead * kWarps * ROWS) {
 #pragma unroll
@@ -158,8 +156,8 @@ __device__ __forceinline__ void write_queries(const WriteParams& p, float2* turn
     }
 }
 
-template <uint32_t DIM, bool NORM_ROPE>
-__global__ void __launch_bounds__(kThreads, DIM == 64 ? 3 : 2)
+template <uint32_t DIM, bool NORM_ROPE, uint32_t kWarps>
+__global__ void __launch_bounds__(kWarps * 32, (DIM == 64 ? 24 : 16) / kWarps)
 e4m3_cache_write_kernel(const WriteParams p) {
     constexpr uint32_t LANES = DIM / 8;            // lanes of a row
     constexpr uint32_t ROWS = 32 / LANES;          // rows of a pass
@@ -173,7 +171,7 @@ e4m3_cache_write_kernel(const WriteParams p) {
     pdl_wait();
     if constexpr (NORM_ROPE) {
         if (blockIdx.x < p.query_blocks) {
-            write_queries<DIM>(p, turns);
+            write_queries<DIM, kWarps>(p, turns);
             return;
         }
     }
@@ -234,7 +232,7 @@ e4m3_cache_write_kernel(const WriteParams p) {
     if (NORM_ROPE && !is_value) {
         weight = unpack(load_values<DIM>(p.key_norm, piece));
         const uint32_t last = 31 - __clz(leaders);
-        angles<DIM>(p, begin, last - 1 + run_length(last), turns);
+        angles<DIM, kWarps>(p, begin, last - 1 + run_length(last), turns);
         __syncthreads();
     }
     for (uint32_t unit = warp; unit < units; unit += kWarps) {
@@ -295,10 +293,15 @@ e4m3_cache_write_kernel(const WriteParams p) {
     }
 }
 
+template <uint32_t DIM, uint32_t kWarps>
+cudaError_t launch_warps(cudaStream_t stream, const WriteParams& params, unsigned int blocks) {
+    return params.query != nullptr ? launch_kernel(e4m3_cache_write_kernel<DIM, true, kWarps>, blocks, kWarps * 32, 0, stream, 1, params)
+                                   : launch_kernel(e4m3_cache_write_kernel<DIM, false, kWarps>, blocks, kWarps * 32, 0, stream, 1, params);
+}
+
 template <uint32_t DIM>
-cudaError_t launch_dim(cudaStream_t stream, const WriteParams& params, unsigned int blocks) {
-    return params.query != nullptr ? launch_kernel(e4m3_cache_write_kernel<DIM, true>, blocks, kThreads, 0, stream, 1, params)
-                                   : launch_kernel(e4m3_cache_write_kernel<DIM, false>, blocks, kThreads, 0, stream, 1, params);
+cudaError_t launch_dim(cudaStream_t stream, const WriteParams& params, uint32_t warps, unsigned int blocks) {
+    return warps == 4 ? launch_warps<DIM, 4>(stream, params, blocks) : launch_warps<DIM, 8>(stream, params, blocks);
 }
 
 }  // namespace
@@ -320,6 +323,10 @@ cudaError_t launch_e4m3_cache_write(cudaStream_t stream, const E4m3WriteLaunch& 
     params.num_tokens = static_cast<uint32_t>(launch.num_tokens);
     params.query_heads = launch.query_heads;
     params.eps = launch.eps;
+    // A CTA of a prompt has one run or two, and a unit for each KV head of them: with fewer than 8 heads, 4 warps (8 prompts of 437 to 512
+    // with norms, 4 against 8 warps: 2 heads of 128 11.5 and 12.8 us, 4 of 128 26.2 and 28.1, 8 of 64 17.9 and 15.8; without norms
+    // 4.6 and 6.1, 5.1 and 6.6, 6.0 and 5.5).
+    const uint32_t warps = launch.cache.kv_heads < 8 ? 4 : 8;
     // Tokens of a CTA that looks for runs: as many as leave 2 CTAs an SM with keys and 2 with values.  A decode step's tokens
     // then run side by side, and the tokens of a long prompt share the search (3800 tokens: 8 to a CTA 16.0 us, 4 to a CTA 17.3 us;
     // 700 tokens: 2 to a CTA 8.3 us, 1 to a CTA 9.3 us).
@@ -329,7 +336,7 @@ cudaError_t launch_e4m3_cache_write(cudaStream_t stream, const E4m3WriteLaunch& 
     size_t query_blocks = 0;
     if (params.query != nullptr) {
         // as many tokens as a CTA's lanes load at once
-        const uint32_t rows = kAhead * kWarps * (256 / launch.cache.head_dim);
+        const uint32_t rows = kAhead * warps * (256 / launch.cache.head_dim);
         params.query_span = rows / params.query_heads < 1 ? 1 : rows / params.query_heads;
         if (params.query_span > kSpanMost) params.query_span = kSpanMost;
         query_blocks = (launch.num_tokens + params.query_span - 1) / params.query_span;
@@ -340,7 +347,7 @@ cudaError_t launch_e4m3_cache_write(cudaStream_t stream, const E4m3WriteLaunch& 
     params.query_blocks = static_cast<uint32_t>(query_blocks);
     params.run_blocks = static_cast<uint32_t>(run_blocks);
     const unsigned int blocks = static_cast<unsigned int>(2 * run_blocks + query_blocks);
-    return launch.cache.head_dim == 64 ? launch_dim<64>(stream, params, blocks) : launch_dim<128>(stream, params, blocks);
+    return launch.cache.head_dim == 64 ? launch_dim<64>(stream, params, warps, blocks) : launch_dim<128>(stream, params, warps, blocks);
 }
 
 }  // namespace lfm25
