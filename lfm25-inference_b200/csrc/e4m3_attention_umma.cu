@@ -743,31 +743,31 @@ e4m3_prompt_attention_kernel(const PromptParams p) {
                 constexpr bool kMasked = decltype(masked)::value;
                 uint32_t bits[2] = {0, 0};
                 if constexpr (kMasked) seen_keys(bits);
-                // 32 keys at a time, the first ones twice: all scores at once leave no registers for this many warps
-                uint32_t raw[2][16];
-                auto fetch = [&](uint32_t half) {
-                    load_columns(columns + half * 32, raw[0], raw[1]);
-                };
+                // Two sets leave no registers for all scores at once: 32 keys at a time, the first ones twice.
+                constexpr bool kWhole = kSets == 1;
+                uint32_t raw[kWhole ? 4 : 2][16];
+                auto fetch = [&](uint32_t half) { load_columns(columns + half * 32, raw[kWhole ? half * 2 : 0], raw[kWhole ? half * 2 + 1 : 1]); };
                 // ---- maximum ----
                 float most = -INFINITY;
 #pragma unroll
                 for (uint32_t half = 0; half < 2; ++half) {
                     fetch(half);
+                    const uint32_t at = kWhole ? half * 2 : 0;
                     if constexpr (kMasked) {
                         // masked scores, whatever they are, become -inf (the factor is positive or 0, so not by the product)
 #pragma unroll
                         for (uint32_t j = 0; j < 32; ++j) {
-                            if (((bits[half] >> j) & 1) == 0) raw[j / 16][j % 16] = 0xff800000u;
+                            if (((bits[half] >> j) & 1) == 0) raw[at + j / 16][j % 16] = 0xff800000u;
                         }
                     }
 #pragma unroll
                     for (uint32_t sub = 0; sub < 2; ++sub) {
-                        float a = __uint_as_float(raw[sub][0]);
-                        float b = __uint_as_float(raw[sub][1]);
+                        float a = __uint_as_float(raw[at + sub][0]);
+                        float b = __uint_as_float(raw[at + sub][1]);
 #pragma unroll
                         for (uint32_t j = 2; j < 16; j += 4) {
-                            a = max3(a, __uint_as_float(raw[sub][j]), __uint_as_float(raw[sub][j + 1]));
-                            if (j + 2 < 16) b = max3(b, __uint_as_float(raw[sub][j + 2]), __uint_as_float(raw[sub][j + 3]));
+                            a = max3(a, __uint_as_float(raw[at + sub][j]), __uint_as_float(raw[at + sub][j + 1]));
+                            if (j + 2 < 16) b = max3(b, __uint_as_float(raw[at + sub][j + 2]), __uint_as_float(raw[at + sub][j + 3]));
                         }
                         const float here = fmaxf(a, b);
                         most = fmaxf(most, here * factor[half * 2 + sub]);
@@ -802,7 +802,8 @@ e4m3_prompt_attention_kernel(const PromptParams p) {
 #pragma unroll
                 for (uint32_t turn = 0; turn < 2; ++turn) {
                     const uint32_t half = 1 - turn;
-                    if (turn == 1) fetch(half);
+                    if (!kWhole && turn == 1) fetch(half);
+                    const uint32_t at = kWhole ? half * 2 : 0;
                     uint32_t packed[16];
 #pragma unroll
                     for (uint32_t sub = 0; sub < 2; ++sub) {
@@ -810,7 +811,7 @@ e4m3_prompt_attention_kernel(const PromptParams p) {
 #pragma unroll
                         for (uint32_t pair = 0; pair < 8; ++pair) {
                             const uint32_t j = sub * 16 + pair * 2;
-                            float2 w = pair_out(pair_fma(pair_of(__uint_as_float(raw[sub][pair * 2]), __uint_as_float(raw[sub][pair * 2 + 1])),
+                            float2 w = pair_out(pair_fma(pair_of(__uint_as_float(raw[at + sub][pair * 2]), __uint_as_float(raw[at + sub][pair * 2 + 1])),
                                                          multiplier, offset));
                             w = make_float2(fast_exp2(w.x), fast_exp2(w.y));
                             if constexpr (kMasked) {
