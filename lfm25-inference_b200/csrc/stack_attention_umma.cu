@@ -19,6 +19,7 @@
 
 #include "common.cuh"
 #include "launch.h"
+#include "ring.h"
 #include "stack_attention.h"
 #include "stack_common.cuh"
 #include "stack_latent.h"
@@ -329,7 +330,7 @@ stack_attention_umma_kernel(const __grid_constant__ CUtensorMap query_map, const
                     }
                 }
                 umma_commit(bar_pv + 8 * buffer);
-                umma_commit(bar_empty + 8 * stage);
+                if (filled_again(index, stages_total, L::kStages)) umma_commit(bar_empty + 8 * stage);
             }
             if (!ok && !flags[1]) {
                 flags[1] = 1;

@@ -1,0 +1,58 @@
+"""Arrivals on the barriers that free a ring's buffers: the tensor core makes them (tcgen05.commit) whenever it gets there, and one
+that nobody waits for may come when its CTA has ended.  Shown without a GPU: that a late arrival would fault one."""
+import os
+import re
+import shutil
+import subprocess
+
+import pytest
+
+CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "lfm25-inference_b200", "csrc")
+
+PROGRAM = r"""
+#include <cstdio>
+#include <vector>
+#include "ring.h"
+
+// The producer of a ring waits for a buffer's arrival before it fills it again; the consumer arrives where `filled_again`
+// says so.  Every arrival is waited for, and every wait has its arrival.
+int main() {
+    for (unsigned buffers = 1; buffers < 9; ++buffers) {
+        for (unsigned items = 0; items < 40; ++items) {
+            std::vector<unsigned> arrivals(buffers, 0), waits(buffers, 0);
+            for (unsigned index = 0; index < items; ++index) {
+                if (index >= buffers) ++waits[index % buffers];
+                if (lfm25::filled_again(index, items, buffers)) ++arrivals[index % buffers];
+            }
+            if (arrivals != waits) {
+                std::printf("%u items in %u buffers\n", items, buffers);
+                return 1;
+            }
+        }
+    }
+    std::puts("ok");
+    return lfm25::filled_again(0xfffffff0u, 0xffffffffu, 15) ? 1 : 0;   // no sum that wraps
+}
+"""
+
+
+def test_a_buffer_is_reported_free_as_often_as_it_is_filled_again(tmp_path):
+    if shutil.which("g++") is None:
+        pytest.skip("no g++")
+    source = tmp_path / "ring.cpp"
+    source.write_text(PROGRAM)
+    binary = tmp_path / "ring"
+    compiled = subprocess.run(["g++", "-std=c++17", "-Wall", "-Wextra", "-Werror", "-I", CSRC, str(source), "-o", str(binary)],
+                              capture_output=True, text=True)
+    assert compiled.returncode == 0, compiled.stderr
+    ran = subprocess.run([str(binary)], capture_output=True, text=True, timeout=60)
+    assert ran.returncode == 0 and ran.stdout.strip() == "ok", ran.stdout
+
+
+# The kernels whose last work is waited for by other barriers than those of the ring.  (The GEMM kernels commit to a barrier of
+# their accumulator behind all others, and that one is waited for.)
+@pytest.mark.parametrize("name", ["stack_attention_umma.cu"])
+def test_kernels_ask_for_arrivals_that_are_waited_for(name):
+    with open(os.path.join(CSRC, name)) as handle:
+        commits = [line.strip() for line in handle if re.search(r"umma_commit\(bar_empty", line)]
+    assert commits and all(line.startswith("if (filled_again(") for line in commits), commits
