@@ -26,6 +26,7 @@
 #include "common.cuh"
 #include "kernels.h"
 #include "launch.h"
+#include "ring.h"
 #include "tcgen05.cuh"
 #include "tensor_map.h"
 
@@ -314,7 +315,7 @@ hybrid_attention_umma_kernel(const __grid_constant__ CUtensorMap query_map, cons
                                  v_desc + step * (kPageBytes >> 4), idesc_pv, step);
                 }
                 umma_commit(bar_pv + 8 * buffer);
-                umma_commit(bar_empty + 8 * stage);
+                if (filled_again(macro, macro_tiles, kUmmaStages)) umma_commit(bar_empty + 8 * stage);
             }
             if (!ok && !flags[1]) {
                 flags[1] = 1;
