@@ -23,6 +23,7 @@
 
 #include "launch.h"
 #include "options.h"
+#include "ring.h"
 #include "stack_latent.h"
 #include "tcgen05.cuh"
 #include "tensor_map.h"
@@ -405,7 +406,7 @@ latent_attention_umma_kernel(const __grid_constant__ CUtensorMap absorbed_map,
                         v_desc += 2 * group_bytes >> 4;
                     }
                     umma_commit(bar_product + 8 * buffer);
-                    umma_commit(bar_empty + 8 * stage);
+                    if (filled_again(index, count, p.stages)) umma_commit(bar_empty + 8 * stage);
                 }
                 __syncwarp();
                 if (index + 1 < count && !ahead) {
