@@ -32,6 +32,7 @@
 #include "e4m3_cache.h"
 #include "e4m3_visible.cuh"
 #include "launch.h"
+#include "ring.h"
 #include "tcgen05.cuh"
 
 namespace lfm25 {
@@ -97,6 +98,7 @@ struct Layout {
     static constexpr uint32_t kBytes = kControl + 512 + kRowWords * kTiles * kRows * 4;
     static constexpr uint32_t kAlloc = kBytes + 1024;
     static_assert(kColumnO + kTiles * kSets * DIM <= kTmemColumns, "tensor memory has 512 columns");
+    static_assert(kSets <= 2, "a set's stages are all even or all odd");
     static_assert(kControl >= kTiles * kRows * DIM * 4, "the sums that a cluster joins lie where the operands were");
 };
 
@@ -106,7 +108,10 @@ struct Control {
     uint64_t empty[kBuffersMost];          // both tiles' P V are done with them
     uint64_t scores[kTiles][2];
     uint64_t weights[kTiles][2];
-    uint64_t product[kTiles][2];       // P V of an even / odd stage is complete: one barrier could be two phases behind
+    // P V of an even / odd stage is complete.  Nothing orders the arrivals of two commits on different barriers, so each phase of
+    // these is waited for.  With two sets the scores of a set's next stage, issued behind P V of the one before, say as much, and
+    // only each set's last stage is reported.
+    uint64_t product[kTiles][2];
     uint64_t drained[kTiles];          // after a wait ran out: no MMA is in flight any more
     alignas(16) float key_scales[kBuffersMost][kPagesPerStage];   // read four at a time
     alignas(16) unsigned long long nan_keys[kBuffersMost][kPageWarps];   // of each page warp: keys with a NaN among their values
@@ -584,10 +589,8 @@ e4m3_prompt_attention_kernel(const PromptParams p) {
                                 v_desc + part * (kTile >> 4) + step * (2048 >> 4), idesc_product, stage >= kSets || step > 0);
                     }
                 }
-                umma_commit(my_product + 8 * parity);
-                // Only where the buffer is filled once more: an arrival that nobody waits for may come when the CTA has gone, and
-                // its shared memory with it.
-                if (stage + kBuffers < stages) umma_commit(bar_empty + 8 * buffer);
+                if (kSets == 1 || last_of_set(stage, my_stages, kSets)) umma_commit(my_product + 8 * parity);
+                if (filled_again(stage, stages, kBuffers)) umma_commit(bar_empty + 8 * buffer);
             }
             __syncwarp();
             // Behind it the scores of two stages on: MMAs execute in order, so the weights in their columns have been consumed.
@@ -595,7 +598,7 @@ e4m3_prompt_attention_kernel(const PromptParams p) {
             if (++buffer == kBuffers) buffer = 0;
         }
         // stages that only the other tile takes part in
-        for (uint32_t stage = my_stages; stage + kBuffers < stages && ok; ++stage) {
+        for (uint32_t stage = my_stages; stage < stages && filled_again(stage, stages, kBuffers) && ok; ++stage) {
             ok = wait_for(bar_full + 8 * (stage % kBuffers), (stage / kBuffers) & 1);
             if (ok && lane == 0) mbar_arrive(bar_empty + 8 * (stage % kBuffers));
             __syncwarp();
@@ -731,6 +734,9 @@ e4m3_prompt_attention_kernel(const PromptParams p) {
                 buffer_parity ^= 1;
             }
             ok = ok && mbar_wait_bounded(bar_scores + 8 * (2 * tile + (stage & 1)), (stage >> 1) & 1, p.wait_limit_ns);
+            if (kSets == 1 && stage >= 2) {
+                ok = ok && mbar_wait_bounded(bar_product + 8 * (2 * tile + (stage & 1)), ((stage >> 1) - 1) & 1, p.wait_limit_ns);
+            }
             if (!__all_sync(0xffffffffu, ok)) {
                 ok = false;
                 break;
@@ -779,12 +785,14 @@ e4m3_prompt_attention_kernel(const PromptParams p) {
                     if (raise) reference = most;
                     sum *= shrink;
                     if (stage >= kSets) {
-                        const uint32_t before = stage - kSets;
-                        ok = *abort == 0 && mbar_wait_bounded(bar_product + 8 * (2 * tile + (before & 1)), (before >> 1) & 1, p.wait_limit_ns);
-                        if (!__all_sync(0xffffffffu, ok)) {
-                            return false;
+                        if constexpr (kSets == 1) {
+                            const uint32_t before = stage - 1;
+                            ok = *abort == 0 && mbar_wait_bounded(bar_product + 8 * (2 * tile + (before & 1)), (before >> 1) & 1, p.wait_limit_ns);
+                            if (!__all_sync(0xffffffffu, ok)) {
+                                return false;
+                            }
+                            tcgen05_fence_after();
                         }
-                        tcgen05_fence_after();
 #pragma unroll 1
                         for (uint32_t c = 0; c < DIM; c += 16) {
                             uint32_t o[16];
@@ -833,8 +841,17 @@ e4m3_prompt_attention_kernel(const PromptParams p) {
             hand_over(stage);
         }
         if (ok && my_stages > set) {
-            const uint32_t last = my_stages - 1 - (my_stages - 1 - set) % kSets;      // of this set
-            ok = *abort == 0 && mbar_wait_bounded(bar_product + 8 * (2 * tile + (last & 1)), (last >> 1) & 1, p.wait_limit_ns);
+            ok = *abort == 0;
+            if constexpr (kSets == 1) {
+                if (my_stages > 1) {
+                    const uint32_t before = my_stages - 2;
+                    ok = ok && mbar_wait_bounded(bar_product + 8 * (2 * tile + (before & 1)), (before >> 1) & 1, p.wait_limit_ns);
+                }
+                const uint32_t last = my_stages - 1;
+                ok = ok && mbar_wait_bounded(bar_product + 8 * (2 * tile + (last & 1)), (last >> 1) & 1, p.wait_limit_ns);
+            } else {
+                ok = ok && mbar_wait_bounded(bar_product + 8 * (2 * tile + set), 0, p.wait_limit_ns);   // a set's stages have its parity
+            }
             ok = __all_sync(0xffffffffu, ok);
         }
         if (!ok && lane == 0 && *abort == 0) {

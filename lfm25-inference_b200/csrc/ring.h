@@ -16,4 +16,7 @@ namespace lfm25 {
 // after its CTA has ended and its shared memory is gone, so it is not asked for.
 LFM25_RING_FUNCTION bool filled_again(uint32_t index, uint32_t items, uint32_t buffers) { return items - index > buffers; }
 
+// Whether item `index` of `items` is the last that its set takes, where `sets` take items by turns.
+LFM25_RING_FUNCTION bool last_of_set(uint32_t index, uint32_t items, uint32_t sets) { return items - index <= sets; }
+
 }  // namespace lfm25

@@ -30,6 +30,20 @@ int main() {
             }
         }
     }
+    // sets that take items by turns wait once each, for their last item
+    for (unsigned sets = 1; sets < 4; ++sets) {
+        for (unsigned items = 0; items < 40; ++items) {
+            std::vector<unsigned> reports(sets, 0), waits(sets, 0);
+            for (unsigned index = 0; index < items; ++index) {
+                if (lfm25::last_of_set(index, items, sets)) ++reports[index % sets];
+            }
+            for (unsigned set = 0; set < sets; ++set) waits[set] = items > set ? 1 : 0;
+            if (reports != waits) {
+                std::printf("%u items, %u sets\n", items, sets);
+                return 1;
+            }
+        }
+    }
     std::puts("ok");
     return lfm25::filled_again(0xfffffff0u, 0xffffffffu, 15) ? 1 : 0;   // no sum that wraps
 }
@@ -51,8 +65,19 @@ def test_a_buffer_is_reported_free_as_often_as_it_is_filled_again(tmp_path):
 
 # The kernels whose last work is waited for by other barriers than those of the ring.  (The GEMM kernels commit to a barrier of
 # their accumulator behind all others, and that one is waited for.)
-@pytest.mark.parametrize("name", ["stack_attention_umma.cu", "hybrid_attention_umma.cu", "stack_latent_decode.cu"])
+@pytest.mark.parametrize("name", ["stack_attention_umma.cu", "hybrid_attention_umma.cu", "stack_latent_decode.cu", "e4m3_attention_umma.cu"])
 def test_kernels_ask_for_arrivals_that_are_waited_for(name):
     with open(os.path.join(CSRC, name)) as handle:
         commits = [line.strip() for line in handle if re.search(r"umma_commit\(bar_empty", line)]
     assert commits and all(line.startswith("if (filled_again(") for line in commits), commits
+
+
+def test_every_product_of_the_prompt_attention_is_waited_for():
+    """One set of softmax warps waits for every stage's product in turn; of two sets each waits for its last stage's, and no other
+    is reported."""
+    with open(os.path.join(CSRC, "e4m3_attention_umma.cu")) as handle:
+        source = handle.read()
+    commits = re.findall(r"^ *(.*umma_commit\(my_product.*)$", source, re.M)
+    assert commits == ["if (kSets == 1 || last_of_set(stage, my_stages, kSets)) umma_commit(my_product + 8 * parity);"]
+    loop = source[source.index("for (uint32_t stage = set; stage < my_stages; stage += kSets)"):]
+    assert re.search(r"if \(kSets == 1 && stage >= 2\) \{\s*ok = ok && mbar_wait_bounded\(bar_product", loop)
