@@ -549,7 +549,9 @@ latent_attention_umma_kernel(const __grid_constant__ CUtensorMap absorbed_map,
             if (lane == 0) mbar_arrive(bar_weights + 8 * buffer);
         }
         if (count > 0) {
+            // both barriers: nothing orders the arrivals of two commits on different ones, and nobody leaves before they came
             const uint32_t last = count - 1;
+            if (last > 0) ok = ok && mbar_wait_bounded(bar_product + 8 * ((last - 1) & 1), ((last - 1) >> 1) & 1, p.wait_limit);
             ok = ok && mbar_wait_bounded(bar_product + 8 * (last & 1), (last >> 1) & 1, p.wait_limit);
             if (!__all_sync(0xffffffffu, ok)) {
                 if (lane == 0) fail(3);

@@ -81,3 +81,13 @@ def test_every_product_of_the_prompt_attention_is_waited_for():
     assert commits == ["if (kSets == 1 || last_of_set(stage, my_stages, kSets)) umma_commit(my_product + 8 * parity);"]
     loop = source[source.index("for (uint32_t stage = set; stage < my_stages; stage += kSets)"):]
     assert re.search(r"if \(kSets == 1 && stage >= 2\) \{\s*ok = ok && mbar_wait_bounded\(bar_product", loop)
+
+
+def test_every_product_of_the_latent_decode_attention_is_waited_for():
+    """Stage `index` waits for the product of index - 2, and the end for the last two."""
+    with open(os.path.join(CSRC, "stack_latent_decode.cu")) as handle:
+        source = handle.read()
+    assert len(re.findall(r"umma_commit\(bar_product", source)) == 1
+    assert re.search(r"if \(index >= 2\) \{\s*ok = mbar_wait_bounded\(bar_product \+ 8 \* buffer", source)
+    end = source[source.index("const uint32_t last = count - 1;"):]
+    assert re.search(r"bar_product \+ 8 \* \(\(last - 1\) & 1\)", end) and re.search(r"bar_product \+ 8 \* \(last & 1\)", end)
