@@ -19,8 +19,11 @@
 // lost lies 2^-36 below the largest element.  Page scales multiply S in front of the exponential and the page's P V behind the
 // MMA, both in f32, where a power of two rounds nothing.
 //
-// The maximum that weights refer to is only raised when a score exceeds it by more than 8 (weights are then at most 2^8,
-// which f16 holds): most pages need no exchange between lanes.
+// The maximum that weights refer to is only raised when a score exceeds it by more than 4 (log2): most pages need no exchange between
+// lanes.  Weights go to the product in f16, rounded to 11 bits: times 2^11, which the sum of weights has as well, so that the largest
+// there can be, 2^15, still fits and the smallest step is 2^-35 of the weight of the maximum.  (Without that factor and with a
+// headroom of 8 the step was 2^-24: a first token that takes nearly all left nothing of the others.  Both take the same time: 128 tokens
+// at contexts 128..4096 49.7 us, 3 at 20480..65536 36.7 against 36.4.)
 //
 // Without its arithmetic the kernel streams at the copy peak (128 tokens at contexts 128..4096: 43.3 us); with it 50.2, bound by the
 // instructions of a page: about 180, 40 of them conversions.  K by the 8-bit MMA instead (its operands as they are, the query in two
@@ -39,7 +42,9 @@ namespace lfm25 {
 
 namespace {
 
-constexpr float kHeadroom = 8.0f;        // log2 of the largest weight against the reference maximum
+constexpr float kHeadroom = 4.0f;        // log2 of the largest weight against that of the reference maximum
+constexpr float kLift = 11.0f;           // log2 of that of the reference maximum
+static_assert(kHeadroom + kLift < 16.0f, "f16 ends in front of 2^16");
 constexpr float kNoResult = -1.0f;       // sum of a share that met an unassigned page
 
 struct DecodeParams {
@@ -436,7 +441,7 @@ e4m3_attention_kernel(const DecodeParams p) {
             for (uint32_t n = 0; n < NT; ++n) {
                 float w[4];
 #pragma unroll
-                for (uint32_t i = 0; i < 4; ++i) w[i] = fast_exp2(fmaf(s[j][i >> 1][2 * n + (i & 1)], factor[j][n], -maximum[n]));
+                for (uint32_t i = 0; i < 4; ++i) w[i] = fast_exp2(fmaf(s[j][i >> 1][2 * n + (i & 1)], factor[j][n], kLift - maximum[n]));
                 weights[j][n][0] = pack_f16x2(w[0], w[1]);
                 weights[j][n][1] = pack_f16x2(w[2], w[3]);
                 // the sum of the weights before their rounding to 11 bits, which averages out over the keys
