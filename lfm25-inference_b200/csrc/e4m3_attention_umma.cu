@@ -434,6 +434,16 @@ e4m3_prompt_attention_kernel(const PromptParams p) {
                 }
             }
             copies_wait<L::kAhead - 1>();
+            if (stage % kBlock == 0) {
+                // A page that none of the tile's rows sees (it belongs to a token that has no result) may hold anything.  Masked scores
+                // are -inf, which a negative factor would make the largest of all, and a weight of 0 must not meet an infinity or a NaN:
+                // 0 in the place of what is no scale.  A NaN among the factors of keys reaches the rows that see them, and no others.
+                // (Here, two stages behind the loads, and not where they are asked for.)
+                const bool number = fabsf(value_scale[0]) <= 3.4028235e38f;
+                if (!(key_scale[0] > 0.0f && key_scale[0] <= 3.4028235e38f)) key_scale[0] = 0.0f;
+                if (!number) key_scale[0] = __int_as_float(0x7fc00000);
+                if (!number) value_scale[0] = 0.0f;
+            }
             uint4 k_now[kLoads];
             uint4 v_now[kLoads];
 #pragma unroll

@@ -5,7 +5,9 @@ import torch
 
 import e4m3_cases as plain
 from conftest import to_u32
-from test_gpu_e4m3_cache import BF16_WEIGHTS, F16_WEIGHTS, PAGE, arena_of, attention_call, bf16, host, pool_of, tables_of
+from lfm25_inference_b200 import ops
+from test_gpu_e4m3_cache import (BF16_WEIGHTS, F16_WEIGHTS, PAGE, arena_of, attention_call, bf16, check_attention, host, pool_of,
+                                 random_cache, tables_of)
 
 pytestmark = pytest.mark.gpu
 
@@ -43,3 +45,45 @@ def test_a_first_token_that_takes_nearly_all(device, kind, heads, kv_heads, dim,
         bound = bound + context * 2.0 ** -36
     worst = np.abs((host(out) - exact) / bound).max()
     assert worst <= 1, f"error over its bound: {worst}, {host(out).max()} for {exact.max()}"
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim", [(8, 2, 64), (8, 2, 128)])
+@pytest.mark.parametrize("stray", [float("nan"), float("inf"), -float("inf"), -1.0])
+def test_prompt_tiles_with_pages_that_none_of_their_rows_sees(device, heads, kv_heads, dim, stray):
+    """A segment ends in tokens of nobody (a padded portion), whose pages are assigned and were never written: whatever lies there,
+    the tokens in front of them have their results, and those behind keep their rows."""
+    rng = np.random.default_rng(31)
+    arena, *cache = random_cache(rng, 9, kv_heads, dim, device)
+    tables = np.arange(9)[None]
+    count, real = 50, 20                        # positions 60 .. 79, then up to 109: pages 5 and 6 belong to nobody
+    for tensor in (arena.key_scales, arena.value_scales):
+        tensor[5:7] = stray
+    for part in cache:
+        part.values[5:7] = 0
+    rows = np.where(np.arange(count) < real, 0, plain.UNASSIGNED)
+    positions = np.where(np.arange(count) < real, 60 + np.arange(count), 0)
+    query = bf16(rng.standard_normal((count, heads, dim)), device)
+    out = torch.full_like(query, 3.0)
+    ops.paged_prompt_attention_e4m3_into(query, arena, to_u32(tables, device), to_u32(rows, device), to_u32(positions, device),
+                                         to_u32([0, count], device), out)
+    assert (out[real:] == 3.0).all()
+    check_attention(out[:real], query[:real], cache, tables, rows[:real], positions[:real], BF16_WEIGHTS, out[:real])
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_prompt_rows_that_see_a_page_whose_scale_is_no_number(device, dim):
+    """... are no numbers either, and only they."""
+    rng = np.random.default_rng(32)
+    arena, *cache = random_cache(rng, 9, 2, dim, device)
+    tables = np.arange(9)[None]
+    arena.value_scales[5, 1] = float("nan")
+    cache[1].scales[5, 1] = 0
+    positions = 60 + np.arange(50)
+    query = bf16(rng.standard_normal((50, 4, dim)), device)
+    out = torch.full_like(query, 3.0)
+    ops.paged_prompt_attention_e4m3_into(query, arena, to_u32(tables, device), to_u32(np.zeros(50), device), to_u32(positions, device),
+                                         to_u32([0, 50], device), out)
+    sees = positions >= 80
+    got = host(out)
+    assert np.isnan(got[sees, 2:]).all() and not np.isnan(got[:, :2]).any() and not np.isnan(got[~sees]).any()
+    check_attention(out[:20], query[:20], cache, tables, np.zeros(20, dtype=int), positions[:20], BF16_WEIGHTS, out[:20])
