@@ -20,8 +20,8 @@
 // MMA, both in f32, where a power of two rounds nothing.
 //
 // The maximum that weights refer to is only raised when a score exceeds it by more than 4 (log2): most pages need no exchange between
-// lanes.  Weights go to the product in f16, rounded to 11 bits: times 2^11, which the sum of weights has as well, so that the largest
-// there can be, 2^15, still fits and the smallest step is 2^-35 of the weight of the maximum.  (Without that factor and with a
+// lanes.  Weights go to the product in f16, rounded to 11 bits: times 2^11, which the page's scale and the sum of weights take back, so
+// that the largest there can be, 2^15, still fits and the smallest step is 2^-35 of the weight of the maximum.  (Without that factor and with a
 // headroom of 8 the step was 2^-24: a first token that takes nearly all left nothing of the others.  Both take the same time: 128 tokens
 // at contexts 128..4096 49.7 us, 3 at 20480..65536 36.7 against 36.4.)
 //
@@ -44,6 +44,7 @@ namespace {
 
 constexpr float kHeadroom = 4.0f;        // log2 of the largest weight against that of the reference maximum
 constexpr float kLift = 11.0f;           // log2 of that of the reference maximum
+constexpr float kUnlift = 1.0f / 2048.0f;
 static_assert(kHeadroom + kLift < 16.0f, "f16 ends in front of 2^16");
 constexpr float kNoResult = -1.0f;       // sum of a share that met an unassigned page
 
@@ -382,7 +383,7 @@ e4m3_attention_kernel(const DecodeParams p) {
             }
             const uint32_t source = group % kBlock * NP + j;
             const float key_scale = __shfl_sync(0xffffffffu, group >= block ? scales[0][0] : scales[1][0], source);
-            value_scale[j] = __shfl_sync(0xffffffffu, group >= block ? scales[0][1] : scales[1][1], source);
+            value_scale[j] = __shfl_sync(0xffffffffu, group >= block ? scales[0][1] : scales[1][1], source) * kUnlift;
             // never 0, so that -inf stays what it is (a score is below 2^28: with this factor it is 0)
 #pragma unroll
             for (uint32_t n = 0; n < NT; ++n) factor[j][n] = fmaxf(key_scale * query_factor[n], 1.1754944e-38f);
@@ -510,6 +511,7 @@ e4m3_attention_kernel(const DecodeParams p) {
     for (uint32_t n = 0; n < NT; ++n) {
         sum[n] += __shfl_xor_sync(0xffffffffu, sum[n], 1);
         sum[n] += __shfl_xor_sync(0xffffffffu, sum[n], 2);
+        sum[n] *= kUnlift;
         float* mine = merge + warp * HEADS * STRIDE;
         if (t == 0) {
             mine[(8 * n + g) * STRIDE + DIM] = maximum[n];

@@ -4,7 +4,7 @@ import pytest
 import torch
 
 import e4m3_cases as plain
-from conftest import to_u32
+from conftest import to_i64, to_u32
 from lfm25_inference_b200 import ops
 from test_gpu_e4m3_cache import (BF16_WEIGHTS, F16_WEIGHTS, PAGE, arena_of, attention_call, bf16, check_attention, host, pool_of,
                                  random_cache, tables_of)
@@ -87,3 +87,23 @@ def test_prompt_rows_that_see_a_page_whose_scale_is_no_number(device, dim):
     got = host(out)
     assert np.isnan(got[sees, 2:]).all() and not np.isnan(got[:, :2]).any() and not np.isnan(got[~sees]).any()
     check_attention(out[:20], query[:20], cache, tables, np.zeros(20, dtype=int), positions[:20], BF16_WEIGHTS, out[:20])
+
+
+@pytest.mark.parametrize("kind", ["decode", "prompts"])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_large_values(device, kind, dim):
+    """Values of 1e37 times a weight of 1 are what f32 holds; the factor that keeps small weights must not show."""
+    rng = np.random.default_rng(35)
+    arena = ops.E4m3KvArena.new(8, 1, dim, device=device)
+    cache = [plain.Cache(np.zeros((8, 1, PAGE, dim), dtype=np.uint8), np.zeros((8, 1))) for _ in range(2)]
+    key, value = bf16(rng.standard_normal((128, 1, dim)) * 0.1, device), bf16(rng.uniform(-1e37, 1e37, (128, 1, dim)) / 8, device)
+    arena.write(key, value, to_i64(np.arange(128), device))
+    for part, array in zip(cache, (key, value)):
+        part.append(host(array), np.arange(128))
+    positions = np.arange(30, 128)
+    query = bf16(rng.standard_normal((98, 4, dim)), device)
+    out = torch.zeros_like(query)
+    given = to_u32(np.arange(8)[None], device), to_u32(np.zeros(98), device), to_u32(positions, device)
+    attention_call(kind, query, arena, *given, out)
+    check_attention(out, query, cache, np.arange(8)[None], np.zeros(98, dtype=int), positions,
+                    F16_WEIGHTS if kind == "decode" else BF16_WEIGHTS, out)
