@@ -155,6 +155,14 @@ __device__ __forceinline__ uint32_t add_f16x2(uint32_t a, uint32_t b) {
     return v;
 }
 
+// A pair of bf16 with the largest finite number in the place of an infinity: 256 * 2^120 and beyond, codes of values that bf16 holds
+// rounded up to the next code, are more than f32 does.  (A weight of 0 must not meet an infinity.)
+__device__ __forceinline__ uint32_t pack_finite_bf16x2(float low, float high) {
+    uint32_t v;
+    asm("cvt.rn.satfinite.bf16x2.f32 %0, %1, %2;" : "=r"(v) : "f"(high), "f"(low));
+    return v;
+}
+
 __device__ __forceinline__ void umma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
         "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
@@ -471,7 +479,7 @@ e4m3_prompt_attention_kernel(const PromptParams p) {
                         check = add_f16x2(check, halves);
                         const float2 x = f16x2_to_float2(halves);
                         const float2 scaled = pair_out(pair_mul(pair_of(x.x, x.y), scales));
-                        pairs[j] = pack_bf16x2(scaled.x, scaled.y);
+                        pairs[j] = pack_finite_bf16x2(scaled.x, scaled.y);
                     }
                     store_shared(place + (((2 * dims % 8 + h) ^ turn) << 4), make_uint4(pairs[0], pairs[1], pairs[2], pairs[3]));
                 }

@@ -107,3 +107,31 @@ def test_large_values(device, kind, dim):
     attention_call(kind, query, arena, *given, out)
     check_attention(out, query, cache, np.arange(8)[None], np.zeros(98, dtype=int), positions,
                     F16_WEIGHTS if kind == "decode" else BF16_WEIGHTS, out)
+
+
+@pytest.mark.parametrize("kind", ["decode", "prompts"])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_values_at_the_end_of_f32_reach_nobody_who_does_not_see_them(device, kind, dim):
+    """A value of 3.35e38 is the code of 256 at 2^120, which f32 does not hold.  Tokens in front of it are as ever."""
+    rng = np.random.default_rng(33)
+    arena = ops.E4m3KvArena.new(8, 1, dim, device=device)
+    cache = [plain.Cache(np.zeros((8, 1, PAGE, dim), dtype=np.uint8), np.zeros((8, 1))) for _ in range(2)]
+    key, value = (rng.standard_normal((128, 1, dim)) for _ in range(2))
+    value[64:] *= 1e37
+    value[100, 0, 3] = 3.35e38
+    key, value = bf16(key, device), bf16(value, device)
+    arena.write(key, value, to_i64(np.arange(128), device))
+    cache[0].append(host(key), np.arange(128))
+    cache[1].append(host(value), np.arange(128))
+    positions = np.arange(50, 128)
+    query = bf16(rng.standard_normal((78, 4, dim)), device)
+    out = torch.zeros_like(query)
+    given = to_u32(np.arange(8)[None], device), to_u32(np.zeros(78), device), to_u32(positions, device)
+    if kind == "decode":
+        ops.paged_attention_e4m3_into(query, arena, *given, out)
+    else:
+        ops.paged_prompt_attention_e4m3_into(query, arena, *given, to_u32([0, 78], device), out)
+    rows = np.zeros(50, dtype=int)
+    check_attention(out[:50], query[:50], cache, np.arange(8)[None], rows, positions[:50], F16_WEIGHTS if kind == "decode" else BF16_WEIGHTS,
+                    out[:50])
+    assert not out[50:].isnan().any()
