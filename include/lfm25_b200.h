@@ -304,7 +304,8 @@ int32_t lfm25_decode_one_kernel_preferred(size_t page_size, size_t context_token
  * ------------------------------------------------------------------------------------------
  * Keys and values as E4M3 codes with one scale for each page of 16 tokens and KV head: an element stands for
  * code * scale.  A scale is the smallest power of two, 2^-126 at least, under which the largest finite magnitude that
- * the page's tokens of this head brought is at most 448; a page that was never written may hold anything.  No
+ * the page's tokens of this head brought is at most 448 (a page that is filled by other means and appended to may have
+ * any scale in 2^-126 .. 2^120; it becomes the next power of two); a page that was never written may hold anything.  No
  * counterpart in the reference, whose cache is bf16.  Heads of 64 or 128, any number of KV heads (up to 1024) and of
  * query heads to each.  Code buffers, activations and norms are 16-byte aligned; token strides are counted in
  * elements, 0 = dense, else a multiple of 8.  No entry point needs a workspace. */

@@ -4,7 +4,8 @@
 // heads), or one share of their keys.  Keys come in stages of 64 (4 pages), converted once for both tiles:
 //
 //   page warps (4)      E4M3 codes by asynchronous copies two stages ahead, then converted into the operands of the MMA in shared
-//                       memory (128-byte swizzle): K to f16 as it is, V to bf16 with its page's scale, both without a rounding
+//                       memory (128-byte swizzle): K to f16 as it is, V to bf16 with its page's scale, both without a rounding (below
+//                       2^-124 a scale leaves the smallest codes less than bf16 holds: 2^-134 off at most)
 //   issuing warps (2)   one for each tile, per stage S = Q K^T (kind::f16 on f16 operands) and, once the weights are there, O += P V
 //                       (bf16, P read from tensor memory, V as an MN-major operand); S of two stages on right behind P V of this
 //                       one, so that the tensor core works while the softmax does

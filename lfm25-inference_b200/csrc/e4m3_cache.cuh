@@ -3,7 +3,7 @@
 // A scale is the smallest power of two 2^e, e >= -126, with largest <= 448 * 2^e.  E4M3 is a floating format: its relative
 // precision does not depend on where in its range a value lies, so a scale only has to place that range, and a power of two
 // does so without a rounding of its own.  x / 2^e is exact, raising a scale re-rounds only codes that become subnormal, and
-// code * 2^e is exact in bf16 as well as in f32.
+// code * 2^e is exact in f32, and in bf16 from e = -124 on (below, subnormal codes are off by 2^-134 at most).
 #pragma once
 
 #include <cuda_fp16.h>
@@ -20,11 +20,16 @@ __device__ __forceinline__ int32_t scale_exponent(uint32_t largest_bits) {
     return max(exponent, kLeastScaleExponent);
 }
 
-// e of a stored scale; what is no power of two in range (an arena that was never written, stray bits) counts as the least
-__device__ __forceinline__ int32_t stored_exponent(float scale) {
+// The scale that a page goes on with.  What is no number in 2^-126 .. 2^120 (an arena that was never written, stray bits) counts as the
+// least; a number in between that is no power of two, which no append leaves, is taken as it is.
+__device__ __forceinline__ float stored_scale(float scale) {
+    return scale >= 1.1754944e-38f && scale <= 1.329228e36f ? scale : 1.1754944e-38f;
+}
+
+// least e with scale <= 2^e
+__device__ __forceinline__ int32_t exponent_above(float scale) {
     const uint32_t bits = __float_as_uint(scale);
-    const int32_t exponent = static_cast<int32_t>(bits >> 23) - 127;
-    return (bits >> 31) != 0 || exponent > 120 ? kLeastScaleExponent : max(exponent, kLeastScaleExponent);
+    return static_cast<int32_t>(bits >> 23) - 127 + ((bits & 0x7fffffu) != 0 ? 1 : 0);
 }
 
 // 2^e for -126 <= e <= 127; below that 0, as the product with a code rounds to 0 there anyway

@@ -257,9 +257,9 @@ e4m3_cache_write_kernel(const WriteParams p) {
         }
         if (unit + kWarps < units) load(unit + kWarps);
         largest = __reduce_max_sync(0xffffffffu, largest);
-        const int32_t old_exponent = stored_exponent(now.old_scale);
+        const float old_scale = stored_scale(now.old_scale);
         int32_t exponent = scale_exponent(largest);
-        if (now.offset > 0) exponent = max(exponent, old_exponent);
+        if (now.offset > 0) exponent = max(exponent, exponent_above(old_scale));
 
         const float factor = power_of_two(-exponent);
 #pragma unroll
@@ -272,8 +272,8 @@ e4m3_cache_write_kernel(const WriteParams p) {
             }
         }
         // what the page holds already goes over to a larger scale
-        if (now.offset > 0 && exponent > old_exponent) {
-            const float shrink = power_of_two(old_exponent - exponent);
+        const float shrink = old_scale * factor;
+        if (now.offset > 0 && shrink != 1.0f) {
 #pragma unroll 1
             for (uint32_t row = lane_row; row < now.offset; row += ROWS) {
                 uint2* place = reinterpret_cast<uint2*>(now.codes + row * DIM + 8 * piece);

@@ -135,3 +135,35 @@ def test_values_at_the_end_of_f32_reach_nobody_who_does_not_see_them(device, kin
     check_attention(out[:50], query[:50], cache, np.arange(8)[None], rows, positions[:50], F16_WEIGHTS if kind == "decode" else BF16_WEIGHTS,
                     out[:50])
     assert not out[50:].isnan().any()
+
+
+# ------------------------------------------------------------------------------------------------ append
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_append_to_pages_whose_scale_is_no_power_of_two(device, dim):
+    """The scale becomes the next power of two at least, and what the page holds keeps its values up to one more rounding."""
+    rng = np.random.default_rng(34)
+    given = np.array([1.5, 0.75, 2.0, 1.0 + 2.0 ** -23, 3e-3, 1.99, 1.25 * 2.0 ** 100, 1.75 * 2.0 ** -126])
+    heads, pages = 2, len(given)
+    codes = [rng.integers(0, 256, (pages, heads, PAGE, dim), dtype=np.uint8) for _ in range(2)]
+    scales = [np.repeat(given[:, None], heads, axis=1) for _ in range(2)]
+    arena = arena_of(codes, scales, device)
+    # the tokens bring nothing large to head 0 and 2^12 times the scale to head 1
+    rows = np.ones((pages, heads, dim)) * 2.0 ** -133
+    rows[:, 1] = (given * 2.0 ** 12)[:, None]
+    offset = 9
+    rows = bf16(rows, device)
+    ops.kv_cache_write_e4m3(rows, rows, arena, to_i64(np.arange(pages) * PAGE + offset, device))
+    for tensor, stored, before in ((arena.key, arena.key_scales, codes[0]), (arena.value, arena.value_scales, codes[1])):
+        stored = stored.cpu().numpy().astype(np.float64)
+        brought = host(rows)[:, :, 0]
+        for page in range(pages):
+            for head in range(heads):
+                scale = 2.0 ** np.ceil(np.log2(np.float32(given[page]).astype(np.float64)))
+                scale = max(scale, plain.scale_of(brought[page, head]))
+                assert stored[page, head] == scale
+                kept = plain.CODE_VALUES[before[page, head, :offset]] * np.float64(np.float32(given[page]))
+                got = plain.CODE_VALUES[tensor[page, head].cpu().numpy()]
+                assert np.array_equal(got[:offset], plain.round_e4m3(kept / scale), equal_nan=True)
+                assert np.array_equal(got[offset], plain.round_e4m3(host(rows)[page, head] / scale))
