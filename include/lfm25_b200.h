@@ -922,7 +922,8 @@ void lfm25_kv_allocator_release_sequence(lfm25_kv_allocator* allocator, size_t t
  * fork_sequence: block_table becomes a second sequence over the first `tokens` tokens of source_table.  Full pages are
  * shared, a last, partly filled one gets a page of its own: copy_pages = {source, destination} then, to be copied with
  * lfm25_kv_pages_copy before either sequence is appended to.  Returns the number of pages to copy (0 or 1).  The entries
- * that are filled must be unassigned before; on an error nothing has changed.
+ * that are filled must be unassigned before; on an error nothing has changed.  source_table holds at least the entries that
+ * `tokens` tokens take (ceil(tokens / page size)), which are read where block_table_len is as large.
  * release_window: gives back the pages that no later token sees, with `tokens` tokens cached, a window and first tokens that
  * stay visible (the rule of lfm25_paged_attention_e4m3); their entries become unassigned.  Returns their number.
  * compact: moves pages with high numbers to free ones with low numbers and rewrites `entries` block table entries (all rows of all

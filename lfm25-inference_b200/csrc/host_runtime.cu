@@ -39,7 +39,7 @@ struct lfm25_dispatcher {
 
 namespace {
 
-size_t div_ceil(size_t value, size_t divisor) { return (value + divisor - 1) / divisor; }
+size_t div_ceil(size_t value, size_t divisor) { return value / divisor + (value % divisor != 0 ? 1 : 0); }
 
 }  // namespace
 

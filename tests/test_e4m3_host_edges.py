@@ -1,0 +1,30 @@
+"""Calls of the 8-bit cache's host side with numbers that no cache has."""
+import numpy as np
+import pytest
+
+from lfm25_inference_b200 import _abi
+from lfm25_inference_b200.cache import KvAllocationError, KvPageAllocator
+
+FREE = 0xFFFFFFFF
+
+
+def table(length=8):
+    return np.full(length, FREE, dtype=np.uint32)
+
+
+@pytest.mark.parametrize("tokens", [2 ** 64 - 1, 2 ** 64 - 15, 2 ** 64 - 16, 2 ** 63])
+def test_more_tokens_than_pages_can_be_counted_for(tokens):
+    """Rounded up to whole pages, these wrapped to none: a fork then wrote behind its table."""
+    allocator = KvPageAllocator(8)
+    first, second = table(), table()
+    allocator.grow_sequence(0, 64, first)
+    library, pair = _abi.library(), np.zeros(2, dtype=np.uint32)
+
+    def pointer(array):
+        return array.ctypes.data_as(_abi._P(_abi.ctypes.c_uint32))
+
+    code = library.lfm25_kv_allocator_fork_sequence(allocator._handle, tokens, pointer(first), pointer(second), 8, pointer(pair))
+    assert code == _abi.KV_SEQUENCE_CAPACITY_EXCEEDED and (second == FREE).all()
+    with pytest.raises(KvAllocationError, match="capacity"):
+        allocator.grow_sequence(64, tokens, first)
+    assert allocator.snapshot()["allocated_pages"] == 4
