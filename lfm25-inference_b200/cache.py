@@ -29,6 +29,12 @@ def _count(value: int) -> int:
     return int(value)
 
 
+def _not_negative(what: str, *numbers: int) -> None:
+    """The library counts in size_t, where a negative number is a huge one."""
+    if min(numbers) < 0:
+        raise _abi.Lfm25Error(_abi.ERR_INVALID_ARGUMENT, f"{what} does not take negative numbers: {numbers}")
+
+
 def _table_pointer(table: np.ndarray):
     assert table.dtype == np.uint32 and table.flags["C_CONTIGUOUS"]
     return table.ctypes.data_as(ctypes.POINTER(ctypes.c_uint32))
@@ -76,7 +82,9 @@ class KvPageAllocator:
     def fork_sequence(self, tokens: int, source_table: np.ndarray, block_table: np.ndarray):
         """`block_table` (its entries unassigned) becomes a second sequence over the first `tokens` tokens of `source_table`:
         full pages are shared, a partly filled last one gets a page of its own.  Returns (source pages, destination pages) to be
-        copied with `ops.kv_pages_copy` before either sequence is appended to; no counterpart in the reference."""
+        copied with `ops.kv_pages_copy` before either sequence is appended to, both empty where there is nothing to copy; no
+        counterpart in the reference."""
+        _not_negative("fork of a sequence", tokens)
         pair = np.zeros(2, dtype=np.uint32)
         if -(-tokens // self._page_size) > source_table.size:
             raise KvAllocationError(_abi.KV_SEQUENCE_CAPACITY_EXCEEDED)
@@ -87,6 +95,7 @@ class KvPageAllocator:
     def release_window(self, tokens: int, window: int, sinks: int, block_table: np.ndarray) -> int:
         """Gives back the pages of a sequence of `tokens` cached tokens that no later token sees through a window with `sinks`
         first tokens kept; returns their number.  No counterpart in the reference."""
+        _not_negative("release behind a window", tokens, window, sinks)
         return self._moves(library().lfm25_kv_allocator_release_window(self._handle, tokens, window, sinks, _table_pointer(block_table),
                                                                        block_table.size))
 
@@ -94,7 +103,10 @@ class KvPageAllocator:
         """Moves pages with high numbers to free low ones and rewrites `block_tables` (the tables of all live sequences, any
         shape).  Returns (source pages, destination pages) to be copied with `ops.kv_pages_copy`.  Pages that somebody else holds as
         well (a prefix cache) stay.  No counterpart in the reference."""
-        capacity = self.snapshot()["total_pages"] if maximum_moves is None else maximum_moves
+        capacity = self.snapshot()["total_pages"]          # there are no more moves than pages
+        if maximum_moves is not None:
+            _not_negative("compaction", maximum_moves)
+            capacity = min(capacity, maximum_moves)
         source, destination = (np.zeros(max(1, capacity), dtype=np.uint32) for _ in range(2))
         moves = self._moves(library().lfm25_kv_allocator_compact(self._handle, _table_pointer(block_tables), block_tables.size,
                                                                  _table_pointer(source), _table_pointer(destination), capacity))

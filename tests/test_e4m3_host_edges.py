@@ -28,3 +28,21 @@ def test_more_tokens_than_pages_can_be_counted_for(tokens):
     with pytest.raises(KvAllocationError, match="capacity"):
         allocator.grow_sequence(64, tokens, first)
     assert allocator.snapshot()["allocated_pages"] == 4
+
+
+def test_negative_numbers_are_refused():
+    """... and change nothing: as size_t they are huge, and a compaction would have written that many moves."""
+    allocator = KvPageAllocator(8)
+    first, second = table(), table()
+    allocator.grow_sequence(0, 32, first)
+    allocator.grow_sequence(0, 32, second)
+    allocator.release_sequence(32, first)
+    before = second.copy()
+    for call in (lambda: allocator.compact(second, maximum_moves=-1), lambda: allocator.fork_sequence(-1, second, first),
+                 lambda: allocator.release_window(-1, 4, 0, second), lambda: allocator.release_window(32, -1, 0, second),
+                 lambda: allocator.release_window(32, 4, -1, second)):
+        with pytest.raises(_abi.Lfm25Error, match="negative"):
+            call()
+    assert np.array_equal(second, before) and allocator.snapshot()["allocated_pages"] == 2
+    assert len(allocator.compact(second, maximum_moves=0)[0]) == 0
+    assert len(allocator.compact(second, maximum_moves=2 ** 40)[0]) == 2      # more than there are pages
