@@ -378,6 +378,10 @@ class E4m3KvArena:
         if len(shape) != 4 or shape[2] != self.page_size:
             _refuse("8-bit cache: codes must have shape [pages, heads, 16, dim]")
         pages, heads, page_size, dim = shape
+        if self.value.shape != shape:
+            _refuse("8-bit cache: value codes must have the shape of key codes")
+        if self.key_scales.shape != (pages, heads) or self.value_scales.shape != (pages, heads):
+            _refuse("8-bit cache: scales must have shape [pages, heads]")
         codes, scales = pages * heads * page_size * dim, pages * heads
         return (page_size, pages, heads, dim, *_dense("key codes", self.key, _CODES, device),
                 *_dense("value codes", self.value, _CODES, device, codes), *_dense("key scales", self.key_scales, _F32, device, scales),

@@ -1,8 +1,9 @@
 """Calls of the 8-bit cache's host side with numbers that no cache has."""
 import numpy as np
 import pytest
+import torch
 
-from lfm25_inference_b200 import _abi
+from lfm25_inference_b200 import _abi, ops
 from lfm25_inference_b200.cache import KvAllocationError, KvPageAllocator
 
 FREE = 0xFFFFFFFF
@@ -46,3 +47,20 @@ def test_negative_numbers_are_refused():
     assert np.array_equal(second, before) and allocator.snapshot()["allocated_pages"] == 2
     assert len(allocator.compact(second, maximum_moves=0)[0]) == 0
     assert len(allocator.compact(second, maximum_moves=2 ** 40)[0]) == 2      # more than there are pages
+
+
+@pytest.mark.parametrize("change,message", [
+    (dict(value=torch.zeros((4, 3, 16, 64), dtype=torch.uint8)), "value codes"),
+    (dict(value=torch.zeros((3, 4, 16 * 64), dtype=torch.uint8)), "value codes"),
+    (dict(key_scales=torch.zeros((4, 3))), "scales must have shape"),
+    (dict(value_scales=torch.zeros((4, 3))), "scales must have shape"),
+    (dict(value_scales=torch.zeros((12,))), "scales must have shape"),
+    (dict(key=torch.zeros((3, 4, 8, 128), dtype=torch.uint8)), "codes must have shape")])
+def test_arenas_whose_buffers_disagree_are_refused(change, message):
+    """Buffers of the right number of elements in another order, as a transposed table of scales has, are no cache."""
+    whole = ops.E4m3KvArena.new(3, 4, 64, device="cpu")
+    fields = {name: getattr(whole, name) for name in ("key", "value", "key_scales", "value_scales")}
+    arena = ops.E4m3KvArena(**{**fields, **change})
+    rows = torch.zeros((2, 4, 64), dtype=torch.bfloat16)
+    with pytest.raises(_abi.Lfm25Error, match=message):
+        arena.write(rows, rows, torch.zeros(2, dtype=torch.int64))
