@@ -385,6 +385,10 @@ typedef struct lfm25_paged_attention_e4m3_launch {
 } lfm25_paged_attention_e4m3_launch;
 /* Single tokens, each by itself: a decode step. */
 int32_t lfm25_paged_attention_e4m3(void* stream, const lfm25_paged_attention_e4m3_launch* launch);
+/* How that call is shared out, without making it: warps of a CTA (4 or 8) and CTAs that share a token's keys (1, 2, 4, 8, or 16
+ * where clusters_of_16 is not 0 -- the call asks the device whether it holds such clusters). */
+int32_t lfm25_paged_attention_e4m3_plan(const lfm25_paged_attention_e4m3_launch* launch, int32_t clusters_of_16, uint32_t* warps,
+                                        uint32_t* splits);
 /* Portions of prompts, whose own keys were appended before: the tokens segment_offsets[s] .. segment_offsets[s + 1] sit at
  * consecutive positions of one request slot; tokens outside every segment, and tokens that do not continue their
  * segment's first, keep their output row. */

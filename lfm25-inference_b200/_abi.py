@@ -305,6 +305,8 @@ PROTOTYPES = {
     "lfm25_kv_cache_write_e4m3": (ctypes.c_int32, [_stream, _P(KvCacheWriteE4m3Launch)]),
     "lfm25_qk_norm_rope_kv_write_e4m3": (ctypes.c_int32, [_stream, _P(QkNormRopeKvWriteE4m3Launch)]),
     "lfm25_paged_attention_e4m3": (ctypes.c_int32, [_stream, _P(PagedAttentionE4m3Launch)]),
+    "lfm25_paged_attention_e4m3_plan": (
+        ctypes.c_int32, [_P(PagedAttentionE4m3Launch), ctypes.c_int32, _P(ctypes.c_uint32), _P(ctypes.c_uint32)]),
     "lfm25_paged_prompt_attention_e4m3": (ctypes.c_int32, [_stream, _P(PagedAttentionE4m3Launch)]),
     "lfm25_kv_pages_copy": (ctypes.c_int32, [_stream, _P(PageArena), _size, Slice, Slice, _size]),
     "lfm25_quantize_bf16_e4m3": (ctypes.c_int32, [_stream, Slice, Slice, _size, ctypes.c_float]),

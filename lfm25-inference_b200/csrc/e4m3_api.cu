@@ -199,6 +199,17 @@ int32_t lfm25_paged_attention_e4m3(void* stream, const lfm25_paged_attention_e4m
     return cuda_result(lfm25::launch_e4m3_attention(static_cast<cudaStream_t>(stream), args), "8-bit cache attention launch failed");
 }
 
+int32_t lfm25_paged_attention_e4m3_plan(const lfm25_paged_attention_e4m3_launch* launch, int32_t clusters_of_16, uint32_t* warps,
+                                        uint32_t* splits) {
+    E4M3_ENSURE(launch != nullptr && warps != nullptr && splits != nullptr, LFM25_ERR_NULL_POINTER, "8-bit cache attention plan received a null pointer");
+    lfm25::E4m3AttentionLaunch args = {};
+    E4M3_CHECK(take_attention(*launch, &args));
+    const lfm25::E4m3DecodePlan plan = lfm25::plan_e4m3_attention(args, clusters_of_16 != 0);
+    *warps = plan.warps;
+    *splits = 1u << plan.splits_log2;
+    return LFM25_OK;
+}
+
 int32_t lfm25_paged_prompt_attention_e4m3(void* stream, const lfm25_paged_attention_e4m3_launch* launch) {
     E4M3_ENSURE(launch != nullptr, LFM25_ERR_NULL_POINTER, "8-bit cache attention launch is null");
     lfm25::E4m3AttentionLaunch args = {};

@@ -31,6 +31,7 @@
 //
 // Split: with few (token, KV head) pairs the pages of one are shared by the CTAs of a cluster, joined through distributed
 // shared memory: no workspace, so calls never share memory, and one launch.
+#include <atomic>
 #include <type_traits>
 
 #include "e4m3_cache.cuh"
@@ -586,6 +587,38 @@ e4m3_attention_kernel(const DecodeParams p) {
     cluster_barrier();      // nobody leaves while its share is read
 }
 
+// Whether the device holds a cluster of 16 CTAs of this shape, which needs as many places in one group of SMs: asked once per device.
+template <uint32_t DIM, uint32_t HEADS, uint32_t WARPS>
+bool clusters_of_16_fit() {
+    using S = Shape<DIM, HEADS, WARPS>;
+    static std::atomic<uint64_t> asked{0}, fits{0};
+    int device = 0;
+    if (cudaGetDevice(&device) != cudaSuccess) return false;
+    const uint64_t bit = uint64_t{1} << (device & 63);
+    if ((asked.load(std::memory_order_acquire) & bit) == 0) {
+        cudaLaunchConfig_t config = {};
+        config.gridDim = dim3(16, 1, 1);
+        config.blockDim = dim3(S::kThreads, 1, 1);
+        config.dynamicSmemBytes = S::kBytes;
+        cudaLaunchAttribute attribute;
+        attribute.id = cudaLaunchAttributeClusterDimension;
+        attribute.val.clusterDim.x = 16;
+        attribute.val.clusterDim.y = 1;
+        attribute.val.clusterDim.z = 1;
+        config.attrs = &attribute;
+        config.numAttrs = 1;
+        int clusters = 0;
+        if (allow_shared_memory<e4m3_attention_kernel<DIM, HEADS, WARPS>, true>(S::kBytes) != cudaSuccess ||
+            cudaOccupancyMaxActiveClusters(&clusters, e4m3_attention_kernel<DIM, HEADS, WARPS>, &config) != cudaSuccess) {
+            (void)cudaGetLastError();
+            clusters = 0;
+        }
+        if (clusters > 0) fits.fetch_or(bit, std::memory_order_relaxed);
+        asked.fetch_or(bit, std::memory_order_release);
+    }
+    return (fits.load(std::memory_order_relaxed) & bit) != 0;
+}
+
 template <uint32_t DIM, uint32_t HEADS, uint32_t WARPS>
 cudaError_t launch_shape(cudaStream_t stream, const DecodeParams& params, uint64_t blocks) {
     using S = Shape<DIM, HEADS, WARPS>;
@@ -597,6 +630,21 @@ cudaError_t launch_shape(cudaStream_t stream, const DecodeParams& params, uint64
                          params.splits, params);
 }
 
+// (token, KV head, chunk of query heads) triples, and pages of the longest context that a token can see
+struct DecodeWork {
+    uint64_t items;
+    uint64_t pages;
+};
+
+DecodeWork decode_work(const E4m3AttentionLaunch& launch) {
+    const uint64_t group = launch.query_heads / launch.cache.kv_heads;
+    uint64_t longest = launch.maximum_context_tokens;
+    if (launch.window != 0 && longest > static_cast<uint64_t>(launch.window) + launch.sinks) {
+        longest = static_cast<uint64_t>(launch.window) + launch.sinks + kPageSize;
+    }
+    return {static_cast<uint64_t>(launch.num_tokens) * launch.cache.kv_heads * ((group + 15) / 16), (longest + kPageSize - 1) / kPageSize};
+}
+
 // CTAs of 4 warps, their pages shared by a cluster of as many (up to 16) as fill the SMs once, a quarter over, while each warp
 // has 8 pages or more: a cluster costs about as much as 6 pages of one warp (23 padded to 32 tokens through a window of 4096, 2 KV heads of
 // 128: 4 CTAs 18.1, 8 CTAs 14.9, 16 CTAs 24.8 us; 3 tokens at 20480..65536: 4 CTAs 69, 8 CTAs 47, 16 CTAs 36.9 us; 32 tokens at 64..400:
@@ -604,26 +652,47 @@ cudaError_t launch_shape(cudaStream_t stream, const DecodeParams& params, uint64
 // 32 tokens at 64..400: 5.8 against 6.5 us).  8 of those rather than 16 CTAs up to 48 pages a warp (4 tokens at 8000..16000: 16.7 us
 // against 19.8 with 16 of 4 warps; 2 at 30000: 23.2 against 25.2 with 16 of 8), beyond that 16 (1 at 65536: 24.6 against 30.7 us).
 template <uint32_t DIM, uint32_t HEADS>
-cudaError_t launch_heads(cudaStream_t stream, DecodeParams params, uint64_t items, uint64_t pages) {
+E4m3DecodePlan plan_heads(const DecodeWork& work, bool clusters_of_16) {
     using S = Shape<DIM, HEADS, 4>;
     constexpr uint64_t kSms = 148;
     constexpr uint64_t kResident = kSms * S::kPerSm;
-    while (params.splits_log2 < 4 && (items << (params.splits_log2 + 1)) <= kResident + kResident / 4 &&
-           pages >= (8ull * 4 << params.splits_log2)) {
-        ++params.splits_log2;
+    const uint32_t most = clusters_of_16 ? 4 : 3;
+    E4m3DecodePlan plan = {4, 0};
+    while (plan.splits_log2 < most && (work.items << (plan.splits_log2 + 1)) <= kResident + kResident / 4 &&
+           work.pages >= (8ull * 4 << plan.splits_log2)) {
+        ++plan.splits_log2;
     }
-    auto wide_fits = [&](uint32_t splits_log2) { return (items << splits_log2) * 8 <= kSms * S::kWarpsPerSm; };
-    if (params.splits_log2 == 4 && wide_fits(3) && pages < 48 * 8 * 8) params.splits_log2 = 3;
-    const bool wide = wide_fits(params.splits_log2);
-    params.splits = 1u << params.splits_log2;
-    const uint64_t blocks = items << params.splits_log2;
+    auto wide_fits = [&](uint32_t splits_log2) { return (work.items << splits_log2) * 8 <= kSms * S::kWarpsPerSm; };
+    if (plan.splits_log2 == 4 && wide_fits(3) && work.pages < 48 * 8 * 8) plan.splits_log2 = 3;
+    if (wide_fits(plan.splits_log2)) plan.warps = 8;
+    return plan;
+}
+
+template <uint32_t DIM, uint32_t HEADS>
+cudaError_t launch_heads(cudaStream_t stream, DecodeParams params, const DecodeWork& work) {
+    E4m3DecodePlan plan = plan_heads<DIM, HEADS>(work, true);
+    if (plan.splits_log2 == 4 && !(plan.warps == 8 ? clusters_of_16_fit<DIM, HEADS, 8>() : clusters_of_16_fit<DIM, HEADS, 4>())) {
+        plan = plan_heads<DIM, HEADS>(work, false);
+    }
+    params.splits_log2 = plan.splits_log2;
+    params.splits = 1u << plan.splits_log2;
+    const uint64_t blocks = work.items << plan.splits_log2;
     if (blocks > 0x7fffffffu) {
         return cudaErrorInvalidConfiguration;
     }
-    return wide ? launch_shape<DIM, HEADS, 8>(stream, params, blocks) : launch_shape<DIM, HEADS, 4>(stream, params, blocks);
+    return plan.warps == 8 ? launch_shape<DIM, HEADS, 8>(stream, params, blocks) : launch_shape<DIM, HEADS, 4>(stream, params, blocks);
 }
 
 }  // namespace
+
+E4m3DecodePlan plan_e4m3_attention(const E4m3AttentionLaunch& launch, bool clusters_of_16) {
+    const DecodeWork work = decode_work(launch);
+    const bool few = launch.query_heads / launch.cache.kv_heads <= 8;
+    if (launch.cache.head_dim == 64) {
+        return few ? plan_heads<64, 8>(work, clusters_of_16) : plan_heads<64, 16>(work, clusters_of_16);
+    }
+    return few ? plan_heads<128, 8>(work, clusters_of_16) : plan_heads<128, 16>(work, clusters_of_16);
+}
 
 cudaError_t launch_e4m3_attention(cudaStream_t stream, const E4m3AttentionLaunch& launch) {
     DecodeParams params = {};
@@ -644,20 +713,14 @@ cudaError_t launch_e4m3_attention(cudaStream_t stream, const E4m3AttentionLaunch
     params.window = launch.window;
     params.sinks = launch.sinks;
     params.scale_log2 = launch.scale * kLog2e;
-    const uint64_t items = static_cast<uint64_t>(launch.num_tokens) * launch.cache.kv_heads * params.chunks;
-    if (items > 0x7fffffffu) {
+    const DecodeWork work = decode_work(launch);
+    if (work.items > 0x7fffffffu) {
         return cudaErrorInvalidConfiguration;
     }
-    // pages of the longest context that a token can see
-    uint64_t longest = launch.maximum_context_tokens;
-    if (launch.window != 0 && longest > static_cast<uint64_t>(launch.window) + launch.sinks) {
-        longest = static_cast<uint64_t>(launch.window) + launch.sinks + kPageSize;
-    }
-    const uint64_t pages = (longest + kPageSize - 1) / kPageSize;
     if (launch.cache.head_dim == 64) {
-        return params.group <= 8 ? launch_heads<64, 8>(stream, params, items, pages) : launch_heads<64, 16>(stream, params, items, pages);
+        return params.group <= 8 ? launch_heads<64, 8>(stream, params, work) : launch_heads<64, 16>(stream, params, work);
     }
-    return params.group <= 8 ? launch_heads<128, 8>(stream, params, items, pages) : launch_heads<128, 16>(stream, params, items, pages);
+    return params.group <= 8 ? launch_heads<128, 8>(stream, params, work) : launch_heads<128, 16>(stream, params, work);
 }
 
 }  // namespace lfm25

@@ -62,6 +62,14 @@ struct E4m3AttentionLaunch {
     float scale;
 };
 cudaError_t launch_e4m3_attention(cudaStream_t stream, const E4m3AttentionLaunch& launch);
+
+// How single tokens are shared out: warps of a CTA (4 or 8) and CTAs of a cluster, 1 << splits_log2, clusters of 16 only where the device
+// holds them.
+struct E4m3DecodePlan {
+    uint32_t warps;
+    uint32_t splits_log2;
+};
+E4m3DecodePlan plan_e4m3_attention(const E4m3AttentionLaunch& launch, bool clusters_of_16);
 cudaError_t launch_e4m3_prompt_attention(cudaStream_t stream, const E4m3AttentionLaunch& launch);
 
 // `bytes` per page, pages one behind the other from `base`

@@ -3,6 +3,7 @@ import numpy as np
 import pytest
 import torch
 
+from e4m3_batches import ALL, BATCHES, plan
 from lfm25_inference_b200 import _abi, ops
 from lfm25_inference_b200.cache import KvAllocationError, KvPageAllocator
 
@@ -64,3 +65,15 @@ def test_arenas_whose_buffers_disagree_are_refused(change, message):
     rows = torch.zeros((2, 4, 64), dtype=torch.bfloat16)
     with pytest.raises(_abi.Lfm25Error, match=message):
         arena.write(rows, rows, torch.zeros(2, dtype=torch.int64))
+
+
+@pytest.mark.parametrize("layout,form,tokens,longest", ALL)
+def test_batches_take_the_form_that_they_are_tested_for(layout, form, tokens, longest):
+    assert plan(tokens, *layout, longest) == form
+    warps, splits = plan(tokens, *layout, longest, clusters_of_16=False)
+    assert splits <= 8 and warps in (4, 8) and (splits == form[1] or form[1] == 16)
+
+
+def test_every_form_has_its_batch():
+    forms = {(warps, splits) for warps in (4, 8) for splits in (1, 2, 4, 8, 16)}
+    assert all(set(batches) == forms for batches in BATCHES.values())
