@@ -1,9 +1,10 @@
-"""The 8-bit paged cache at the ends of its number formats."""
+"""The 8-bit paged cache at the ends of its number formats, and single tokens in every form of the kernel."""
 import numpy as np
 import pytest
 import torch
 
 import e4m3_cases as plain
+from e4m3_batches import ALL, plan
 from conftest import to_i64, to_u32
 from lfm25_inference_b200 import ops
 from test_gpu_e4m3_cache import (BF16_WEIGHTS, F16_WEIGHTS, PAGE, arena_of, attention_call, bf16, check_attention, host, pool_of,
@@ -167,3 +168,31 @@ def test_append_to_pages_whose_scale_is_no_power_of_two(device, dim):
                 got = plain.CODE_VALUES[tensor[page, head].cpu().numpy()]
                 assert np.array_equal(got[:offset], plain.round_e4m3(kept / scale), equal_nan=True)
                 assert np.array_equal(got[offset], plain.round_e4m3(host(rows)[page, head] / scale))
+
+
+# ------------------------------------------------------------------------------------------------ forms of the kernel
+
+
+@pytest.mark.parametrize("windowed", [False, True])
+@pytest.mark.parametrize("layout,form,tokens,longest", ALL)
+def test_decode_attention_in_every_form(device, layout, form, tokens, longest, windowed):
+    """4 or 8 warps a CTA, clusters of 1 to 16, few and many heads to a KV head, in batches that take them (that is looked at, too);
+    some tokens are compared, the one of the longest context among them.  With a window that leaves as much to see."""
+    heads, kv_heads, dim = layout
+    window, sinks = (longest - 21, 5) if windowed else (0, 0)
+    most = longest + (longest // 3 if windowed else 0)
+    assert plan(tokens, *layout, most, window, sinks) == form
+    rng = np.random.default_rng(tokens * dim + longest)
+    contexts = tuple(int(c) for c in rng.integers(1, most + 1, tokens - 1)) + (most,)
+    pool = pool_of(contexts)
+    arena, *cache = random_cache(rng, pool, kv_heads, dim, device)
+    tables = tables_of(rng, contexts, pool)
+    order = rng.permutation(tokens)
+    positions = np.array(contexts)[order] - 1
+    query = bf16(rng.standard_normal((tokens, heads, dim)) * 0.5, device)
+    out = torch.full_like(query, float("nan"))
+    ops.paged_attention_e4m3_into(query, arena, to_u32(tables, device), to_u32(order, device), to_u32(positions, device), out,
+                                  window=window, sinks=sinks, maximum_context_tokens=most)
+    assert not out.isnan().any()
+    some = np.unique(np.concatenate(([np.argmax(positions)], rng.integers(0, tokens, 6))))
+    check_attention(out[some], query[some], cache, tables, order[some], positions[some], F16_WEIGHTS, out[some], window=window, sinks=sinks)
