@@ -645,25 +645,44 @@ DecodeWork decode_work(const E4m3AttentionLaunch& launch) {
     return {static_cast<uint64_t>(launch.num_tokens) * launch.cache.kv_heads * ((group + 15) / 16), (longest + kPageSize - 1) / kPageSize};
 }
 
+// Clusters of 1, 2, 4, 8 and 16 CTAs that a B200 holds at once, with 1 to 4 CTAs an SM, as cudaOccupancyMaxActiveClusters answers: a
+// cluster stays within one group of SMs.
+constexpr uint32_t kResidentClusters[4][5] = {{148, 74, 33, 15, 7}, {296, 148, 71, 33, 14}, {444, 222, 104, 48, 21}, {592, 296, 142, 71, 31}};
+
 // CTAs of 4 warps, their pages shared by a cluster of as many (up to 16) as fill the SMs once, a quarter over, while each warp
-// has 8 pages or more: a cluster costs about as much as 6 pages of one warp (23 padded to 32 tokens through a window of 4096, 2 KV heads of
-// 128: 4 CTAs 18.1, 8 CTAs 14.9, 16 CTAs 24.8 us; 3 tokens at 20480..65536: 4 CTAs 69, 8 CTAs 47, 16 CTAs 36.9 us; 32 tokens at 64..400:
-// 1 CTA 6.5, 2 CTAs 7.5 us).  Where that leaves half of the warps' places free, CTAs of 8 warps (1 token at 8000: 8.2 against 8.9 us;
-// 32 tokens at 64..400: 5.8 against 6.5 us).  8 of those rather than 16 CTAs up to 48 pages a warp (4 tokens at 8000..16000: 16.7 us
-// against 19.8 with 16 of 4 warps; 2 at 30000: 23.2 against 25.2 with 16 of 8), beyond that 16 (1 at 65536: 24.6 against 30.7 us).
+// has 8 pages or more; where all clusters run at once with CTAs of 8 warps, those.  Of 32 heads on 8 of 64, 1 token at 8000: 8 CTAs of 8
+// warps 8.3, 16 of 4 8.7, 8 of 4 9.0 us; 32 at 64..400: 1 CTA of 8 warps 5.7, of 4 6.5, 2 of 4 7.3 us.  Of 8 heads on 2 of 128, 4 tokens
+// at 8000..16000: 8 of 8 15.5, 16 of 4 15.0, 16 of 8 19.5 us; 100 at 500..5000: 2 of 4 34.4, 1 of 8 39.2, 1 of 4 45.5 us.
+// Clusters that do not all run at once cost their whole time again for the last ones: 16 of 8 CTAs of 8 warps where 15 find room take
+// 13.7 us (16 tokens at 4000, 16 heads on 1 of 64) and 16 CTAs of 4 warps 10.0, at heads of 128 20.2 us and 8 of 4 14.6.
+// 16 wide CTAs from 2 pages a warp on where they do run at once (1 token at 16000, 16 on 1 of 64: 9.6 against 12.0 us with 8; 8 on 2 of
+// 128: 10.8 and 14.8; 16 on 1 of 128: 13.7 and 17.7; 32 on 8 of 64: 11.5 and 11.9).
+// Beyond 48 pages a warp of 8 CTAs the longest context decides, and shares as short as they get win over running at once (3 tokens at
+// 20480..65536, 32 on 8 of 64: 16 CTAs of 4 warps 36.5, 8 of 8 40.4 us; 2 at 65536: 16 of 8 34.2, 8 of 8 40.2; 12 at 1250..50000, 8 on 2
+// of 128: 45.0 with 16 of 4).  Not known to the host, and so not in the rule, is how unequal the contexts of a batch are: over 399
+// batches of four layouts, 1 to 128 tokens at 300..65536, it is 5 % from the best form where contexts are alike and 7 % where they are
+// spread from 1/40 on, 56 % at worst (64 tokens at 4000, 16 on 1 of 64: 22.2 us in clusters of 8, 14.2 in clusters of 2 wide ones).
 template <uint32_t DIM, uint32_t HEADS>
 E4m3DecodePlan plan_heads(const DecodeWork& work, bool clusters_of_16) {
     using S = Shape<DIM, HEADS, 4>;
     constexpr uint64_t kSms = 148;
-    constexpr uint64_t kResident = kSms * S::kPerSm;
-    const uint32_t most = clusters_of_16 ? 4 : 3;
+    constexpr uint64_t kSlots = kSms * S::kPerSm;
+    constexpr auto& kNarrow = kResidentClusters[S::kPerSm - 1];
+    constexpr auto& kWide = kResidentClusters[Shape<DIM, HEADS, 8>::kPerSm - 1];
+    const bool long_contexts = work.pages >= 48 * 8 * 8;
+    auto wide_fits = [&](uint32_t splits_log2) {
+        return long_contexts ? (work.items << splits_log2) * 8 <= kSms * S::kWarpsPerSm : work.items <= kWide[splits_log2];
+    };
+    if (clusters_of_16 && !long_contexts && work.pages >= 2 * 8 * 16 && wide_fits(4)) {
+        return {8, 4};
+    }
+    const uint32_t most = clusters_of_16 && (long_contexts || work.items <= kNarrow[4]) ? 4 : 3;
     E4m3DecodePlan plan = {4, 0};
-    while (plan.splits_log2 < most && (work.items << (plan.splits_log2 + 1)) <= kResident + kResident / 4 &&
+    while (plan.splits_log2 < most && (work.items << (plan.splits_log2 + 1)) <= kSlots + kSlots / 4 &&
            work.pages >= (8ull * 4 << plan.splits_log2)) {
         ++plan.splits_log2;
     }
-    auto wide_fits = [&](uint32_t splits_log2) { return (work.items << splits_log2) * 8 <= kSms * S::kWarpsPerSm; };
-    if (plan.splits_log2 == 4 && wide_fits(3) && work.pages < 48 * 8 * 8) plan.splits_log2 = 3;
+    if (plan.splits_log2 == 4 && !long_contexts && wide_fits(3)) plan.splits_log2 = 3;
     if (wide_fits(plan.splits_log2)) plan.warps = 8;
     return plan;
 }

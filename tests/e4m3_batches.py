@@ -25,12 +25,12 @@ def plan(tokens, heads, kv_heads, dim, longest, window=0, sinks=0, clusters_of_1
 # (heads, KV heads, dimensions) -> (warps, CTAs of a cluster) -> (tokens, longest context)
 BATCHES = {
     (32, 8, 64): {(4, 1): (48, 40), (4, 2): (20, 600), (4, 4): (12, 1100), (4, 8): (6, 2100), (4, 16): (3, 65536), (8, 1): (5, 300),
-                  (8, 2): (3, 600), (8, 4): (3, 1100), (8, 8): (2, 4200), (8, 16): (1, 65536)},
-    (16, 1, 64): {(4, 1): (300, 40), (4, 2): (128, 600), (4, 4): (64, 1100), (4, 8): (32, 2100), (4, 16): (32, 4200), (8, 1): (5, 300),
-                  (8, 2): (3, 600), (8, 4): (3, 1100), (8, 8): (2, 4200), (8, 16): (3, 65536)},
-    (8, 2, 128): {(4, 1): (128, 40), (4, 2): (64, 600), (4, 4): (32, 1100), (4, 8): (16, 2100), (4, 16): (16, 4200), (8, 1): (5, 300),
-                  (8, 2): (3, 600), (8, 4): (3, 1100), (8, 8): (2, 4200), (8, 16): (2, 65536)},
-    (16, 1, 128): {(4, 1): (160, 40), (4, 2): (80, 600), (4, 4): (40, 1100), (4, 8): (20, 2100), (4, 16): (20, 4200), (8, 1): (5, 300),
-                   (8, 2): (3, 600), (8, 4): (3, 1100), (8, 8): (2, 4200), (8, 16): (2, 65536)},
+                  (8, 2): (3, 600), (8, 4): (3, 1100), (8, 8): (3, 4200), (8, 16): (1, 65536)},
+    (16, 1, 64): {(4, 1): (300, 40), (4, 2): (128, 600), (4, 4): (64, 1100), (4, 8): (32, 2100), (4, 16): (20, 4200), (8, 1): (5, 300),
+                  (8, 2): (3, 600), (8, 4): (3, 1100), (8, 8): (12, 4200), (8, 16): (3, 6000)},
+    (8, 2, 128): {(4, 1): (128, 40), (4, 2): (64, 600), (4, 4): (32, 1100), (4, 8): (16, 2100), (4, 16): (10, 4200), (8, 1): (5, 300),
+                  (8, 2): (3, 600), (8, 4): (3, 1100), (8, 8): (6, 4200), (8, 16): (2, 65536)},
+    (16, 1, 128): {(4, 1): (160, 40), (4, 2): (80, 600), (4, 4): (40, 1100), (4, 8): (20, 2100), (4, 16): (12, 65536), (8, 1): (5, 300),
+                   (8, 2): (3, 600), (8, 4): (3, 1100), (8, 8): (12, 4200), (8, 16): (2, 6000)},
 }
 ALL = [(layout, form, *batch) for layout, forms in BATCHES.items() for form, batch in forms.items()]

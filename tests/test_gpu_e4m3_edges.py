@@ -183,7 +183,7 @@ def test_decode_attention_in_every_form(device, layout, form, tokens, longest, w
     most = longest + (longest // 3 if windowed else 0)
     assert plan(tokens, *layout, most, window, sinks) == form
     rng = np.random.default_rng(tokens * dim + longest)
-    contexts = tuple(int(c) for c in rng.integers(1, most + 1, tokens - 1)) + (most,)
+    contexts = tuple(int(c) for c in rng.integers(1, min(most, 6000) + 1, tokens - 1)) + (most,)
     pool = pool_of(contexts)
     arena, *cache = random_cache(rng, pool, kv_heads, dim, device)
     tables = tables_of(rng, contexts, pool)
