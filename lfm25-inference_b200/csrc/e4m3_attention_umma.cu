@@ -1056,18 +1056,24 @@ cudaError_t launch_e4m3_prompt_attention(cudaStream_t stream, const E4m3Attentio
     params.scale_log2 = launch.scale * kLog2e;
     params.wait_limit_ns = wait_limit_ns();
     params.selftest_drop = wait_selftest_drop() ? 1 : 0;
-    // at most so many tiles: full ones, and one that is not for each segment
-    const uint64_t tiles = launch.num_tokens / params.cta_tokens + launch.num_segments;
+    // at most so many tiles, by how the tokens lie in the segments: a segment's first token is one, and cta_tokens more each is another
+    const uint64_t tiles = launch.num_segments < launch.num_tokens
+                               ? (launch.num_tokens - launch.num_segments) / params.cta_tokens + launch.num_segments : launch.num_segments;
     const uint64_t items = tiles * launch.cache.kv_heads * params.chunks;
     uint64_t longest = launch.maximum_context_tokens;
     if (launch.window != 0 && longest > static_cast<uint64_t>(launch.window) + launch.sinks + params.cta_tokens) {
         longest = static_cast<uint64_t>(launch.window) + launch.sinks + params.cta_tokens;
     }
-    // Shares of the keys as long as all CTAs run at once and each has a few stages (with one set of softmax warps: 37 tokens behind
-    // 8000, 8 KV heads: 1 share 152, 2 84, 4 49, 8 32.6 us; 64 behind 500: 18.8, 17.7, 15.5, 16.7; 64 behind 200: 13.6, 15.2;
-    // 2 x 64 behind 4000, where 8 shares are 256 CTAs: 4 shares 31.4, 8 44.9).
-    params.splits = 1;
-    while (params.splits < 8 && items * params.splits * 2 <= 148 && longest >= (2 * params.splits + 4) * kKeys) params.splits *= 2;
+    // Shares of the keys as long as all CTAs run at once, one an SM, and each has a few stages.  A B200 holds 74, 33 and 15 clusters of 2,
+    // 4 and 8 such CTAs, and those that find no room cost their whole time again.  32 heads on 8 of 64: 37 tokens behind 8000 126 us whole,
+    // 2 shares 71, 4 41, 8 26.9; 2 x 64 behind 4000 (16 clusters) 8 shares 38.5, 4 26.7; 64 behind 500 1 16.6, 4 14.4, 8 15.6; 64 behind
+    // 200 1 12.5, 2 14.9, 4 13.2; 512 behind 2000 1 46.3, 2 32.3, 4 42.2.  8 heads on 2 of 128: 37 behind 8000 153, 92, 53, 33.0; 512 behind
+    // 2000 (16 clusters) 8 shares 41.0, 4 28.6; 64 behind 500 1 20.2, 4 19.4, 8 17.5; 64 behind 200 1 15.1, 8 16.5.  (Short segments count
+    // for more tiles than they are: 4 x 64 behind 2000, 32 on 8 of 64, take 2 shares and 28.8 us, 4 would take 22.1.)
+    constexpr uint32_t kResidentClusters[4] = {148, 74, 33, 15};
+    uint32_t splits_log2 = 0;
+    while (splits_log2 < 3 && items <= kResidentClusters[splits_log2 + 1] && longest >= ((2u << splits_log2) + 4) * kKeys) ++splits_log2;
+    params.splits = 1u << splits_log2;
     const uint64_t blocks = items * params.splits;
     if (blocks > 0x7fffffffu) {
         return cudaErrorInvalidConfiguration;
