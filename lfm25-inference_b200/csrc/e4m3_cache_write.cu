@@ -323,10 +323,13 @@ cudaError_t launch_e4m3_cache_write(cudaStream_t stream, const E4m3WriteLaunch& 
     params.num_tokens = static_cast<uint32_t>(launch.num_tokens);
     params.query_heads = launch.query_heads;
     params.eps = launch.eps;
-    // A CTA of a prompt has one run or two, and a unit for each KV head of them: with fewer than 8 heads, 4 warps (8 prompts of 437 to 512
-    // with norms, 4 against 8 warps: 2 heads of 128 11.5 and 12.8 us, 4 of 128 26.2 and 28.1, 8 of 64 17.9 and 15.8; without norms
-    // 4.6 and 6.1, 5.1 and 6.6, 6.0 and 5.5).
-    const uint32_t warps = launch.cache.kv_heads < 8 ? 4 : 8;
+    // A CTA of a prompt has one run or two, and a unit for each KV head of them: with fewer than 8 heads, 4 warps (8 prompts of 437 to 512,
+    // 4 against 8 warps: 2 heads of 128 4.7 and 6.1 us, 4 of 128 5.2 and 6.6, 8 of 64 5.9 and 5.5; 200 tokens 3.3 and 3.5, 3.5 and
+    // 3.7, 3.8 and 3.1; 128 single tokens 3.0 and 3.0, 3.2 and 3.0, 3.8 and 3.1).  With norms a CTA computes its angles first, for which 8 warps
+    // are better until many CTAs share an SM (8 query heads on 2 of 128: 200 tokens 6.5 and 5.8 us, 600 6.5 and 6.3, 2400 9.4 and
+    // 8.9, 3800 11.6 and 12.7; 16 on 4 of 128: 6.9 and 5.8, 7.2 and 6.7, 12.5 and 11.7, 18.2 and 19.9; 32 on 2 of 64: 4.7 and 4.0, 4.9
+    // and 4.7, 7.9 and 8.0, 11.8 and 12.7; 128 single tokens the same to 0.2 us).
+    const uint32_t warps = launch.cache.kv_heads < 8 && (launch.query == nullptr || launch.num_tokens >= 8 * 2 * 148) ? 4 : 8;
     // Tokens of a CTA that looks for runs: as many as leave 2 CTAs an SM with keys and 2 with values.  A decode step's tokens
     // then run side by side, and the tokens of a long prompt share the search (3800 tokens: 8 to a CTA 16.0 us, 4 to a CTA 17.3 us;
     // 700 tokens: 2 to a CTA 8.3 us, 1 to a CTA 9.3 us).
