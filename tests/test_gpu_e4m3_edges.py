@@ -170,6 +170,35 @@ def test_append_to_pages_whose_scale_is_no_power_of_two(device, dim):
                 assert np.array_equal(got[offset], plain.round_e4m3(host(rows)[page, head] / scale))
 
 
+@pytest.mark.parametrize("heads,kv_heads,dim,tokens,first", [
+    (32, 8, 64, 1, 0), (32, 8, 64, 128, 77), (8, 2, 128, 40, 9), (12, 4, 64, 700, 100000), (5, 1, 128, 3, 2 ** 31), (8, 2, 128, 2400, 5),
+    (12, 4, 64, 2401, 16384)])
+def test_keys_are_rounded_once_behind_norm_and_rotation(device, heads, kv_heads, dim, tokens, first):
+    """A key is off by half a step of E4M3 and by what f32 is off in front of it (dim squares and a handful of products, an angle of
+    2^-22): nothing that a call brings is rounded a second time, since a page takes one run a call.  Few tokens and so many that CTAs
+    of four warps take them."""
+    rng = np.random.default_rng(tokens + dim)
+    pages = -(-tokens // PAGE) + 1
+    arena, *_ = random_cache(rng, pages, kv_heads, dim, device, low=-14, high=-12)
+    slots = np.arange(tokens, dtype=np.int64) + 3
+    positions = np.arange(first, first + tokens, dtype=np.uint32)
+    query, key, value = (bf16(rng.standard_normal((tokens, n, dim)), device) for n in (heads, kv_heads, kv_heads))
+    weights = [bf16(1 + 0.3 * rng.standard_normal(dim), device) for _ in range(2)]
+    inv_freq = torch.from_numpy((1e6 ** (-np.arange(0, dim, 2) / dim)).astype(np.float32)).to(device)
+    out = torch.empty_like(query)
+    ops.qk_norm_rope_kv_write_e4m3(query, key, value, *weights, inv_freq, to_u32(positions, device), to_i64(slots, device), arena, 1e-5,
+                                   query_out=out)
+    half = dim // 2
+    slack = lambda x: (dim / 2 + 16) * 2.0 ** -23 * (np.abs(x) + np.abs(np.concatenate((x[:, :, half:], x[:, :, :half]), axis=2)))  # noqa: E731
+    want = plain.norm_rope(host(query), host(weights[0]), inv_freq.cpu().numpy(), positions, 1e-5)
+    assert np.all(np.abs(host(out) - want) <= 2.0 ** -8 * np.abs(want) + (1 + 2.0 ** -8) * slack(want))
+    want = plain.norm_rope(host(key), host(weights[1]), inv_freq.cpu().numpy(), positions, 1e-5)
+    scales = arena.key_scales.cpu().numpy().astype(np.float64)[slots // PAGE]
+    got = plain.CODE_VALUES[arena.key.cpu().numpy()][slots // PAGE, :, slots % PAGE] * scales[:, :, None]
+    bound = np.maximum(2.0 ** -4 * np.abs(want), 2.0 ** -10 * scales[:, :, None]) + 2 * slack(want)
+    assert np.all(np.abs(got - want) <= bound)
+
+
 # ------------------------------------------------------------------------------------------------ forms of the kernel
 
 
