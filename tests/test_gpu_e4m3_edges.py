@@ -1,4 +1,5 @@
-"""The 8-bit paged cache at the ends of its number formats, and single tokens in every form of the kernel."""
+"""The 8-bit paged cache at the ends of its number formats, single tokens in every form of the kernel, many segments, and
+page copies between other words."""
 import numpy as np
 import pytest
 import torch
@@ -225,3 +226,57 @@ def test_decode_attention_in_every_form(device, layout, form, tokens, longest, w
     assert not out.isnan().any()
     some = np.unique(np.concatenate(([np.argmax(positions)], rng.integers(0, tokens, 6))))
     check_attention(out[some], query[some], cache, tables, order[some], positions[some], F16_WEIGHTS, out[some], window=window, sinks=sinks)
+
+
+# ------------------------------------------------------------------------------------------------ segments
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim", [(32, 8, 64), (8, 2, 128), (35, 1, 64)])
+@pytest.mark.parametrize("count,window", [(33, 0), (64, 20), (101, 0)])
+def test_prompt_attention_of_many_segments(device, heads, kv_heads, dim, count, window):
+    """Tiles are found in blocks of 32 segments: short ones of unequal lengths, empty ones between them and at the ends of the blocks,
+    some of two tiles or more, one that takes the place of a whole block's tiles, and tokens of nobody around all."""
+    rng = np.random.default_rng(count + dim)
+    lengths = rng.integers(1, 12, count)
+    lengths[[5, 31, 32]] = 0
+    lengths[rng.integers(0, count, count // 8)] = 0
+    lengths[[0, 17, count - 1]] = 97, 140, 70
+    if count > 64:
+        lengths[[33, 63, 64, 90]] = 130, 0, 0, 66
+    prefixes = rng.integers(0, 60, count)
+    contexts = tuple(int(c) for c in np.maximum(prefixes + lengths, 1))
+    pool = pool_of(contexts)
+    arena, *cache = random_cache(rng, pool, kv_heads, dim, device)
+    tables = tables_of(rng, contexts, pool)
+    lead, tail = 4, 5
+    rows = np.concatenate((np.zeros(lead, dtype=np.int64), np.repeat(np.arange(count), lengths), np.zeros(tail, dtype=np.int64)))
+    positions = np.concatenate([np.zeros(lead, dtype=np.int64)] + [np.arange(p, p + n) for p, n in zip(prefixes, lengths)] +
+                               [np.zeros(tail, dtype=np.int64)])
+    offsets = lead + np.concatenate(([0], np.cumsum(lengths)))
+    query = bf16(rng.standard_normal((len(rows), heads, dim)) * 0.5, device)
+    out = bf16(rng.standard_normal(query.shape), device)
+    before = out.clone()
+    ops.paged_prompt_attention_e4m3_into(query, arena, to_u32(tables, device), to_u32(rows, device), to_u32(positions, device),
+                                         to_u32(offsets, device), out, window=window)
+    assert torch.equal(out[:lead], before[:lead]) and torch.equal(out[-tail:], before[-tail:])
+    inside = slice(lead, len(rows) - tail)
+    check_attention(out[inside], query[inside], cache, tables, rows[inside], positions[inside], BF16_WEIGHTS, before[inside], window=window)
+
+
+# ------------------------------------------------------------------------------------------------ pages
+
+
+@pytest.mark.parametrize("words", [1, 3, 4, 8, 33, 512, 2048, 5000])
+@pytest.mark.parametrize("front", [1, 4])
+def test_page_copies_stay_within_their_arena(device, words, front):
+    """Words in front of each arena and behind it, on a 16-byte boundary and off one, and all pages that are no destination stay as they
+    were; the first page and the last one are among those copied."""
+    pages, source, destination = 40, [38, 20, 5, 39], [1, 21, 0, 7]
+    buffers = [torch.arange(front + pages * words + 5, device=device, dtype=torch.int32) * 7 + index for index in range(3)]
+    arenas = [buffer[front:front + pages * words].view(pages, words) for buffer in buffers]
+    wants = [buffer.clone() for buffer in buffers]
+    for want in wants:
+        inner = want[front:front + pages * words].view(pages, words)
+        inner[destination] = inner[source]
+    ops.kv_pages_copy(arenas, to_u32(source, device), to_u32(destination, device))
+    assert all(torch.equal(buffer, want) for buffer, want in zip(buffers, wants))
