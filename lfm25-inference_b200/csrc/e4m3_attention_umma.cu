@@ -548,8 +548,10 @@ e4m3_prompt_attention_kernel(const PromptParams p) {
         // -------------------------------------------------------------------------------- MMA issuers, one for each tile
         const uint32_t which = warp - (kSoftmaxWarps + kPageWarps);
         tmem = meet();
-        // The warp stays together: all lanes wait, one of them issues.  A lane that runs the whole loop by itself is 2 us faster over
-        // eight portions of 512, but builds of that now and then ended in an illegal address while the other lanes came late.
+        // The warp stays together: all lanes wait, one of them issues, and none runs ahead of the others.  (Two builds in which one lane
+        // ran the whole loop by itself ended in an illegal address now and then, in their first launches.  The cause is not known: that
+        // form is legal, other kernels have it, reading found no access out of range in it, and keeping the warp together may have
+        // changed no more than the timing.  It costs 2 us over eight portions of 512.)
         // f32 results of 128 rows; Q K^T: f16, both K-major, 64 keys; P V: bf16, V MN-major, 64 dimensions
         constexpr uint32_t idesc_scores = (1u << 4) | ((kKeys >> 3) << 17) | ((kRows >> 4) << 24);
         constexpr uint32_t idesc_product = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((64u >> 3) << 17) | ((kRows >> 4) << 24);
@@ -845,6 +847,9 @@ e4m3_prompt_attention_kernel(const PromptParams p) {
                                 w.x = (bits[half] >> j) & 1 ? w.x : 0.0f;
                                 w.y = (bits[half] >> (j + 1)) & 1 ? w.y : 0.0f;
                             }
+                            // 8 bits, since both operands of the product have one type and values with their page's scale need
+                            // bf16's range: 2^-9 a weight on average, which over many keys leaves 0.0021 to 0.0023 of the result
+                            // (root of mean squares, the result's own rounding to bf16 among it) instead of 0.0016
                             packed[sub * 8 + pair] = pack_bf16x2(w.x, w.y);
                             part_sum[pair & 1] = pair_add(part_sum[pair & 1], pair_of(w.x, w.y));   // unrounded: roundings average out
                         }

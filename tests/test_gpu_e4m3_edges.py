@@ -263,6 +263,24 @@ def test_prompt_attention_of_many_segments(device, heads, kv_heads, dim, count, 
     check_attention(out[inside], query[inside], cache, tables, rows[inside], positions[inside], BF16_WEIGHTS, before[inside], window=window)
 
 
+@pytest.mark.parametrize("heads,kv_heads,dim", [(32, 8, 64), (8, 2, 128)])
+def test_prompt_attention_whose_shares_are_empty(device, heads, kv_heads, dim):
+    """Block tables far wider than the contexts, and nothing said about these: eight CTAs share the keys of a tile that has one stage or
+    a few, and most have none."""
+    rng = np.random.default_rng(dim)
+    contexts = (70, 9)
+    pool = pool_of(contexts)
+    arena, *cache = random_cache(rng, pool, kv_heads, dim, device)
+    tables = tables_of(rng, contexts, pool, spare_columns=300)
+    rows, positions = np.repeat([0, 1], 9), np.concatenate((np.arange(61, 70), np.arange(9)))
+    query = bf16(rng.standard_normal((18, heads, dim)), device)
+    for longest in (0, 70):
+        out = torch.full_like(query, float("nan"))
+        ops.paged_prompt_attention_e4m3_into(query, arena, to_u32(tables, device), to_u32(rows, device), to_u32(positions, device),
+                                             to_u32([0, 9, 18], device), out, maximum_context_tokens=longest)
+        check_attention(out, query, cache, tables, rows, positions, BF16_WEIGHTS, out)
+
+
 # ------------------------------------------------------------------------------------------------ pages
 
 
