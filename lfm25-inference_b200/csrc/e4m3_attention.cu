@@ -25,7 +25,7 @@
 // headroom of 8 the step was 2^-24: a first token that takes nearly all left nothing of the others.  Both take the same time: 128 tokens
 // at contexts 128..4096 49.7 us, 3 at 20480..65536 36.7 against 36.4.)
 //
-// Without its arithmetic the kernel streams at the copy peak (128 tokens at contexts 128..4096: 43.3 us); with it 50.2, bound by the
+// Without its arithmetic the kernel streams at the copy peak (128 tokens at contexts 128..4096: 43.3 us); with it 49.7, bound by the
 // instructions of a page: about 180, 40 of them conversions.  K by the 8-bit MMA instead (its operands as they are, the query in two
 // parts) took as long: that instruction unpacks to f16 itself.
 //

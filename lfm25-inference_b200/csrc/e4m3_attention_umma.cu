@@ -17,11 +17,11 @@
 // only then is O read, scaled and stored.  The query is brought to f16 by a power of two per row, which the scores get back
 // together with the page's scale in the multiply-add in front of the exponential.
 //
-// Eight portions of 512 tokens at depths of 0 to 3584, 32 heads on 8 of 64: 142 us, 0.49 PFLOP/s, where the exponentials alone (16 a
-// cycle and SM) need 60.  What bounds it is the chain of a stage through its roles, 1900 cycles: no unit is busy for much more than
-// half of that, page warps as long as softmax warps, and 11,000 cycles go to the ends of a CTA.  One set of softmax warps takes 156 us (166
-// with codes in registers one stage ahead); without its exponentials the kernel takes 139, without conversions 146, without both 133.
-// Eight page warps leave 72 registers a thread: 146 us.
+// Eight portions of 512 tokens at depths of 0 to 3584, 32 heads on 8 of 64: 140 us, 0.49 PFLOP/s, where the exponentials alone (16 a
+// cycle and SM) need 60.  What bounds it is the chain of a stage through its roles, 1.0 us or 1950 cycles (1.27 us at heads of 128, one
+// set): no unit is busy for much more than half of that, page warps as long as softmax warps, and 11,000 cycles go to the ends of a CTA.
+// 22 warps leave 80 registers a thread, and 72 bytes of each spill.  Measured while it took 142 us: one set of softmax warps 156 (166 with
+// codes in registers one stage ahead), without exponentials 139, without conversions 146, without both 133, eight page warps 146.
 //
 // Rows of a mask edge test bits of their own; a NaN among the values is replaced in the operand (a weight of 0 times NaN is
 // NaN) and remembered by key: a row that sees it becomes NaN as a whole.  Few tiles: a cluster shares a tile's keys and joins

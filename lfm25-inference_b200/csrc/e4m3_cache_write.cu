@@ -7,9 +7,10 @@
 // that they are rotated with, so that a row of 64 takes 8 lanes, a warp 4 rows at a time, and a rotation no exchange.  The run
 // finds itself: every warp looks at the slots of the tokens around its own.
 //
-// The kernel is bound by chains of dependent loads (slots -> values and old scale -> maximum -> codes) in a decode step (128 tokens
-// with norms 3.7 us), and by its instructions over long prompts: 3800 tokens with 32 query heads on 8 of 64 move 43 MB in 16.0 us
-// (2.7 TB/s), without norms 12 MB in 5.4 us.  Queries, keys and values have CTAs of their own: queries do not wait for slots, values not for
+// The kernel is bound by chains of dependent loads (slots -> values and old scale -> maximum -> codes): in a decode step (128 tokens
+// with norms 3.8 us), and over long prompts as well, where 80 registers a thread leave few warps to hide them: 3800 tokens with 32 query
+// heads on 8 of 64 move 43 MB in 15.9 us (2.7 TB/s; 52 % of the issue slots used, 35 % of the ALU, 34 % of the places for warps), without
+// norms 12 MB in 5.3 us.  Queries, keys and values have CTAs of their own: queries do not wait for slots, values not for
 // angles, and all loads of a CTA are under way while it computes its angles.
 //
 // Arithmetic: everything in f32.  With norms, x / sqrt(mean(x^2) + eps) * w is rotated by position * inv_freq[d] in the
