@@ -40,6 +40,7 @@
 #include "kernels.h"
 #include "launch.h"
 #include "options.h"
+#include "ring.h"
 #include "tcgen05.cuh"
 #include "tensor_map.h"
 
@@ -357,7 +358,7 @@ gemm_rows_umma_kernel(const __grid_constant__ CUtensorMap weight_map, const __gr
                     umma_rows<BF16>(second, a_desc_second + 4, b_desc + 4, idesc, 1u);
                     umma_rows<BF16>(second, a_desc_second + 6, b_desc + 6, idesc, 1u);
                 }
-                umma_commit(bar_empty + 8 * stage);
+                if (filled_again(block, k_count, p.stages)) umma_commit(bar_empty + 8 * stage);
                 accumulate = 1;
                 stage += p.issuers;
                 slot += slot_step;
