@@ -34,6 +34,7 @@
 #include "kernels.h"
 #include "launch.h"
 #include "options.h"
+#include "ring.h"
 #include "tcgen05.cuh"
 #include "tensor_map.h"
 
@@ -283,7 +284,7 @@ gemm_umma_kernel(const __grid_constant__ CUtensorMap weight_map, const __grid_co
                 umma<BF16>(accumulator, a_desc + 2, b_desc + 2, idesc, 1u);
                 umma<BF16>(accumulator, a_desc + 4, b_desc + 4, idesc, 1u);
                 umma<BF16>(accumulator, a_desc + 6, b_desc + 6, idesc, 1u);
-                umma_commit(bar_empty + 8 * stage);
+                if (filled_again(block, k_count, p.stages)) umma_commit(bar_empty + 8 * stage);
                 accumulate = 1;
                 stage += p.issuers;
                 slot += slot_step;

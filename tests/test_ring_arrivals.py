@@ -63,7 +63,7 @@ def test_a_buffer_is_reported_free_as_often_as_it_is_filled_again(tmp_path):
     assert ran.returncode == 0 and ran.stdout.strip() == "ok", ran.stdout
 
 
-@pytest.mark.parametrize("name", ["stack_attention_umma.cu", "hybrid_attention_umma.cu", "stack_latent_decode.cu", "e4m3_attention_umma.cu", "gemm_rows_umma.cu"])
+@pytest.mark.parametrize("name", ["stack_attention_umma.cu", "hybrid_attention_umma.cu", "stack_latent_decode.cu", "e4m3_attention_umma.cu", "gemm_rows_umma.cu", "fp8_gemm_umma.cu"])
 def test_kernels_ask_for_arrivals_that_are_waited_for(name):
     with open(os.path.join(CSRC, name)) as handle:
         commits = [line.strip() for line in handle if re.search(r"umma_commit\(bar_empty", line)]
