@@ -89,3 +89,11 @@ def test_every_product_of_the_latent_decode_attention_is_waited_for():
     assert re.search(r"if \(index >= 2\) \{\s*ok = mbar_wait_bounded\(bar_product \+ 8 \* buffer", source)
     end = source[source.index("const uint32_t last = count - 1;"):]
     assert re.search(r"bar_product \+ 8 \* \(\(last - 1\) & 1\)", end) and re.search(r"bar_product \+ 8 \* \(last & 1\)", end)
+
+
+def test_every_block_of_the_f32_product_is_waited_for():
+    """Pairs of blocks: the adding warps wait for the later one, and for the earlier one where its slot is not filled again."""
+    with open(os.path.join(CSRC, "linear_f32.cu")) as handle:
+        source = handle.read()
+    adding = source[source.index("MMAs are complete in the order of the blocks"):]
+    assert re.search(r"if \(both && !filled_again\(first, blocks, S::kStages\)\) \{\s*ok = ok && mbar_wait_bounded\(bar_read", adding)
