@@ -42,7 +42,6 @@
 
 #include "kernels.h"
 #include "launch.h"
-#include "ring.h"
 #include "stack_common.cuh"
 #include "tcgen05.cuh"
 #include "tensor_map.h"
@@ -290,6 +289,12 @@ linear_f32_umma_kernel(const __grid_constant__ CUtensorMap weight_map, const Lin
                 }
             }
             store_shared(progress + offsetof(Progress, multiplied), block);
+            // Arrivals come by themselves, and nobody leaves before they do: the producer and the converting warps wait for those whose
+            // slot is filled again, the adding warps for the later block of each pair.  The rest are waited for here.
+            const uint32_t unfilled = blocks > S::kStages ? blocks - S::kStages : 0;
+            for (uint32_t first = (unfilled + 1) & ~1u; block == blocks && first + 1 < blocks; first += 2) {
+                (void)mbar_wait_bounded(bar_read + 8 * (first % S::kStages), first / S::kStages & 1, p.wait_limit);
+            }
         }
         __syncwarp();
     } else if (warp < kFirstAdder) {
@@ -354,14 +359,7 @@ linear_f32_umma_kernel(const __grid_constant__ CUtensorMap weight_map, const Lin
             // MMAs are complete in the order of the blocks: the pair's last one speaks for both
             const bool both = pair * 2 + 1 < blocks;
             const uint32_t last = pair * 2 + (both ? 1 : 0);
-            ok = mbar_wait_bounded(bar_read + 8 * (last % S::kStages), last / S::kStages & 1, p.wait_limit);
-            // The arrival of the first one comes by itself, and nobody leaves before it does: where the slot is not filled again the
-            // producer and the converting warps do not wait for it.
-            const uint32_t first = pair * 2;
-            if (both && !filled_again(first, blocks, S::kStages)) {
-                ok = ok && mbar_wait_bounded(bar_read + 8 * (first % S::kStages), first / S::kStages & 1, p.wait_limit);
-            }
-            ok = __all_sync(0xffffffffu, ok);
+            ok = __all_sync(0xffffffffu, mbar_wait_bounded(bar_read + 8 * (last % S::kStages), last / S::kStages & 1, p.wait_limit));
             if (!ok) break;
             tcgen05_fence_after();
             const uint32_t source = address + (pair & 1) * 2 * N;

@@ -92,8 +92,17 @@ def test_every_product_of_the_latent_decode_attention_is_waited_for():
 
 
 def test_every_block_of_the_f32_product_is_waited_for():
-    """Pairs of blocks: the adding warps wait for the later one, and for the earlier one where its slot is not filled again."""
+    """Waited for are: by the producer blocks whose slot is filled again, by the adding warps the later block of each pair, by the issuing
+    lane the earlier ones of the pairs that are left."""
     with open(os.path.join(CSRC, "linear_f32.cu")) as handle:
         source = handle.read()
-    adding = source[source.index("MMAs are complete in the order of the blocks"):]
-    assert re.search(r"if \(both && !filled_again\(first, blocks, S::kStages\)\) \{\s*ok = ok && mbar_wait_bounded\(bar_read", adding)
+    issuing = source[source.index("umma_commit(bar_read"):source.index("} else if (warp < kFirstAdder)")]
+    assert "unfilled = blocks > S::kStages ? blocks - S::kStages : 0;" in issuing
+    assert re.search(r"first = \(unfilled \+ 1\) & ~1u; block == blocks && first \+ 1 < blocks; first \+= 2\) \{\s*\(void\)mbar_wait_bounded\(bar_read",
+                     issuing)
+    for stages in (3, 4, 5):
+        for blocks in range(1, 40):
+            unfilled = max(blocks - stages, 0)
+            waited = set(range(unfilled)) | {min(pair + 1, blocks - 1) for pair in range(0, blocks, 2)}
+            waited |= set(range((unfilled + 1) & ~1, blocks - 1, 2))
+            assert waited == set(range(blocks)), (blocks, stages)
